@@ -190,7 +190,15 @@ unsigned long long lmc_rng_seed(unsigned long long seed);
  * row's fp32 scale (LMC_KV_Q8: value = code * scale; a new row is quantized
  * with m = max|x|, code = clamp(rint(x * (127 / m)), +-127), scale = m / 127;
  * Dh + 16 bytes per row, head sizes that are multiples of 16 up to 512;
- * LMC_KV_ROW_BYTES gives the row size).  For `batch` sequences
+ * LMC_KV_ROW_BYTES gives the row size), or Dh 4-bit codes (LMC_KV_Q4): Dh / 2
+ * bytes with dim 2 i in the low half of byte i and dim 2 i + 1 in its high
+ * half, then for each group of 64 dims (the last has 32 when Dh % 64 is 32)
+ * two fp16 numbers d, m; value = d * code + m.  A new row's group is
+ * quantized with m = fp16(min), d = fp16((max - m) / 15) (fp32 steps; both
+ * saturate at +-65504) and the code in 0..15 nearest to (x - m) / d, ties to
+ * even (decided exactly; all 0 when d is 0).  A group with an infinity or a
+ * NaN gets d = NaN: its values read back as NaN.  Such caches start on a
+ * 16-byte boundary.  For `batch` sequences
  * the caches are batch consecutive [Hkv][S][Dh] slabs and q/k_new/v_new/out
  * are batch rows of H*Dh (q, out) and Hkv*Dh (k_new, v_new) floats.
  * d_pos[b] is the position written this step; positions 0..d_pos[b] are
@@ -201,8 +209,12 @@ unsigned long long lmc_rng_seed(unsigned long long seed);
 #define LMC_KV_F32 0
 #define LMC_KV_F16 1
 #define LMC_KV_Q8 2
-#define LMC_KV_ROW_BYTES(kv_dtype, Dh) \
-    ((kv_dtype) == LMC_KV_F32 ? 4 * (size_t)(Dh) : (kv_dtype) == LMC_KV_F16 ? 2 * (size_t)(Dh) : (size_t)(Dh) + 16)
+#define LMC_KV_Q4 3
+#define LMC_KV_ROW_BYTES(kv_dtype, Dh)                                                                \
+    ((kv_dtype) == LMC_KV_F32   ? 4 * (size_t)(Dh)                                                    \
+     : (kv_dtype) == LMC_KV_F16 ? 2 * (size_t)(Dh)                                                    \
+     : (kv_dtype) == LMC_KV_Q4  ? (size_t)(Dh) / 2 + 4 * (((size_t)(Dh) + 63) / 64)                   \
+                                : (size_t)(Dh) + 16)
 size_t lmc_attention_workspace_bytes(int batch, int H, int Dh, int S);
 int lmc_attention_decode(float *d_out, const float *d_q, const float *d_k_new,
                          const float *d_v_new, void *d_k_cache, void *d_v_cache,
@@ -247,6 +259,77 @@ int lmc_attention_decode_paged(float *d_out, const float *d_q, const float *d_k_
                                int page_size, const int *d_pos, int batch, int H, int Hkv,
                                int Dh, void *d_workspace, size_t workspace_bytes,
                                void *stream);
+/* K/V rows into a cache and back, for prompts whose rows are computed many
+ * at a time (lmc_attention_decode appends one row per sequence) and for
+ * callers that move or inspect a cache.  No counterpart in LMc, whose cache
+ * is a host fp32 array.  Row r (0 <= r < rows) belongs to position d_pos[r]
+ * of sequence d_seq[r] (d_seq NULL: sequence r); its K and V are Hkv * Dh
+ * floats at d_k + r * ld and d_v + r * ld (ld >= Hkv * Dh).  The cache is
+ * contiguous, [n_seqs][Hkv][S][row] (d_pages NULL; page_size and n_pages are
+ * not used), or paged as in lmc_attention_decode_paged with S / page_size
+ * table entries per sequence (S a multiple of page_size).  Any kv_dtype; Dh
+ * as in lmc_attention_decode; d_k and d_v NULL together are refused, one of
+ * them NULL leaves that side out (its cache may be NULL too).
+ * lmc_kv_append stores the rows in the cache's row form (the same bytes
+ * lmc_attention_decode writes); rows must name distinct positions.
+ * lmc_kv_read writes the values the cached rows stand for.  A row whose
+ * position is negative is padding: nothing is read or written for it.  A
+ * position >= S, a sequence outside [0, n_seqs) or a page outside
+ * [0, n_pages) is left out the same way, and lmc_device_status() then
+ * reports LMC_ERR_INVALID. */
+int lmc_kv_append(const float *d_k, const float *d_v, int ld, void *d_k_cache, void *d_v_cache, int kv_dtype,
+                  const int *d_seq, const int *d_pos, int rows, int n_seqs, int Hkv, int Dh, int S,
+                  const int *d_pages, int page_size, int n_pages, void *stream);
+int lmc_kv_read(float *d_k, float *d_v, int ld, const void *d_k_cache, const void *d_v_cache, int kv_dtype,
+                const int *d_seq, const int *d_pos, int rows, int n_seqs, int Hkv, int Dh, int S,
+                const int *d_pages, int page_size, int n_pages, void *stream);
+
+/* ---- pages of a paged cache ---------------------------------------------------
+ * Page bookkeeping on the device, for servers that run the op-level paged
+ * cache (lmc_attention_decode_paged) and want sequences to share pages:
+ * parallel samples of one prompt, beam search.  No counterpart in LMc.  The
+ * state is the page table d_pages [n_seqs][max_pages] (-1: no page) and the
+ * use counts d_refs [n_pages]: d_refs[p] is the number of table entries that
+ * name page p, 0 for a free page (the caller starts with both empty: entries
+ * -1, counts 0).  The same page id is used in every layer's K and V pool.
+ * All three calls change table and counts in place, in stream order, without
+ * host synchronization, so they can be captured in a graph.  An entry, parent
+ * or position outside its range is left as it is, and lmc_device_status()
+ * then reports LMC_ERR_INVALID.
+ *
+ * fork: sequence b becomes a copy of sequence d_parent[b] (all rows as they
+ * were before the call), sharing its pages; d_parent[b] == b leaves it as it
+ * is, -1 gives its pages back (entries -1).  So one call forks samples,
+ * reorders beams and frees finished sequences.  No page is copied here.
+ *
+ * reserve: makes position d_pos[b] of every sequence b writable (negative:
+ * nothing to do for b): an entry that is -1 gets a free page, and a page that
+ * other entries name too is copied to a free page of b's own, in every pool
+ * (copy-on-write; of the sequences that are about to write one page the last
+ * keeps it when no other entry names it).  Free pages are handed out lowest
+ * id first, in order of b.  When fewer are free than needed nothing changes
+ * and *d_short receives how many are missing (else 0).  Call it before the
+ * step that writes those positions.
+ *
+ * compact: moves the pages in use to the ids 0 .. *d_n_live - 1 (the i-th
+ * page in use above that range, in ascending order, to the i-th free id in
+ * it), in every pool, and renames them in table and counts, so the memory
+ * above can be given back.
+ *
+ * h_pools is a host array of n_pools device addresses (each layer's K pool
+ * and V pool; 16-byte aligned), read during the call; page_bytes = Hkv *
+ * page_size * LMC_KV_ROW_BYTES (a multiple of 16).  d_workspace holds
+ * lmc_kv_pages_workspace_bytes(n_seqs, n_pages) bytes, used until the call's
+ * work is done: calls that may overlap on the GPU need one each. */
+size_t lmc_kv_pages_workspace_bytes(int n_seqs, int n_pages);
+int lmc_kv_pages_fork(int *d_pages, int n_seqs, int max_pages, int *d_refs, int n_pages, const int *d_parent,
+                      void *stream);
+int lmc_kv_pages_reserve(void *const *h_pools, int n_pools, size_t page_bytes, int *d_pages, int n_seqs,
+                         int max_pages, int page_size, int *d_refs, int n_pages, const int *d_pos, int *d_short,
+                         void *d_workspace, size_t workspace_bytes, void *stream);
+int lmc_kv_pages_compact(void *const *h_pools, int n_pools, size_t page_bytes, int *d_pages, int n_seqs,
+                         int max_pages, int *d_refs, int n_pages, int *d_n_live, void *d_workspace,
+                         size_t workspace_bytes, void *stream);
 
 /* ---- whole model: load_model + model_forward on the device -------------------
  * lmc_model_load parses a GGUF v1-3 file the way load_model does

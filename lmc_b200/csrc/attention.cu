@@ -433,11 +433,13 @@ static int attention_impl(float *out, int ldo, const float *q, int ldq, const fl
                           int max_pages, int n_pages, cudaStream_t s) {
     if (!out || !q || !k_new || !v_new || !k_cache || !v_cache || !d_pos)
         return lmc_set_error(LMC_ERR_INVALID, "attention: null pointer");
-    if (batch <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Dh % 32 || Dh > 256 || S <= 0)
+    if (batch <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Dh <= 0 || Dh % 32 || Dh > 256 || S <= 0)
         return lmc_set_error(LMC_ERR_INVALID, "attention: H=%d Hkv=%d Dh=%d S=%d (need H%%Hkv==0, Dh%%32==0, Dh<=256)",
                              H, Hkv, Dh, S);
-    if (kv_dtype != LMC_KV_F32 && kv_dtype != LMC_KV_F16 && kv_dtype != LMC_KV_Q8)
+    if (kv_dtype != LMC_KV_F32 && kv_dtype != LMC_KV_F16 && kv_dtype != LMC_KV_Q8 && kv_dtype != LMC_KV_Q4)
         return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: kv dtype %d", kv_dtype);
+    if (kv_dtype == LMC_KV_Q4 && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15))
+        return lmc_set_error(LMC_ERR_INVALID, "attention: a cache of 4-bit rows must start on a 16-byte boundary");
     if (kv_dtype == LMC_KV_Q8 && (Dh % 16 || Dh > 512))
         return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: int8 rows need a head size that is a multiple of 16, <= 512");
     AttnArgs a;
@@ -457,6 +459,15 @@ static int attention_impl(float *out, int ldo, const float *q, int ldq, const fl
     if (need > ws_bytes || (need && !d_ws))
         return lmc_set_error(LMC_ERR_INVALID, "attention: workspace %zu bytes < %zu needed", ws_bytes, need);
     a.ws = (float *)d_ws;
+    if (kv_dtype == LMC_KV_Q4) {
+        if (d_seq) {  // rows share cache sequences: append every row's K/V first
+            const int rc = lmc_kv_append_launch(k_new, v_new, ldkv, ldkv, k_cache, v_cache, kv_dtype, d_seq, d_pos,
+                                                batch, 0, Hkv, Dh, S, pages, page_shift, max_pages, n_pages, rope_cos,
+                                                rope_sin, s);
+            if (rc != LMC_OK) return rc;
+        }
+        return lmc_attention_q4_launch(&a, batch, ws_bytes, s);
+    }
     const int G = H / Hkv;
     // tensor-core body: fp16 cache, head 64 / 128, 1-8 query heads per kv head
     // (LMC_ATTN_TC=0 selects the CUDA-core body; both give the same result)
@@ -590,8 +601,10 @@ extern "C" int lmc_attention_decode_noalloc(float *out, const float *q, const fl
     if (batch <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Dh <= 0 || Dh % 32 || Dh > 256 || S <= 0)
         return lmc_set_error(LMC_ERR_INVALID, "attention_noalloc: batch=%d H=%d Hkv=%d Dh=%d S=%d", batch, H, Hkv,
                              Dh, S);
-    if (kv_dtype != LMC_KV_F32 && kv_dtype != LMC_KV_F16 && kv_dtype != LMC_KV_Q8)
+    if (kv_dtype != LMC_KV_F32 && kv_dtype != LMC_KV_F16 && kv_dtype != LMC_KV_Q8 && kv_dtype != LMC_KV_Q4)
         return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention_noalloc: kv dtype %d", kv_dtype);
+    if (kv_dtype == LMC_KV_Q4 && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15))
+        return lmc_set_error(LMC_ERR_INVALID, "attention_noalloc: a cache of 4-bit rows must start on a 16-byte boundary");
     const size_t need = lmc_attention_workspace_bytes(batch, H, Dh, S);
     if (need > LMC_ATTN_STATIC_SCRATCH_BYTES)
         return lmc_set_error(LMC_ERR_INVALID,

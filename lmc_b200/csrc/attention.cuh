@@ -79,6 +79,7 @@ __device__ __forceinline__ void kv_q8_store_row(KvQ8 *row, const float *src, con
     if (lane == 0) *reinterpret_cast<float *>(q + Dh) = m / 127.0f;
 }
 
+}  // namespace
 struct AttnArgs {
     float *out;
     const float *q, *k_new, *v_new;
@@ -104,6 +105,7 @@ struct AttnArgs {
     const int *pages;
     int page_shift, max_pages, n_pages;
 };
+namespace {
 __device__ int g_attn_page_err;  // an out-of-range page id was met (lmc_device_status)
 
 // Row t of cache sequence cs, kv head kh in a paged pool (a.pages set):

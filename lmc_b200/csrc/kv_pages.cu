@@ -1,0 +1,330 @@
+// kv_pages.cu - page bookkeeping of a paged KV cache on the device
+// (lmc_kv_pages_fork, _reserve, _compact).
+//
+// The table and the counts are small (four bytes a page and entry), so the
+// plans run in one CTA (reserve, compact) or in column stripes (fork) and are
+// bound by latency; what costs bandwidth is copying pages, 2 x page_bytes x
+// pools for each, done by one kernel for all pools of a call from the list of
+// page pairs that the plan left in the workspace.
+#include "lmc_common.cuh"
+#include "lmc_internal.h"
+
+namespace {
+
+__device__ int g_kv_pages_err;  // an index outside its range was met (lmc_device_status)
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int MAX_POOLS = 256;  // pool addresses passed in one launch (2 KiB of parameters)
+
+// Workspace: [0] pages to copy, then from WS_LIST on pairs (source, destination),
+// then arrays of the plan.
+constexpr int WS_LIST = 16;
+
+struct Pools {
+    uint4 *p[MAX_POOLS];
+};
+
+// Exclusive prefix sum of v over the CTA's 1024 threads; *total gets the sum.
+// `part` holds 33 ints.
+__device__ __forceinline__ int block_scan(int v, int *part, int *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();  // part's last use
+    if (lane == 31) part[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int p = part[lane], s = p;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += y;
+        }
+        part[lane] = s - p;
+        if (lane == 31) part[32] = s;
+    }
+    __syncthreads();
+    *total = part[32];
+    return part[warp] + x - v;
+}
+
+// Column stripe of the table: every row's entries of C columns are read
+// before any is written, so parents may be any mapping.
+__global__ void __launch_bounds__(256) k_pages_fork(int *pages, int n_seqs, int max_pages, int *refs, int n_pages,
+                                                    const int *parent, int C) {
+    extern __shared__ int tile[];  // [n_seqs][C]
+    pdl_wait();
+    pdl_launch_dependents();
+    const int c0 = blockIdx.x * C, nc = min(C, max_pages - c0);
+    for (int i = threadIdx.x; i < n_seqs * C; i += 256) {
+        const int b = i / C, j = i % C;
+        if (j < nc) tile[i] = pages[(size_t)b * max_pages + c0 + j];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_seqs * C; i += 256) {
+        const int b = i / C, j = i % C, p = parent[b];
+        if (j >= nc || p == b) continue;
+        if (p >= n_seqs) {
+            atomicExch(&g_kv_pages_err, 1);
+            continue;
+        }
+        const int was = tile[i], now = p < 0 ? -1 : tile[p * C + j];
+        if (was >= n_pages || now >= n_pages) atomicExch(&g_kv_pages_err, 1);
+        if (was == now) continue;
+        if (was >= 0 && was < n_pages) atomicSub(refs + was, 1);
+        if (now >= 0 && now < n_pages) atomicAdd(refs + now, 1);
+        pages[(size_t)b * max_pages + c0 + j] = now;
+    }
+}
+
+// Reserve, the plan.  Workspace after the list: entry[n_seqs] (the page that
+// sequence b writes, -1 none, -2 nothing to do), rank[n_seqs] (its number
+// among those that need a page, or -1).
+__global__ void __launch_bounds__(PLAN_THREADS) k_reserve_plan(int *pages, int n_seqs, int max_pages, int page_shift,
+                                                               int *refs, int n_pages, const int *pos, int *d_short,
+                                                               int *ws) {
+    __shared__ int part[33], n_copy;
+    pdl_wait();
+    pdl_launch_dependents();
+    int *const list = ws + WS_LIST, *const entry = list + 2 * n_seqs, *const rank = entry + n_seqs;
+    const int tid = threadIdx.x;
+    if (tid == 0) n_copy = 0;
+    for (int b = tid; b < n_seqs; b += PLAN_THREADS) {
+        const int p = pos[b];
+        int e = -2;
+        if (p >= 0) {
+            const int j = p >> page_shift;
+            if (j < max_pages) e = pages[(size_t)b * max_pages + j];
+            if (j >= max_pages || e >= n_pages) {
+                atomicExch(&g_kv_pages_err, 1);
+                e = -2;
+            } else if (e < 0) {
+                e = -1;
+            }
+        }
+        entry[b] = e;
+    }
+    __syncthreads();
+    int need_total = 0;
+    for (int b0 = 0; b0 < n_seqs; b0 += PLAN_THREADS) {
+        const int b = b0 + tid;
+        bool need = false;
+        if (b < n_seqs) {
+            const int e = entry[b];
+            need = e == -1;
+            if (e >= 0) {  // the i-th writer of a page copies it while more than i + 1 entries name it
+                const int r = refs[e];
+                if (r > 1) {
+                    int before = 0;
+                    for (int i = 0; i < b; i++) before += entry[i] == e;
+                    need = before < r - 1;
+                }
+            }
+        }
+        int total;
+        const int k = block_scan(need ? 1 : 0, part, &total);
+        if (b < n_seqs) rank[b] = need ? need_total + k : -1;
+        need_total += total;
+    }
+    // the lowest free ids, into the destinations of the list
+    int found = 0;
+    for (int p0 = 0; p0 < n_pages && found < need_total; p0 += PLAN_THREADS) {
+        const int p = p0 + tid;
+        const bool fr = p < n_pages && refs[p] == 0;
+        int total;
+        const int k = block_scan(fr ? 1 : 0, part, &total);
+        if (fr && found + k < need_total) list[2 * (found + k) + 1] = p;
+        found += total;
+    }
+    const int missing = max(need_total - found, 0);
+    __syncthreads();
+    if (missing == 0) {
+        // the destinations move into rank first: the list is rewritten as pairs to copy
+        for (int b = tid; b < n_seqs; b += PLAN_THREADS)
+            if (rank[b] >= 0) rank[b] = list[2 * rank[b] + 1];
+        __syncthreads();
+        for (int b = tid; b < n_seqs; b += PLAN_THREADS) {
+            const int p = rank[b], e = entry[b];
+            if (p < 0) continue;
+            pages[(size_t)b * max_pages + (pos[b] >> page_shift)] = p;
+            refs[p] = 1;
+            if (e >= 0) {
+                atomicSub(refs + e, 1);
+                const int k = atomicAdd(&n_copy, 1);
+                list[2 * k] = e;
+                list[2 * k + 1] = p;
+            }
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        *d_short = missing;
+        ws[0] = n_copy;
+    }
+}
+
+// Compact, the plan.  Workspace: the list, then map[n_pages] (new id of a
+// page at or above n_live, -1 for a free one).
+__global__ void __launch_bounds__(PLAN_THREADS) k_compact_plan(int *refs, int n_pages, int *d_n_live, int *ws) {
+    __shared__ int part[33];
+    pdl_wait();
+    pdl_launch_dependents();
+    int *const list = ws + WS_LIST, *const map = list + n_pages + 2;
+    const int tid = threadIdx.x;
+    int n_live = 0;
+    for (int p0 = 0; p0 < n_pages; p0 += PLAN_THREADS) {
+        const int p = p0 + tid;
+        n_live += __syncthreads_count(p < n_pages && refs[p] > 0);
+    }
+    int holes = 0, movers = 0;
+    for (int p0 = 0; p0 < n_pages; p0 += PLAN_THREADS) {
+        const int p = p0 + tid;
+        const bool live = p < n_pages && refs[p] > 0, pick = p < n_pages && (p < n_live ? !live : live);
+        int total_hole, total_mover;
+        const int kh = block_scan(pick && p < n_live ? 1 : 0, part, &total_hole);
+        const int km = block_scan(pick && p >= n_live ? 1 : 0, part, &total_mover);
+        if (pick && p < n_live) list[2 * (holes + kh) + 1] = p;
+        if (pick && p >= n_live) list[2 * (movers + km)] = p;
+        if (p >= n_live && p < n_pages) map[p] = -1;
+        holes += total_hole;
+        movers += total_mover;
+    }
+    __syncthreads();
+    for (int k = tid; k < movers; k += PLAN_THREADS) {
+        const int src = list[2 * k], dst = list[2 * k + 1];
+        map[src] = dst;
+        refs[dst] = refs[src];
+        refs[src] = 0;
+    }
+    if (tid == 0) {
+        *d_n_live = n_live;
+        ws[0] = movers;
+    }
+}
+
+// Renames the table's entries by the plan's map.
+__device__ __forceinline__ void rename_entry(int *entry, int n_live, int n_pages, const int *map) {
+    const int e = *entry;
+    if (e < n_live) return;
+    const int to = e < n_pages ? map[e] : -1;
+    if (to < 0) atomicExch(&g_kv_pages_err, 1);  // no such page, or its count says it is free
+    else *entry = to;
+}
+
+// Copies the listed pages in every pool; pages != NULL: renames the table too.
+__global__ void __launch_bounds__(256) k_pages_copy(Pools pools, int n_pools, int vecs, const int *ws, int *pages,
+                                                    long long entries, const int *d_n_live, int n_pages) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int n = ws[0];
+    const long long tid = (long long)blockIdx.x * 256 + threadIdx.x, nthr = (long long)gridDim.x * 256;
+    if (pages) {
+        const int n_live = *d_n_live;
+        for (long long i = tid; i < entries; i += nthr) rename_entry(pages + i, n_live, n_pages, ws + WS_LIST + n_pages + 2);
+    }
+    for (long long item = blockIdx.x; item < (long long)n * n_pools; item += gridDim.x) {
+        const int k = (int)(item / n_pools), pool = (int)(item % n_pools);
+        const uint4 *src = pools.p[pool] + (size_t)ws[WS_LIST + 2 * k] * vecs;
+        uint4 *dst = pools.p[pool] + (size_t)ws[WS_LIST + 2 * k + 1] * vecs;
+        for (int i = threadIdx.x; i < vecs; i += 256) dst[i] = src[i];
+    }
+}
+
+int check_pools(const char *name, void *const *h_pools, int n_pools, size_t page_bytes) {
+    if (!h_pools || n_pools <= 0 || page_bytes == 0 || page_bytes % 16 || page_bytes / 16 > (1u << 30))
+        return lmc_set_error(LMC_ERR_INVALID, "%s: %d pools, pages of %zu bytes (need a multiple of 16)", name, n_pools,
+                             page_bytes);
+    for (int i = 0; i < n_pools; i++)
+        if (!h_pools[i] || ((uintptr_t)h_pools[i] & 15))
+            return lmc_set_error(LMC_ERR_INVALID, "%s: pool %d is null or not 16-byte aligned", name, i);
+    return LMC_OK;
+}
+
+int copy_launch(const char *name, void *const *h_pools, int n_pools, size_t page_bytes, const int *ws, int *pages,
+                long long entries, const int *d_n_live, int n_pages, cudaStream_t s) {
+    const int grid = lmc_sm_count() * 8;
+    for (int p0 = 0; p0 < n_pools; p0 += MAX_POOLS) {
+        Pools pools;
+        const int n = n_pools - p0 < MAX_POOLS ? n_pools - p0 : MAX_POOLS;
+        for (int i = 0; i < n; i++) pools.p[i] = (uint4 *)h_pools[p0 + i];
+        LMC_LAUNCH(name, k_pages_copy, grid, 256, 0, s, pools, n, (int)(page_bytes / 16), ws, p0 ? nullptr : pages, entries,
+                   d_n_live, n_pages);
+    }
+    return LMC_OK;
+}
+
+}  // namespace
+
+extern "C" size_t lmc_kv_pages_workspace_bytes(int n_seqs, int n_pages) {
+    if (n_seqs < 0 || n_pages < 0) return 0;
+    return sizeof(int) * (64 + 4 * ((size_t)n_seqs + (size_t)n_pages));
+}
+
+extern "C" int lmc_kv_pages_fork(int *d_pages, int n_seqs, int max_pages, int *d_refs, int n_pages, const int *d_parent,
+                                 void *stream) {
+    if (!d_pages || !d_refs || !d_parent) return lmc_set_error(LMC_ERR_INVALID, "kv_pages_fork: null pointer");
+    if (n_seqs <= 0 || max_pages <= 0 || n_pages <= 0 || n_seqs > 32768)
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_fork: %d sequences x %d entries, %d pages (at most 32768 "
+                             "sequences)", n_seqs, max_pages, n_pages);
+    int C = 32;
+    while (C > 1 && (size_t)n_seqs * C * sizeof(int) > 128 * 1024) C /= 2;
+    const size_t smem = (size_t)n_seqs * C * sizeof(int);
+    if (smem > 48 * 1024)
+        LMC_CUDA_TRY(cudaFuncSetAttribute(k_pages_fork, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+    LMC_LAUNCH("kv pages fork", k_pages_fork, lmc_cdiv(max_pages, C), 256, smem, lmc_stream(stream), d_pages, n_seqs,
+               max_pages, d_refs, n_pages, d_parent, C);
+    return LMC_OK;
+}
+
+extern "C" int lmc_kv_pages_reserve(void *const *h_pools, int n_pools, size_t page_bytes, int *d_pages, int n_seqs,
+                                    int max_pages, int page_size, int *d_refs, int n_pages, const int *d_pos,
+                                    int *d_short, void *d_ws, size_t ws_bytes, void *stream) {
+    const int rc = check_pools("kv_pages_reserve", h_pools, n_pools, page_bytes);
+    if (rc != LMC_OK) return rc;
+    if (!d_pages || !d_refs || !d_pos || !d_short || !d_ws)
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_reserve: null pointer");
+    if (n_seqs <= 0 || max_pages <= 0 || n_pages <= 0 || page_size < 16 || (page_size & (page_size - 1)))
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_reserve: %d sequences x %d entries, %d pages of %d positions",
+                             n_seqs, max_pages, n_pages, page_size);
+    if (ws_bytes < lmc_kv_pages_workspace_bytes(n_seqs, n_pages))
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_reserve: workspace %zu bytes < %zu needed", ws_bytes,
+                             lmc_kv_pages_workspace_bytes(n_seqs, n_pages));
+    int shift = 0;
+    while ((1 << shift) < page_size) shift++;
+    cudaStream_t s = lmc_stream(stream);
+    LMC_LAUNCH("kv pages reserve", k_reserve_plan, 1, PLAN_THREADS, 0, s, d_pages, n_seqs, max_pages, shift, d_refs, n_pages,
+               d_pos, d_short, (int *)d_ws);
+    return copy_launch("kv pages copy", h_pools, n_pools, page_bytes, (const int *)d_ws, nullptr, 0, nullptr, n_pages, s);
+}
+
+extern "C" int lmc_kv_pages_compact(void *const *h_pools, int n_pools, size_t page_bytes, int *d_pages, int n_seqs,
+                                    int max_pages, int *d_refs, int n_pages, int *d_n_live, void *d_ws, size_t ws_bytes,
+                                    void *stream) {
+    const int rc = check_pools("kv_pages_compact", h_pools, n_pools, page_bytes);
+    if (rc != LMC_OK) return rc;
+    if (!d_pages || !d_refs || !d_n_live || !d_ws)
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_compact: null pointer");
+    if (n_seqs <= 0 || max_pages <= 0 || n_pages <= 0)
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_compact: %d sequences x %d entries, %d pages", n_seqs, max_pages,
+                             n_pages);
+    if (ws_bytes < lmc_kv_pages_workspace_bytes(n_seqs, n_pages))
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_compact: workspace %zu bytes < %zu needed", ws_bytes,
+                             lmc_kv_pages_workspace_bytes(n_seqs, n_pages));
+    cudaStream_t s = lmc_stream(stream);
+    LMC_LAUNCH("kv pages compact", k_compact_plan, 1, PLAN_THREADS, 0, s, d_refs, n_pages, d_n_live, (int *)d_ws);
+    return copy_launch("kv pages copy", h_pools, n_pools, page_bytes, (const int *)d_ws, d_pages,
+                       (long long)n_seqs * max_pages, d_n_live, n_pages, s);
+}
+
+extern "C" int lmc_kv_pages_status(void) {
+    int v = 0;
+    LMC_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_kv_pages_err, sizeof(int)));
+    if (!v) return LMC_OK;
+    const int zero = 0;
+    LMC_CUDA_TRY(cudaMemcpyToSymbol(g_kv_pages_err, &zero, sizeof(int)));
+    return lmc_set_error(LMC_ERR_INVALID, "kv pages: a table entry, parent or position outside its range (left as it is)");
+}

@@ -121,6 +121,21 @@ int lmc_attention_rows_paged_launch(float *out, int ldo, const float *q, int ldq
                                     const int *d_pages, int max_pages, int page_shift, int n_pages, void *d_ws,
                                     size_t ws_bytes, const float *rope_cos, const float *rope_sin, int *d_cnt,
                                     cudaStream_t s);
+/* Decode attention over 4-bit rows (attention_q4.cu); arguments checked by
+ * the caller (attention.cu), which fills an AttnArgs. */
+struct AttnArgs;
+int lmc_attention_q4_launch(const struct AttnArgs *a, int batch, size_t ws_bytes, cudaStream_t s);
+/* lmc_kv_append on stream s, K rotated by the [S][Dh/2] RoPE tables when they
+ * are given; n_seqs 0: sequences not checked. */
+int lmc_kv_append_launch(const float *k, const float *v, int ldk, int ldv, void *kc, void *vc, int kv_dtype,
+                         const int *d_seq, const int *d_pos, int rows, int n_seqs, int Hkv, int Dh, int S,
+                         const int *d_pages, int page_shift, int max_pages, int n_pages, const float *rope_cos,
+                         const float *rope_sin, cudaStream_t s);
+/* LMC_OK, or LMC_ERR_INVALID once after a kernel of that file met an index
+ * outside its range (the flag is cleared). */
+int lmc_attn_q4_status(void);
+int lmc_kv_rows_status(void);
+int lmc_kv_pages_status(void);
 /* Generation bookkeeping after one step (see lmc_model_generate): the greedy
  * id of each sequence is read from (and reset in) d_keys, or, with
  * from_next, the pick is the one already in d_next (a sampler wrote it; the

@@ -311,6 +311,10 @@ extern "C" int lmc_device_status(void) {
     if (st != LMC_OK) return st;
     const int at = lmc_attn_status();
     if (at != LMC_OK) return at;
+    int kv = lmc_attn_q4_status();
+    if (kv == LMC_OK) kv = lmc_kv_rows_status();
+    if (kv == LMC_OK) kv = lmc_kv_pages_status();
+    if (kv != LMC_OK) return kv;
     const int pe = lmc_peer_status();
     if (pe != LMC_OK) return pe;
     int v = 0;

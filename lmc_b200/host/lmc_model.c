@@ -521,6 +521,8 @@ static int alloc_state(lmc_model *m) {
     const size_t QD = (size_t)c->n_heads * c->head_dim, KV = (size_t)c->n_kv_heads * c->head_dim;
     if (m->kv_dtype == LMC_KV_Q8 && (c->head_dim % 16 || c->head_dim > 512))
         return lmc_set_error(LMC_ERR_UNSUPPORTED, "int8 KV rows need a head size that is a multiple of 16, <= 512");
+    if (m->kv_dtype == LMC_KV_Q4 && (c->head_dim % 32 || c->head_dim > 256))
+        return lmc_set_error(LMC_ERR_UNSUPPORTED, "4-bit KV rows need a head size that is a multiple of 32, <= 256");
     /* this rank's kv heads, rows of LMC_KV_ROW_BYTES */
     const size_t row_bytes = LMC_KV_ROW_BYTES(m->kv_dtype, c->head_dim);
     if (m->page_size) {
@@ -543,6 +545,7 @@ static int alloc_state(lmc_model *m) {
     } else {
         m->kv_layer_bytes = NS * (size_t)m->hkvl * (size_t)c->seq_len * row_bytes;
     }
+    m->kv_layer_bytes = (m->kv_layer_bytes + 15) & ~(size_t)15; /* every layer's rows start on 16 bytes */
     TRY(dev_alloc(&m->kc, m->kv_layer_bytes * c->n_layers));
     TRY(dev_alloc(&m->vc, m->kv_layer_bytes * c->n_layers));
     TRY(dev_alloc((void **)&m->x, 4 * B * D));
@@ -600,7 +603,7 @@ static int model_load(const char *path, int max_batch, int max_rows, int kv_dtyp
     if (page_size && (page_size < 16 || page_size > (1 << 16) || (page_size & (page_size - 1)) || n_pages <= 0))
         return lmc_set_error(LMC_ERR_INVALID, "model_load: KV pages of %d positions, %d pages (need a power of two "
                              "in [16, 65536] and at least one page)", page_size, n_pages);
-    if (kv_dtype != LMC_KV_F32 && kv_dtype != LMC_KV_F16 && kv_dtype != LMC_KV_Q8)
+    if (kv_dtype != LMC_KV_F32 && kv_dtype != LMC_KV_F16 && kv_dtype != LMC_KV_Q8 && kv_dtype != LMC_KV_Q4)
         return lmc_set_error(LMC_ERR_INVALID, "model_load: kv dtype");
     if (tp_size < 1 || tp_rank < 0 || tp_rank >= tp_size || (tp_size > 1 && !nccl_id))
         return lmc_set_error(LMC_ERR_INVALID, "model_load: shard %d of %d", tp_rank, tp_size);

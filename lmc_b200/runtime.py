@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "liblmc_b200.so")
 
 LMC_OK = 0
 EPI_NONE, EPI_GELU, EPI_ACCUM = 0, 1, 2
-KV_F32, KV_F16, KV_Q8 = 0, 1, 2
+KV_F32, KV_F16, KV_Q8, KV_Q4 = 0, 1, 2, 3
 
 _c = ctypes
 _vp, _i, _u32, _sz, _f = _c.c_void_p, _c.c_int, _c.c_uint32, _c.c_size_t, _c.c_float
@@ -45,6 +45,12 @@ SIGNATURES = {
     "lmc_attention_decode_noalloc": ([_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp], _i),
     "lmc_attention_decode_paged": ([_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _sz,
                                     _vp], _i),
+    "lmc_kv_append": ([_vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _i, _vp], _i),
+    "lmc_kv_read": ([_vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _i, _vp], _i),
+    "lmc_kv_pages_workspace_bytes": ([_i, _i], _sz),
+    "lmc_kv_pages_fork": ([_vp, _i, _i, _vp, _i, _vp, _vp], _i),
+    "lmc_kv_pages_reserve": ([_vp, _i, _sz, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _sz, _vp], _i),
+    "lmc_kv_pages_compact": ([_vp, _i, _sz, _vp, _i, _i, _vp, _i, _vp, _vp, _sz, _vp], _i),
     "lmc_model_load": ([_c.c_char_p, _i, _i, _c.POINTER(_vp)], _i),
     "lmc_nccl_unique_id": ([_vp], _i),
     "lmc_model_load_tp": ([_c.c_char_p, _i, _i, _i, _i, _vp, _c.POINTER(_vp)], _i),
@@ -120,6 +126,17 @@ def ptr(t):
     if hasattr(t, "ctypes"):
         return t.ctypes.data
     return int(t)
+
+
+def kv_row_bytes(kv_dtype, head_dim):
+    """Bytes of one cached K or V row (LMC_KV_ROW_BYTES)."""
+    return {KV_F32: 4 * head_dim, KV_F16: 2 * head_dim, KV_Q8: head_dim + 16,
+            KV_Q4: head_dim // 2 + 4 * -(-head_dim // 64)}[kv_dtype]
+
+
+def pool_list(pools):
+    """Host array of device addresses (h_pools of the lmc_kv_pages_* calls)."""
+    return (_vp * len(pools))(*(ptr(p) for p in pools))
 
 
 class ModelConfig(ctypes.Structure):
