@@ -1,9 +1,34 @@
 // attention_q4.cu - decode attention over 4-bit K/V rows (LMC_KV_Q4).
 //
-// One CTA per (query head, row): the new K/V row is quantized into shared
-// memory (and, by the first head of the group, into the cache), each warp
-// walks every fourth cached position with its own running maximum, sum and
-// accumulator, and the warps' results are merged at the end.
+// With codes c and (d, m) of group j (64 dims) of row t, and m' = m + 8 d:
+//   s_t = sum_j [ d_tj (q_j . (c_tj - 8)) + m'_tj sum(q_j) ] / sqrt(Dh)
+//   o_j = sum_t p_t d_tj (c_tj - 8) + sum_t p_t m'_tj,   p_t = 2^(s_t log2 e - max)
+// so the tensor cores only ever see whole numbers and fp32 factors; the
+// scales are applied per group outside (keys) or folded into the
+// probabilities (values).  Codes are centred because a sum of p d c over
+// positive codes would be large against the result of a long, flat softmax
+// and take its rounding with it.
+//
+// A code as fp16: a nibble ORed into the low bits of 1024.0 is 1024 + c,
+// exactly, and 1032 less is c - 8 (two instructions for two operands); the
+// nibble above it gives 16 (c - 8), and the 16 goes into q (keys) or the
+// final factor (values).  fp32 factors become an fp16 pair hi + lo (22
+// bits): q, scaled by a power of two into fp16's range, with hi in rows 0-7
+// of the 16 x 16 operand (8 query heads) and lo in rows 8-15, so the padding
+// that 8 heads leave carries the low part; p d as two products into one
+// accumulator.  The probabilities are scaled so that p d stays just below
+// 2^15 (the largest exponent of d so far is tracked like the running
+// maximum), so small values keep their relative accuracy.  The matrix unit
+// truncates its sums, so a tile's products go to fresh accumulators that are
+// added to the running ones in rounded fp32.
+//
+// Work: tiles of 32 positions of one (sequence, kv head, 8 query heads).  All
+// tiles of the batch, in order, are divided evenly over the CTAs and within a
+// CTA over its four warps, so ragged batches and single long sequences load
+// every SM alike.  A warp streams its tiles through its own ring in shared
+// memory (16-byte asynchronous copies, two tiles ahead) with a running
+// softmax; parts of one item that lie in one CTA are merged in shared memory,
+// parts in several CTAs through the workspace by k_q4_combine.
 #include "attention.cuh"
 #include "kv_q4.cuh"
 #include "lmc_common.cuh"
@@ -13,117 +38,669 @@ namespace {
 
 __device__ int g_attn_q4_err;  // a page id outside the pool was met (lmc_device_status)
 
-__device__ __forceinline__ const uint8_t *q4_row(const AttnArgs &a, const void *cache, size_t cs, int kh, int t, int RB,
-                                                 bool *ok) {
-    const uint8_t *c = (const uint8_t *)cache;
-    if (!a.pages) return c + (((long long)cs * a.Hkv + kh) * a.S + t) * RB;
+constexpr int Q4_WARPS = 4;
+constexpr int Q4_TILE = 32;    // positions per tile
+constexpr int Q4_STAGES = 3;   // tiles in a warp's ring
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Q4Args {
+    AttnArgs a;
+    int HG;         // groups of 8 query heads per kv head
+    int rmin;       // tiles per CTA at least (workspace slots per head: a.nsplit)
+    int items_only; // 1: an item is never divided (a.nsplit is 1)
+    int batch, vec; // vec: q, new rows and out can be moved 16 bytes at a time
+};
+
+template <int NB> struct Q4 {
+    static constexpr int DH = 32 * NB, NG = kv_q4_groups(DH), RB = kv_q4_row_bytes(DH);
+    static constexpr int SIDE = Q4_TILE * RB + 16;        // a tile's K or V rows, from any 4-byte phase
+    static constexpr int STAGE = 2 * SIDE;
+    static constexpr int META = Q4_TILE * NG * 2;         // floats: (d, m) of a tile's rows, one side
+    static constexpr int WARP_BYTES = Q4_STAGES * STAGE + 2 * META * 4;
+    static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, offset, sum)
+    static_assert(Q4_STAGES * STAGE >= 8 * SLOT * 4, "a partial result fits the ring that it is kept in");
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void hmma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// x, y as fp16 pairs hi + lo
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// Eight codes of a word, less 8, as fp16 pairs: nibbles (0, 4), 16 x (1, 5), (2, 6), 16 x (3, 7).
+__device__ __forceinline__ uint32_t h2sub(uint32_t x, uint32_t y) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&y));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ void codes8(uint32_t w, uint32_t (&c)[4]) {
+    const uint32_t w8 = w >> 8;
+    c[0] = h2sub((w & 0x000f000fu) | 0x64006400u, 0x64086408u);
+    c[1] = h2sub((w & 0x00f000f0u) | 0x64006400u, 0x64806480u);
+    c[2] = h2sub((w8 & 0x000f000fu) | 0x64006400u, 0x64086408u);
+    c[3] = h2sub((w8 & 0x00f000f0u) | 0x64006400u, 0x64806480u);
+}
+
+// A place in the batch's order of tiles: sequences, their (kv head, head
+// group) items, the item's tiles.
+struct Place {
+    int b, j, tile, nt, pos, left;  // left: units still to go (tiles, or items with items_only)
+};
+__device__ __forceinline__ int seq_pos(const Q4Args &g, int b) {  // position, or -1 when the row has nothing to do
+    const int p = __ldg(g.a.pos + b);
+    return p < 0 || p >= g.a.S ? -1 : p;
+}
+__device__ __forceinline__ void place_at(const Q4Args &g, Place &p) {  // first sequence >= p.b with work
+    p.pos = -1;
+    while (p.b < g.batch && (p.pos = seq_pos(g, p.b)) < 0) p.b++;
+    p.nt = p.pos / Q4_TILE + 1;
+}
+__device__ __forceinline__ void next_tile(const Q4Args &g, Place &p) {
+    p.tile++;
+    if (!g.items_only) p.left--;
+    if (p.tile < p.nt) return;
+    p.tile = 0;
+    p.j++;
+    if (g.items_only) p.left--;
+    if (p.j < g.a.Hkv * g.HG) return;
+    p.j = 0;
+    p.b++;
+    place_at(g, p);
+}
+
+// Byte offset of row t (the start of a run within one page) in its cache.
+__device__ __forceinline__ long long run_offset(const AttnArgs &a, size_t cs, int kh, int t, int RB, bool *ok) {
+    if (!a.pages) return (((long long)cs * a.Hkv + kh) * a.S + t) * RB;
     int pg = __ldg(a.pages + cs * a.max_pages + (t >> a.page_shift));
     *ok = pg >= 0 && pg < a.n_pages;
     if (!*ok) {
         atomicExch(&g_attn_q4_err, 1);
         pg = 0;
     }
-    return c + ((((long long)pg * a.Hkv + kh) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * RB;
+    return ((((long long)pg * a.Hkv + kh) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * RB;
+}
+__device__ __forceinline__ void copy_run(uint32_t dst, const uint8_t *src, int bytes, int lane) {
+    // from the 16-byte boundary at or before src; the last copy reads no byte past the run
+    const int phase = (int)((uintptr_t)src & 15);
+    const uint8_t *from = src - phase;
+    for (int i = 16 * lane; i < bytes + phase; i += 512) {
+        const int n = min(16, bytes + phase - i);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i), "l"(from + i), "r"(n) : "memory");
+    }
+}
+// Starts the copies of a tile's rows (all but the new row) and closes their group.
+template <int NB>
+__device__ __forceinline__ void fetch(const Q4Args &g, const Place &p, uint32_t stage, int lane) {
+    const AttnArgs &a = g.a;
+    constexpr int RB = Q4<NB>::RB;
+    const int t0 = p.tile * Q4_TILE, rows = min(Q4_TILE, (a.append ? p.pos : p.pos + 1) - t0), kh = p.j / g.HG;
+    const size_t cs = a.seq ? (size_t)__ldg(a.seq + p.b) : (size_t)p.b;
+    const int run = a.pages && a.page_shift == 4 ? 16 : Q4_TILE;  // rows that lie one behind the other
+    for (int r = 0; r < rows; r += run) {
+        bool ok;
+        const long long off = run_offset(a, cs, kh, t0 + r, RB, &ok);
+        const int bytes = min(run, rows - r) * RB;
+        copy_run(stage + r * RB, (const uint8_t *)a.k_cache + off, bytes, lane);
+        copy_run(stage + Q4<NB>::SIDE + r * RB, (const uint8_t *)a.v_cache + off, bytes, lane);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(128) k_attn_q4(AttnArgs a) {
-    pdl_wait();
-    pdl_launch_dependents();
-    __shared__ uint32_t newrow[2][40];
-    __shared__ float red[4][256], stat[4][2];
-    const int h = blockIdx.x, b = blockIdx.y, G = a.H / a.Hkv, kh = h / G, Dh = a.Dh, RB = kv_q4_row_bytes(Dh);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, NW = Dh / 8;
-    const int pos = a.pos[b];
-    if (pos < 0 || pos >= a.S) return;
-    const size_t cs = a.seq ? (size_t)a.seq[b] : (size_t)b;
-    const float *rc = a.rope_cos ? a.rope_cos + (size_t)pos * (Dh / 2) : nullptr;
-    const float *rs = a.rope_sin ? a.rope_sin + (size_t)pos * (Dh / 2) : nullptr;
-    if (a.append && warp < 2) {
+__device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
+    if (vec) {
+        const float4 u = *reinterpret_cast<const float4 *>(p), w = *reinterpret_cast<const float4 *>(p + 4);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = p[i];
+    }
+}
+// Pairs (2 d, 2 d + 1) of dims d0 .. d0 + 7 rotated (src/ops_llama.c:39-48).
+__device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0, float (&x)[8]) {
+    if (!a.rope_cos) return;
+    const size_t t = (size_t)pos * (Dh / 2) + d0 / 2;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float c = a.rope_cos[t + i], s = a.rope_sin[t + i], x0 = x[2 * i], x1 = x[2 * i + 1];
+        x[2 * i] = x0 * c - x1 * s;
+        x[2 * i + 1] = x0 * s + x1 * c;
+    }
+}
+
+// What a warp carries through the tiles of one item.
+template <int NB> struct Q4State {
+    uint32_t qa[2 * NB][4];           // q as matrix operands: head g hi, lo, hi, lo
+    float qsum[Q4<NB>::NG], qfac;     // head g: log2 e / sqrt(Dh) times sum(q_j); factor of q . c
+    float o[2 * NB][4];               // dims x heads (see the output below)
+    float om[Q4<NB>::NG], l, off, mx; // head g, this lane's positions: sum p m, sum p; offset and maximum of s
+    int vexp;                         // largest exponent field of the values' d so far
+};
+
+template <int NB>
+__device__ __forceinline__ void load_q(const Q4Args &g, const Place &p, int lane, Q4State<NB> &st) {
+    const AttnArgs &a = g.a;
+    constexpr int DH = Q4<NB>::DH;
+    const int G = a.H / a.Hkv, kh = p.j / g.HG, head = (p.j % g.HG) * 8 + (lane >> 2), t = lane & 3;
+    float x[NB][8];
+    float big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        if (head < G) {
+            load8(a.q + (size_t)p.b * a.ldq + ((size_t)kh * G + head) * DH + 32 * i + 8 * t, g.vec, x[i]);
+            rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[i][e]));
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // a power of two that brings the largest |q| into [2^12, 2^13)
+    const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+    const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
+    const float scale = LOG2E / sqrtf((float)DH);
+    st.qfac = scale * __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
+#pragma unroll
+    for (int i = 0; i < Q4<NB>::NG; i++) st.qsum[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) s += x[i][e];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        st.qsum[i / 2] += s * scale;
+        // nibbles (0, 4) and (2, 6) of a word meet slice 2 i, (1, 5) and (3, 7), 16 times as large, slice 2 i + 1
+        const float dn = up * 0.0625f;
+        split2(x[i][0] * up, x[i][4] * up, st.qa[2 * i][0], st.qa[2 * i][1]);
+        split2(x[i][2] * up, x[i][6] * up, st.qa[2 * i][2], st.qa[2 * i][3]);
+        split2(x[i][1] * dn, x[i][5] * dn, st.qa[2 * i + 1][0], st.qa[2 * i + 1][1]);
+        split2(x[i][3] * dn, x[i][7] * dn, st.qa[2 * i + 1][2], st.qa[2 * i + 1][3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = st.o[i][2] = st.o[i][3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Q4<NB>::NG; i++) st.om[i] = 0.0f;
+    st.l = 0.0f;
+    st.off = st.mx = -INFINITY;
+    st.vexp = 0;
+}
+
+// The new K and V rows quantized into the tile (and, by the first head group,
+// into the cache).
+template <int NB>
+__device__ __forceinline__ void append(const Q4Args &g, const Place &p, uint8_t *krow, uint8_t *vrow, int lane) {
+    const AttnArgs &a = g.a;
+    constexpr int DH = Q4<NB>::DH, NW = DH / 8;
+    const int kh = p.j / g.HG;
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (lane < NW) {
-            const float *src = (warp ? a.v_new : a.k_new) + (size_t)b * a.ldkv + (size_t)kh * Dh + 8 * lane;
-            for (int i = 0; i < 4; i++) {
-                x[2 * i] = src[2 * i];
-                x[2 * i + 1] = src[2 * i + 1];
-                if (!warp && rc) {
-                    const float c = rc[4 * lane + i], s = rs[4 * lane + i], x0 = x[2 * i], x1 = x[2 * i + 1];
-                    x[2 * i] = x0 * c - x1 * s;
-                    x[2 * i + 1] = x0 * s + x1 * c;
-                }
-            }
+            load8((side ? a.v_new : a.k_new) + (size_t)p.b * a.ldkv + (size_t)kh * DH + 8 * lane, g.vec, x);
+            if (!side) rope8(a, p.pos, DH, 8 * lane, x);
         }
         uint32_t codes, dm;
         kv_q4_quantize<32>(x, lane < NW, codes, dm);
+        uint32_t *row = reinterpret_cast<uint32_t *>(side ? vrow : krow);
         if (lane < NW) {
-            newrow[warp][lane] = codes;
-            if (lane % 8 == 0) newrow[warp][NW + lane / 8] = dm;
+            row[lane] = codes;
+            if (lane % 8 == 0) row[NW + lane / 8] = dm;
         }
-        bool ok = true;
-        uint32_t *dst = (uint32_t *)q4_row(a, warp ? a.v_cache : a.k_cache, cs, kh, pos, RB, &ok);
-        if (lane < NW && h % G == 0 && ok) {
-            dst[lane] = codes;
-            if (lane % 8 == 0) dst[NW + lane / 8] = dm;
-        }
-    }
-    float q[8];
-    for (int i = 0; i < 8; i++) q[i] = 0.0f;
-    if (lane < NW) {
-        const float *qp = a.q + (size_t)b * a.ldq + (size_t)h * Dh + 8 * lane;
-        for (int i = 0; i < 4; i++) {
-            q[2 * i] = qp[2 * i];
-            q[2 * i + 1] = qp[2 * i + 1];
-            if (rc) {
-                const float c = rc[4 * lane + i], s = rs[4 * lane + i], x0 = q[2 * i], x1 = q[2 * i + 1];
-                q[2 * i] = x0 * c - x1 * s;
-                q[2 * i + 1] = x0 * s + x1 * c;
+        if (p.j % g.HG == 0) {
+            bool ok = true;
+            const size_t cs = a.seq ? (size_t)__ldg(a.seq + p.b) : (size_t)p.b;
+            const long long off = run_offset(a, cs, kh, p.pos, Q4<NB>::RB, &ok);
+            uint32_t *dst = reinterpret_cast<uint32_t *>((uint8_t *)(side ? a.v_cache : a.k_cache) + off);
+            if (ok && lane < NW) {
+                dst[lane] = codes;
+                if (lane % 8 == 0) dst[NW + lane / 8] = dm;
             }
         }
     }
-    __syncthreads();
-    const float scale = 1.0f / sqrtf((float)Dh);
-    float m = -INFINITY, l = 0.0f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int t = warp; t <= pos; t += 4) {
-        bool ok;
-        const uint32_t *kr = (const uint32_t *)q4_row(a, a.k_cache, cs, kh, t, RB, &ok);
-        const uint32_t *vr = (const uint32_t *)q4_row(a, a.v_cache, cs, kh, t, RB, &ok);
-        if (a.append && t == pos) { kr = newrow[0]; vr = newrow[1]; }
-        float s = 0.0f;
-        if (lane < NW) {
-            const uint32_t w = kr[lane], dm = kr[NW + lane / 8];
-            const float d = __half2float(__ushort_as_half((unsigned short)(dm & 0xffff)));
-            const float mm = __half2float(__ushort_as_half((unsigned short)(dm >> 16)));
-            for (int i = 0; i < 8; i++) s = fmaf(q[i], fmaf(d, (float)((w >> (4 * i)) & 15u), mm), s);
-        }
-        s = warp_sum(s) * scale;
-        const float mn = fmaxf(m, s), f = expf(m - mn), p = expf(s - mn);
-        m = mn;
-        l = l * f + p;
-        if (lane < NW) {
-            const uint32_t w = vr[lane], dm = vr[NW + lane / 8];
-            const float d = __half2float(__ushort_as_half((unsigned short)(dm & 0xffff)));
-            const float mm = __half2float(__ushort_as_half((unsigned short)(dm >> 16)));
-            for (int i = 0; i < 8; i++) acc[i] = fmaf(p, fmaf(d, (float)((w >> (4 * i)) & 15u), mm), acc[i] * f);
+}
+
+// One tile: n valid rows at kt / vt (row r at r * RB); kdm, vdm: this warp's
+// (d, m) floats.  Of each 16 rows lane (g, t) holds the scores of head g at
+// rows 4 t .. 4 t + 3 (matrix column order 0, 2 | 1, 3: rows that a quarter
+// warp reads then lie in different banks).
+template <int NB>
+__device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const uint8_t *vt, float *kdm, float *vdm, int n, int lane) {
+    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, DH = Q4<NB>::DH;
+    const int gq = lane >> 2, t = lane & 3;
+    // (d, m') of row `lane` to floats; rows past the end: d = m' = 0
+    uint32_t dmax = 0;
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        const uint32_t kw = lane < n ? *reinterpret_cast<const uint32_t *>(kt + lane * RB + DH / 2 + 4 * j) : 0u;
+        const uint32_t vw = lane < n ? *reinterpret_cast<const uint32_t *>(vt + lane * RB + DH / 2 + 4 * j) : 0u;
+        float2 kf = __half22float2(*reinterpret_cast<const __half2 *>(&kw));
+        float2 vf = __half22float2(*reinterpret_cast<const __half2 *>(&vw));
+        kf.y = fmaf(8.0f, kf.x, kf.y);
+        vf.y = fmaf(8.0f, vf.x, vf.y);
+        *reinterpret_cast<float2 *>(kdm + 2 * (lane * NG + j)) = kf;
+        *reinterpret_cast<float2 *>(vdm + 2 * (lane * NG + j)) = vf;
+        dmax = max(dmax, vw & 0xffffu);
+    }
+    const int vexp = min((int)(__reduce_max_sync(0xffffffffu, dmax) >> 10), 30);
+    __syncwarp();
+    float s[2][4];  // [16 rows][row 4 t + r]
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int par = 0; par < 2; par++) {  // rows 16 h + 2 g + par are the columns
+            float c[NG][4];
+#pragma unroll
+            for (int j = 0; j < NG; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+            const uint32_t *kr = reinterpret_cast<const uint32_t *>(kt + (16 * h + 2 * gq + par) * RB) + t;
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                uint32_t w[4];
+                codes8(kr[4 * i], w);
+                hmma(c[i / 2], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
+                hmma(c[i / 2], st.qa[2 * i + 1][0], st.qa[2 * i + 1][1], st.qa[2 * i + 1][2], st.qa[2 * i + 1][3], w[1], w[3]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {  // columns 2 t, 2 t + 1: rows 4 t + par, 4 t + 2 + par
+                const float *dm = kdm + 2 * NG * (16 * h + 4 * t + 2 * e + par);
+                float x = 0.0f, y = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    const float2 f = *reinterpret_cast<const float2 *>(dm + 2 * j);
+                    x = fmaf(f.x, c[j][e] + c[j][2 + e], x);
+                    y = fmaf(f.y, st.qsum[j], y);
+                }
+                s[h][2 * e + par] = fmaf(x, st.qfac, y);
+            }
         }
     }
-    if (lane == 0) { stat[warp][0] = m; stat[warp][1] = l; }
-    if (lane < NW)
-        for (int i = 0; i < 8; i++) red[warp][8 * lane + i] = acc[i];
-    __syncthreads();
-    float M = -INFINITY, L = 0.0f;
-    for (int w = 0; w < 4; w++) M = fmaxf(M, stat[w][0]);
-    for (int w = 0; w < 4; w++) if (stat[w][0] != -INFINITY) L += stat[w][1] * expf(stat[w][0] - M);
-    for (int d = threadIdx.x; d < Dh; d += 128) {
-        float o = 0.0f;
-        for (int w = 0; w < 4; w++) if (stat[w][0] != -INFINITY) o += red[w][d] * expf(stat[w][0] - M);
-        a.out[(size_t)b * a.ldo + (size_t)h * Dh + d] = o / L;
+    if (n < Q4_TILE)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (16 * h + 4 * t + r >= n) s[h][r] = -INFINITY;
+    // running maximum of head g and exponent of the values' scales
+    float m = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    m = fmaxf(m, st.mx);
+    const int ve = max(vexp, st.vexp);
+    const float off = m - (float)(29 - ve), f = ex2(st.off - off);  // (2^-inf = 0 the first time)
+    st.mx = m;
+    st.off = off;
+    st.vexp = ve;
+    st.l *= f;
+    const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            s[h][r] = ex2(s[h][r] - off);
+            st.l += s[h][r];
+        }
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        uint32_t bh[2][2], bl[2][2];  // p d of the 16 rows of each half: hi, lo
+        st.om[j] *= f;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float2 dm = *reinterpret_cast<const float2 *>(vdm + 2 * (NG * (16 * h + 4 * t + r) + j));
+                w[r] = s[h][r] * dm.x;
+                st.om[j] = fmaf(s[h][r], dm.y, st.om[j]);
+            }
+            split2(w[0], w[2], bh[h][0], bl[h][0]);
+            split2(w[1], w[3], bh[h][1], bl[h][1]);
+        }
+        // this lane's dims: word g of the group, or half a word of a group of 32
+        const bool half = NB % 2 && j == NG - 1;
+        const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
+        uint32_t cw[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) cw[h][r] = *reinterpret_cast<const uint32_t *>(vr + (16 * h + r) * RB);
+#pragma unroll
+        for (int k = 0; k < (half ? 1 : 2); k++) {  // nibbles 0-3, 4-7 of the words (or the half word's four)
+            const uint32_t sel = half ? ((gq & 1) ? 0x7632u : 0x5410u) : (k ? 0x7632u : 0x5410u);
+            const int i = 4 * j + 2 * k;
+            float c[2][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[0][e] = c[1][e] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t x[4], y[4];  // rows 4 t + (0, 2) and (1, 3)
+                codes8(__byte_perm(cw[h][0], cw[h][2], sel), x);
+                codes8(__byte_perm(cw[h][1], cw[h][3], sel), y);
+                hmma(c[0], x[0], x[1], y[0], y[1], bh[h][0], bh[h][1]);
+                hmma(c[1], x[2], x[3], y[2], y[3], bh[h][0], bh[h][1]);
+                hmma(c[0], x[0], x[1], y[0], y[1], bl[h][0], bl[h][1]);
+                hmma(c[1], x[2], x[3], y[2], y[3], bl[h][0], bl[h][1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                st.o[i + e][0] = fmaf(st.o[i + e][0], f0, c[e][0]);
+                st.o[i + e][1] = fmaf(st.o[i + e][1], f1, c[e][1]);
+                st.o[i + e][2] = fmaf(st.o[i + e][2], f0, c[e][2]);
+                st.o[i + e][3] = fmaf(st.o[i + e][3], f1, c[e][3]);
+            }
+        }
     }
+}
+
+// The item's result over its tiles so far: head h of the group of 8, dims x
+// .. x + 3 -> put(h, x, values); the sum l and the offset of s -> stat(h, l, off).
+// Lane (g, t) holds heads 2 t and 2 t + 1, dims 8 g .. 8 g + 7 of each group
+// of 64 (4 g .. 4 g + 3 of one of 32).
+template <int NB, typename Put, typename Stat>
+__device__ __forceinline__ void result(Q4State<NB> &st, int lane, Put put, Stat stat) {
+    const int gq = lane >> 2, t = lane & 3;
+    float l = st.l;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const float l0 = __shfl_sync(0xffffffffu, l, 8 * t), l1 = __shfl_sync(0xffffffffu, l, 8 * t + 4);
+    if (t == 0) stat(gq, l, st.off);
+#pragma unroll
+    for (int j = 0; j < Q4<NB>::NG; j++) {
+        float m = st.om[j];
+        m += __shfl_xor_sync(0xffffffffu, m, 1);
+        m += __shfl_xor_sync(0xffffffffu, m, 2);
+        const bool half = NB % 2 && j == Q4<NB>::NG - 1;
+#pragma unroll
+        for (int hd = 0; hd < 2; hd++) {
+            const float mm = __shfl_sync(0xffffffffu, m, 8 * t + 4 * hd), ll = hd ? l1 : l0;
+#pragma unroll
+            for (int k = 0; k < (half ? 1 : 2); k++) {
+                const float *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
+                const float4 v = make_float4(a[hd] + mm, fmaf(a[2 + hd], 0.0625f, mm), b[hd] + mm, fmaf(b[2 + hd], 0.0625f, mm));
+                put(2 * t + hd, 64 * j + (half ? 4 * gq : 8 * gq + 4 * k), v, ll);
+            }
+        }
+    }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Args g) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int sh_total[Q4_WARPS], desc[Q4_WARPS][2][5];  // a warp's parts: first unit of the item, b, j, first tile, end
+    constexpr int DH = Q4<NB>::DH, SLOT = Q4<NB>::SLOT;
+    const AttnArgs &a = g.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int G = a.H / a.Hkv, items = a.Hkv * g.HG, GH = min(G, 8);
+    pdl_wait();
+    pdl_launch_dependents();
+    // units (tiles) of the whole batch, and this CTA's and this warp's share
+    auto units_of = [&](int b) -> int {
+        const int p = seq_pos(g, b);
+        return p < 0 ? 0 : g.items_only ? items : (p / Q4_TILE + 1) * items;
+    };
+    int sum = 0;
+    for (int b = threadIdx.x; b < g.batch; b += 32 * Q4_WARPS) sum += units_of(b);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) {
+        sh_total[warp] = sum;
+        desc[warp][0][0] = desc[warp][1][0] = -1;
+    }
+    __syncthreads();
+    const int total = sh_total[0] + sh_total[1] + sh_total[2] + sh_total[3];
+    const int nC = min((int)gridDim.x, max(1, total / g.rmin));
+    if ((int)blockIdx.x >= nC || total == 0) return;
+    const int c0 = (int)((long long)blockIdx.x * total / nC), c1 = (int)((long long)(blockIdx.x + 1) * total / nC);
+    const int u0 = c0 + (int)((long long)(c1 - c0) * warp / Q4_WARPS), u1 = c0 + (int)((long long)(c1 - c0) * (warp + 1) / Q4_WARPS);
+    uint8_t *const ring = smem + warp * Q4<NB>::WARP_BYTES;
+    float *const kdm = reinterpret_cast<float *>(ring + Q4_STAGES * Q4<NB>::STAGE), *const vdm = kdm + Q4<NB>::META;
+    float *const slots = reinterpret_cast<float *>(smem + Q4_WARPS * Q4<NB>::WARP_BYTES);  // [warp][GH][SLOT]
+    const size_t hstride = (size_t)a.nsplit * (DH + 2);
+
+    if (u0 < u1) {
+        // where unit u0 lies
+        Place in;
+        in.b = 0;
+        int before = 0;
+        for (int b0 = 0; b0 < g.batch; b0 += 32) {
+            const int mine = b0 + lane < g.batch ? units_of(b0 + lane) : 0;
+            int inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, before + inc > u0);
+            if (hit) {
+                const int w = __ffs(hit) - 1;
+                in.b = b0 + w;
+                before += __shfl_sync(0xffffffffu, inc - mine, w);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        place_at(g, in);
+        const int at = u0 - before, per = g.items_only ? 1 : in.nt;
+        in.j = at / per;
+        in.tile = at % per;
+        in.left = u1 - u0;
+        Place ahead = in;
+        const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+#pragma unroll
+        for (int i = 0; i < Q4_STAGES - 1; i++) {
+            if (ahead.left > 0) {
+                fetch<NB>(g, ahead, ring_s + i * Q4<NB>::STAGE, lane);
+                next_tile(g, ahead);
+            } else {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+        }
+        Q4State<NB> st;
+        int stage = 0, fill = Q4_STAGES - 1, first_tile = -1, unit = u0, part = 0;
+        while (in.left > 0) {
+            if (first_tile < 0) {  // an item begins
+                first_tile = in.tile;
+                load_q<NB>(g, in, lane, st);
+            }
+            asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 2) : "memory");
+            __syncwarp();
+            if (ahead.left > 0) {
+                fetch<NB>(g, ahead, ring_s + fill * Q4<NB>::STAGE, lane);
+                next_tile(g, ahead);
+            } else {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+            fill = fill + 1 == Q4_STAGES ? 0 : fill + 1;
+            // rows lie at the phase that they have in the cache
+            const int t0 = in.tile * Q4_TILE, kh = in.j / g.HG;
+            int phase = 0;
+            if (!a.pages) {
+                const size_t cs = a.seq ? (size_t)__ldg(a.seq + in.b) : (size_t)in.b;
+                phase = (int)(((((long long)cs * a.Hkv + kh) * a.S + t0) * Q4<NB>::RB) & 15);
+            }
+            uint8_t *kt = ring + stage * Q4<NB>::STAGE + phase, *vt = kt + Q4<NB>::SIDE;
+            stage = stage + 1 == Q4_STAGES ? 0 : stage + 1;
+            const int n = min(Q4_TILE, in.pos + 1 - t0);
+            const bool last = in.tile == in.nt - 1;
+            if (last && a.append) {
+                append<NB>(g, in, kt + (in.pos - t0) * Q4<NB>::RB, vt + (in.pos - t0) * Q4<NB>::RB, lane);
+                __syncwarp();
+            }
+            tile<NB>(st, kt, vt, kdm, vdm, n, lane);
+            __syncwarp();  // the stage and (d, m) are read; they may be written again
+            const Place now = in;
+            next_tile(g, in);
+            if (last || in.left == 0) {  // the item, or this warp's part of it, ends
+                const int h0 = (now.j % g.HG) * 8, heads = min(8, G - h0);
+                if (first_tile == 0 && last) {
+                    float *out = a.out + (size_t)now.b * a.ldo + ((size_t)(now.j / g.HG) * G + h0) * DH;
+                    result<NB>(st, lane,
+                               [&](int h, int x, float4 v, float l) {
+                                   if (h >= heads) return;
+                                   float *o = out + h * DH + x;
+                                   const float4 r = make_float4(v.x / l, v.y / l, v.z / l, v.w / l);
+                                   if (g.vec) *reinterpret_cast<float4 *>(o) = r;
+                                   else { o[0] = r.x; o[1] = r.y; o[2] = r.z; o[3] = r.w; }
+                               },
+                               [&](int h, float, float) {
+                                   if (h < heads && a.nsplit > 1)  // nothing for the combine kernel to do
+                                       a.ws[((size_t)now.b * a.H + (size_t)(now.j / g.HG) * G + h0 + h) * hstride + DH + 1] = 0.0f;
+                               });
+                } else {
+                    float *slot = part ? reinterpret_cast<float *>(ring) : slots + warp * GH * SLOT;
+                    result<NB>(st, lane,
+                               [&](int h, int x, float4 v, float) { if (h < heads) *reinterpret_cast<float4 *>(slot + h * SLOT + x) = v; },
+                               [&](int h, float l, float off) {
+                                   if (h < heads) { slot[h * SLOT + DH] = off; slot[h * SLOT + DH + 1] = l; }
+                               });
+                    if (lane == 0) {
+                        int *d = desc[warp][part];
+                        d[0] = unit - now.tile;  // the item's first unit
+                        d[1] = now.b;
+                        d[2] = now.j;
+                        d[3] = first_tile;
+                        d[4] = now.tile + 1;
+                    }
+                }
+                part = 1;
+                first_tile = -1;
+            }
+            unit++;
+        }
+    }
+    __syncthreads();
+    // merge this CTA's parts of each item: neighbours in (warp, part) order
+    const int nw = Q4_WARPS;
+    int k = 0;
+    while (k < 2 * nw) {
+        const int *d = desc[k / 2][k % 2];
+        if (d[0] < 0) { k++; continue; }
+        int e = k;  // last part of the same item
+        for (int i = k + 1; i < 2 * nw; i++) {
+            if (desc[i / 2][i % 2][0] < 0) continue;
+            if (desc[i / 2][i % 2][0] != d[0]) break;
+            e = i;
+        }
+        const int b = d[1], j = d[2], h0 = (j % g.HG) * 8, heads = min(8, G - h0), kh = j / g.HG;
+        const int pos = seq_pos(g, b), nt = pos / Q4_TILE + 1;
+        const bool whole = d[3] == 0 && desc[e / 2][e % 2][4] == nt;
+        // the CTAs that hold the item's first and last tile
+        const int ca = (int)(((long long)(d[0] + 1) * nC - 1) / total), cb = (int)(((long long)(d[0] + nt) * nC - 1) / total);
+        for (int i = threadIdx.x; i < heads * DH; i += 32 * Q4_WARPS) {
+            const int h = i / DH, x = i % DH;
+            float M = -INFINITY, L = 0.0f, acc = 0.0f;
+            for (int q = k; q <= e; q++) {
+                if (desc[q / 2][q % 2][0] < 0) continue;
+                const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::WARP_BYTES) : slots + (q / 2) * GH * SLOT) + h * SLOT;
+                M = fmaxf(M, s[DH]);
+            }
+            for (int q = k; q <= e; q++) {
+                if (desc[q / 2][q % 2][0] < 0) continue;
+                const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::WARP_BYTES) : slots + (q / 2) * GH * SLOT) + h * SLOT;
+                const float f = ex2(s[DH] - M);
+                L = fmaf(s[DH + 1], f, L);
+                acc = fmaf(s[x], f, acc);
+            }
+            const size_t head = (size_t)kh * G + h0 + h;
+            if (whole) {
+                a.out[(size_t)b * a.ldo + head * DH + x] = acc / L;
+                if (x == 0 && a.nsplit > 1) a.ws[((size_t)b * a.H + head) * hstride + DH + 1] = 0.0f;
+            } else {
+                float *w = a.ws + ((size_t)b * a.H + head) * hstride + (size_t)((int)blockIdx.x - ca) * (DH + 2);
+                w[x] = acc;
+                if (x == 0) {
+                    w[DH] = M;
+                    // the sum; its sign bit marks the item's last part
+                    w[DH + 1] = __uint_as_float((__float_as_uint(L) & 0x7fffffffu) | ((int)blockIdx.x == cb ? 0x80000000u : 0u));
+                }
+            }
+        }
+        k = e + 1;
+    }
+}
+
+// Merges the parts of each (row, query head) that several CTAs left in the
+// workspace: one warp per head.  Nothing to do when slot 0's sum is zero.
+__global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a, int batch) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, b = (int)(id / a.H), h = (int)(id % a.H), Dh = a.Dh;
+    if (b >= batch) return;
+    const int pos = a.pos[b];
+    if (pos < 0 || pos >= a.S) return;
+    const float *w = a.ws + ((size_t)b * a.H + h) * a.nsplit * (Dh + 2);
+    if (w[Dh + 1] == 0.0f) return;
+    float M = -INFINITY;
+    int n = 0;
+    for (bool last = false; !last; n++) {
+        const float *s = w + (size_t)n * (Dh + 2) + Dh;
+        M = fmaxf(M, s[0]);
+        last = (__float_as_uint(s[1]) >> 31) || n + 1 >= a.nsplit;
+    }
+    float L = 0.0f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; i++) {
+        const float *s = w + (size_t)i * (Dh + 2);
+        const float f = ex2(s[Dh] - M);
+        L = fmaf(fabsf(s[Dh + 1]), f, L);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (lane + 32 * e < Dh) acc[e] = fmaf(s[lane + 32 * e], f, acc[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (lane + 32 * e < Dh) a.out[(size_t)b * a.ldo + (size_t)h * Dh + lane + 32 * e] = acc[e] / L;
+}
+
+template <int NB> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
+    const int GH = g.a.H / g.a.Hkv < 8 ? g.a.H / g.a.Hkv : 8;
+    const size_t smem = (size_t)Q4_WARPS * Q4<NB>::WARP_BYTES + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
+    LMC_CUDA_TRY(cudaFuncSetAttribute(k_attn_q4<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int fit = (int)(227 * 1024 / (smem + 1536)), per_sm = fit < (NB <= 4 ? 3 : 2) ? fit : (NB <= 4 ? 3 : 2);
+    const int most = lmc_sm_count() * (per_sm > 0 ? per_sm : 1), want = max_units / g.rmin;
+    LMC_LAUNCH("attention (4-bit rows)", k_attn_q4<NB>, want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);
+    return LMC_OK;
 }
 
 }  // namespace
 
-extern "C" int lmc_attention_q4_launch(const AttnArgs *a, int batch, size_t ws_bytes, cudaStream_t s) {
-    (void)ws_bytes;
-    LMC_LAUNCH("attention (4-bit rows)", k_attn_q4, dim3(a->H, batch), 128, 0, s, *a);
+extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t ws_bytes, cudaStream_t s) {
+    Q4Args g;
+    g.a = *args;
+    AttnArgs &a = g.a;
+    // one part per head and workspace slot: the most slots that fit, up to the plan's
+    int CH;
+    lmc_attn_plan(a.S, batch * a.H, 1, &CH, &a.nsplit);
+    const size_t slot = (size_t)batch * a.H * (a.Dh + 2) * sizeof(float);
+    if ((size_t)a.nsplit * slot > ws_bytes) a.nsplit = (int)(ws_bytes / slot);
+    if (a.nsplit < 2 || !a.ws) a.nsplit = 1;
+    const int G = a.H / a.Hkv, NT = (a.S + Q4_TILE - 1) / Q4_TILE;
+    g.HG = (G + 7) / 8;
+    g.batch = batch;
+    g.items_only = a.nsplit == 1;
+    // an item of NT tiles then lies in at most (NT - 2) / rmin + 2 <= nsplit CTAs
+    g.rmin = g.items_only || NT < 2 ? 1 : (NT - 2) / (a.nsplit - 1) + 1;
+    g.vec = (((uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.out) & 15) == 0 && a.ldq % 4 == 0 &&
+            a.ldkv % 4 == 0 && a.ldo % 4 == 0;
+    const long long units = (long long)batch * a.Hkv * g.HG * (g.items_only ? 1 : NT);
+    if (units > 0x7fffffffLL) return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: batch %d x context %d is too large", batch, a.S);
+    int (*const fn[8])(const Q4Args &, int, cudaStream_t) = {launch<1>, launch<2>, launch<3>, launch<4>, launch<5>, launch<6>, launch<7>, launch<8>};
+    const int rc = fn[a.Dh / 32 - 1](g, (int)units, s);
+    if (rc != LMC_OK || a.nsplit == 1) return rc;
+    LMC_LAUNCH("attention combine (4-bit rows)", k_q4_combine, lmc_cdiv((size_t)batch * a.H, 4), 128, 0, s, a, batch);
     return LMC_OK;
 }
 
