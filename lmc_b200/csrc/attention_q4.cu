@@ -56,7 +56,8 @@ template <int NB> struct Q4 {
     static constexpr int SIDE = Q4_TILE * RB + 16;        // a tile's K or V rows, from any 4-byte phase
     static constexpr int STAGE = 2 * SIDE;
     static constexpr int META = Q4_TILE * NG * 2;         // floats: (d, m) of a tile's rows, one side
-    static constexpr int WARP_BYTES = Q4_STAGES * STAGE + 2 * META * 4;
+    static constexpr int FRESH = (2 * RB + 15) / 16 * 16; // the new K and V rows
+    static constexpr int WARP_BYTES = Q4_STAGES * STAGE + 2 * META * 4 + FRESH;
     static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, offset, sum)
     static_assert(Q4_STAGES * STAGE >= 8 * SLOT * 4, "a partial result fits the ring that it is kept in");
 };
@@ -81,79 +82,111 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t 
 }
 
 // Eight codes of a word, less 8, as fp16 pairs: nibbles (0, 4), 16 x (1, 5), (2, 6), 16 x (3, 7).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t h2sub(uint32_t x, uint32_t y) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&y));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&c)[4]) {
     const uint32_t w8 = w >> 8;
-    c[0] = h2sub((w & 0x000f000fu) | 0x64006400u, 0x64086408u);
-    c[1] = h2sub((w & 0x00f000f0u) | 0x64006400u, 0x64806480u);
-    c[2] = h2sub((w8 & 0x000f000fu) | 0x64006400u, 0x64086408u);
-    c[3] = h2sub((w8 & 0x00f000f0u) | 0x64006400u, 0x64806480u);
+    c[0] = h2sub(and_or(w, 0x000f000fu, 0x64006400u), 0x64086408u);
+    c[1] = h2sub(and_or(w, 0x00f000f0u, 0x64006400u), 0x64806480u);
+    c[2] = h2sub(and_or(w8, 0x000f000fu, 0x64006400u), 0x64086408u);
+    c[3] = h2sub(and_or(w8, 0x00f000f0u, 0x64006400u), 0x64806480u);
 }
 
 // A place in the batch's order of tiles: sequences, their (kv head, head
 // group) items, the item's tiles.
 struct Place {
     int b, j, tile, nt, pos, left;  // left: units still to go (tiles, or items with items_only)
+    int kh;
+    long long off;   // contiguous: byte offset of the item's row 0 in a cache
+    const int *row;  // paged: the sequence's table row
 };
 __device__ __forceinline__ int seq_pos(const Q4Args &g, int b) {  // position, or -1 when the row has nothing to do
     const int p = __ldg(g.a.pos + b);
     return p < 0 || p >= g.a.S ? -1 : p;
 }
-__device__ __forceinline__ void place_at(const Q4Args &g, Place &p) {  // first sequence >= p.b with work
+template <int RB> __device__ __forceinline__ void set_item(const Q4Args &g, Place &p) {
+    p.kh = g.HG == 1 ? p.j : p.j / g.HG;
+    const long long cs = g.a.seq ? __ldg(g.a.seq + p.b) : p.b;
+    p.row = g.a.pages + cs * g.a.max_pages;
+    p.off = (cs * g.a.Hkv + p.kh) * g.a.S * RB;
+}
+__device__ __forceinline__ void set_seq(const Q4Args &g, Place &p) {  // first sequence >= p.b with work
     p.pos = -1;
     while (p.b < g.batch && (p.pos = seq_pos(g, p.b)) < 0) p.b++;
     p.nt = p.pos / Q4_TILE + 1;
 }
-__device__ __forceinline__ void next_tile(const Q4Args &g, Place &p) {
+template <int RB> __device__ __forceinline__ void next_tile(const Q4Args &g, Place &p) {
     p.tile++;
     if (!g.items_only) p.left--;
     if (p.tile < p.nt) return;
     p.tile = 0;
     p.j++;
     if (g.items_only) p.left--;
-    if (p.j < g.a.Hkv * g.HG) return;
-    p.j = 0;
-    p.b++;
-    place_at(g, p);
+    if (p.left <= 0) return;
+    if (p.j == g.a.Hkv * g.HG) {
+        p.j = 0;
+        p.b++;
+        set_seq(g, p);
+    }
+    set_item<RB>(g, p);
 }
 
-// Byte offset of row t (the start of a run within one page) in its cache.
-__device__ __forceinline__ long long run_offset(const AttnArgs &a, size_t cs, int kh, int t, int RB, bool *ok) {
-    if (!a.pages) return (((long long)cs * a.Hkv + kh) * a.S + t) * RB;
-    int pg = __ldg(a.pages + cs * a.max_pages + (t >> a.page_shift));
-    *ok = pg >= 0 && pg < a.n_pages;
-    if (!*ok) {
+// Byte offset of row t of the item in its cache; *ok: its page is in the pool (page 0 is taken if not).
+template <int RB> __device__ __forceinline__ long long row_offset(const AttnArgs &a, const Place &p, int t, bool *ok) {
+    if (!a.pages) return p.off + (long long)t * RB;
+    int pg = __ldg(p.row + (t >> a.page_shift));
+    if (pg < 0 || pg >= a.n_pages) {
         atomicExch(&g_attn_q4_err, 1);
+        *ok = false;
         pg = 0;
     }
-    return ((((long long)pg * a.Hkv + kh) << a.page_shift) + (t & ((1 << a.page_shift) - 1))) * RB;
+    return (((long long)pg * a.Hkv + p.kh) << a.page_shift) * RB + (t & ((1 << a.page_shift) - 1)) * RB;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t *src, int n = 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_run(uint32_t dst, const uint8_t *src, int bytes, int lane) {
     // from the 16-byte boundary at or before src; the last copy reads no byte past the run
     const int phase = (int)((uintptr_t)src & 15);
-    const uint8_t *from = src - phase;
-    for (int i = 16 * lane; i < bytes + phase; i += 512) {
-        const int n = min(16, bytes + phase - i);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i), "l"(from + i), "r"(n) : "memory");
-    }
+    for (int i = 16 * lane; i < bytes + phase; i += 512) cp16(dst + i, src - phase + i, min(16, bytes + phase - i));
 }
 // Starts the copies of a tile's rows (all but the new row) and closes their group.
 template <int NB>
 __device__ __forceinline__ void fetch(const Q4Args &g, const Place &p, uint32_t stage, int lane) {
     const AttnArgs &a = g.a;
-    constexpr int RB = Q4<NB>::RB;
-    const int t0 = p.tile * Q4_TILE, rows = min(Q4_TILE, (a.append ? p.pos : p.pos + 1) - t0), kh = p.j / g.HG;
-    const size_t cs = a.seq ? (size_t)__ldg(a.seq + p.b) : (size_t)p.b;
-    const int run = a.pages && a.page_shift == 4 ? 16 : Q4_TILE;  // rows that lie one behind the other
-    for (int r = 0; r < rows; r += run) {
+    constexpr int RB = Q4<NB>::RB, CH = 2 * RB;  // 16-byte pieces of a whole tile
+    const int t0 = p.tile * Q4_TILE, rows = min(Q4_TILE, (a.append ? p.pos : p.pos + 1) - t0);
+    if (rows > 0) {
         bool ok;
-        const long long off = run_offset(a, cs, kh, t0 + r, RB, &ok);
-        const int bytes = min(run, rows - r) * RB;
-        copy_run(stage + r * RB, (const uint8_t *)a.k_cache + off, bytes, lane);
-        copy_run(stage + Q4<NB>::SIDE + r * RB, (const uint8_t *)a.v_cache + off, bytes, lane);
+        const bool two = a.pages && a.page_shift == 4;  // 16 rows to a page
+        const long long off0 = row_offset<RB>(a, p, t0, &ok);
+        const long long off1 = two && rows > 16 ? row_offset<RB>(a, p, t0 + 16, &ok) - 16 * RB : off0;
+        const uint8_t *kc = (const uint8_t *)a.k_cache, *vc = (const uint8_t *)a.v_cache;
+        if (rows == Q4_TILE && !(off0 & 15)) {
+#pragma unroll
+            for (int i = 0; i < (CH + 31) / 32; i++) {
+                const int c = lane + 32 * i;
+                const long long at = (c < CH / 2 ? off0 : off1) + 16 * c;
+                if (c < CH) {
+                    cp16(stage + 16 * c, kc + at);
+                    cp16(stage + Q4<NB>::SIDE + 16 * c, vc + at);
+                }
+            }
+        } else {
+            for (int r = 0; r < rows; r += two ? 16 : Q4_TILE) {
+                const long long at = r ? off1 + 16 * RB : off0;
+                const int bytes = min(two ? 16 : Q4_TILE, rows - r) * RB;
+                copy_run(stage + r * RB, kc + at, bytes, lane);
+                copy_run(stage + Q4<NB>::SIDE + r * RB, vc + at, bytes, lane);
+            }
+        }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -193,13 +226,13 @@ template <int NB>
 __device__ __forceinline__ void load_q(const Q4Args &g, const Place &p, int lane, Q4State<NB> &st) {
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH;
-    const int G = a.H / a.Hkv, kh = p.j / g.HG, head = (p.j % g.HG) * 8 + (lane >> 2), t = lane & 3;
+    const int G = a.H / a.Hkv, head = (p.j - p.kh * g.HG) * 8 + (lane >> 2), t = lane & 3;
     float x[NB][8];
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
         if (head < G) {
-            load8(a.q + (size_t)p.b * a.ldq + ((size_t)kh * G + head) * DH + 32 * i + 8 * t, g.vec, x[i]);
+            load8(a.q + (size_t)p.b * a.ldq + ((size_t)p.kh * G + head) * DH + 32 * i + 8 * t, g.vec, x[i]);
             rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
         } else {
 #pragma unroll
@@ -241,37 +274,52 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Place &p, int lane
     st.vexp = 0;
 }
 
-// The new K and V rows quantized into the tile (and, by the first head group,
-// into the cache).
-template <int NB>
-__device__ __forceinline__ void append(const Q4Args &g, const Place &p, uint8_t *krow, uint8_t *vrow, int lane) {
+// The new K and V rows quantized into `fresh` (two rows) and, by the first
+// head group, into the cache.
+template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const Place &p, uint32_t *fresh, int lane) {
     const AttnArgs &a = g.a;
-    constexpr int DH = Q4<NB>::DH, NW = DH / 8;
-    const int kh = p.j / g.HG;
+    constexpr int DH = Q4<NB>::DH, NW = DH / 8, RB = Q4<NB>::RB;
+    float x[2][8];
 #pragma unroll
     for (int side = 0; side < 2; side++) {
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (lane < NW) {
-            load8((side ? a.v_new : a.k_new) + (size_t)p.b * a.ldkv + (size_t)kh * DH + 8 * lane, g.vec, x);
-            if (!side) rope8(a, p.pos, DH, 8 * lane, x);
-        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[side][e] = 0.0f;
+        if (lane < NW) load8((side ? a.v_new : a.k_new) + (size_t)p.b * a.ldkv + (size_t)p.kh * DH + 8 * lane, g.vec, x[side]);
+    }
+    if (lane < NW) rope8(a, p.pos, DH, 8 * lane, x[0]);
+    bool ok = true;
+    const long long off = row_offset<RB>(a, p, p.pos, &ok);
+    ok &= p.j == p.kh * g.HG;
+#pragma unroll 1
+    for (int side = 0; side < 2; side++) {
         uint32_t codes, dm;
-        kv_q4_quantize<32>(x, lane < NW, codes, dm);
-        uint32_t *row = reinterpret_cast<uint32_t *>(side ? vrow : krow);
+        kv_q4_quantize<32>(x[0], lane < NW, codes, dm);
+        uint32_t *dst = reinterpret_cast<uint32_t *>((uint8_t *)(side ? a.v_cache : a.k_cache) + off);
         if (lane < NW) {
-            row[lane] = codes;
-            if (lane % 8 == 0) row[NW + lane / 8] = dm;
-        }
-        if (p.j % g.HG == 0) {
-            bool ok = true;
-            const size_t cs = a.seq ? (size_t)__ldg(a.seq + p.b) : (size_t)p.b;
-            const long long off = run_offset(a, cs, kh, p.pos, Q4<NB>::RB, &ok);
-            uint32_t *dst = reinterpret_cast<uint32_t *>((uint8_t *)(side ? a.v_cache : a.k_cache) + off);
-            if (ok && lane < NW) {
-                dst[lane] = codes;
-                if (lane % 8 == 0) dst[NW + lane / 8] = dm;
+            fresh[side * (RB / 4) + lane] = codes;
+            if (ok) dst[lane] = codes;
+            if (lane % 8 == 0) {
+                fresh[side * (RB / 4) + NW + lane / 8] = dm;
+                if (ok) dst[NW + lane / 8] = dm;
             }
         }
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[0][e] = x[1][e];
+    }
+}
+
+// The NG pairs (d, m') of one row.
+template <int NG> __device__ __forceinline__ void load_dm(const float *p, float2 (&f)[NG]) {
+    if constexpr (NG % 2 == 0) {
+#pragma unroll
+        for (int j = 0; j < NG; j += 2) {
+            const float4 v = *reinterpret_cast<const float4 *>(p + 2 * j);
+            f[j] = make_float2(v.x, v.y);
+            f[j + 1] = make_float2(v.z, v.w);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NG; j++) f[j] = *reinterpret_cast<const float2 *>(p + 2 * j);
     }
 }
 
@@ -317,13 +365,13 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {  // columns 2 t, 2 t + 1: rows 4 t + par, 4 t + 2 + par
-                const float *dm = kdm + 2 * NG * (16 * h + 4 * t + 2 * e + par);
-                float x = 0.0f, y = 0.0f;
+                float2 dm[NG];
+                load_dm<NG>(kdm + 2 * NG * (16 * h + 4 * t + 2 * e + par), dm);
+                float x = dm[0].x * (c[0][e] + c[0][2 + e]), y = dm[0].y * st.qsum[0];
 #pragma unroll
-                for (int j = 0; j < NG; j++) {
-                    const float2 f = *reinterpret_cast<const float2 *>(dm + 2 * j);
-                    x = fmaf(f.x, c[j][e] + c[j][2 + e], x);
-                    y = fmaf(f.y, st.qsum[j], y);
+                for (int j = 1; j < NG; j++) {
+                    x = fmaf(dm[j].x, c[j][e] + c[j][2 + e], x);
+                    y = fmaf(dm[j].y, st.qsum[j], y);
                 }
                 s[h][2 * e + par] = fmaf(x, st.qfac, y);
             }
@@ -354,22 +402,30 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
             s[h][r] = ex2(s[h][r] - off);
             st.l += s[h][r];
         }
+    uint32_t bh[NG][2][2], bl[NG][2][2];  // p d of the 16 rows of each half: hi, lo
+#pragma unroll
+    for (int j = 0; j < NG; j++) st.om[j] *= f;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float w[NG][4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            float2 dm[NG];
+            load_dm<NG>(vdm + 2 * NG * (16 * h + 4 * t + r), dm);
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                w[j][r] = s[h][r] * dm[j].x;
+                st.om[j] = fmaf(s[h][r], dm[j].y, st.om[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            split2(w[j][0], w[j][2], bh[j][h][0], bl[j][h][0]);
+            split2(w[j][1], w[j][3], bh[j][h][1], bl[j][h][1]);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        uint32_t bh[2][2], bl[2][2];  // p d of the 16 rows of each half: hi, lo
-        st.om[j] *= f;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float w[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float2 dm = *reinterpret_cast<const float2 *>(vdm + 2 * (NG * (16 * h + 4 * t + r) + j));
-                w[r] = s[h][r] * dm.x;
-                st.om[j] = fmaf(s[h][r], dm.y, st.om[j]);
-            }
-            split2(w[0], w[2], bh[h][0], bl[h][0]);
-            split2(w[1], w[3], bh[h][1], bl[h][1]);
-        }
         // this lane's dims: word g of the group, or half a word of a group of 32
         const bool half = NB % 2 && j == NG - 1;
         const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
@@ -390,10 +446,10 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
                 uint32_t x[4], y[4];  // rows 4 t + (0, 2) and (1, 3)
                 codes8(__byte_perm(cw[h][0], cw[h][2], sel), x);
                 codes8(__byte_perm(cw[h][1], cw[h][3], sel), y);
-                hmma(c[0], x[0], x[1], y[0], y[1], bh[h][0], bh[h][1]);
-                hmma(c[1], x[2], x[3], y[2], y[3], bh[h][0], bh[h][1]);
-                hmma(c[0], x[0], x[1], y[0], y[1], bl[h][0], bl[h][1]);
-                hmma(c[1], x[2], x[3], y[2], y[3], bl[h][0], bl[h][1]);
+                hmma(c[0], x[0], x[1], y[0], y[1], bh[j][h][0], bh[j][h][1]);
+                hmma(c[1], x[2], x[3], y[2], y[3], bh[j][h][0], bh[j][h][1]);
+                hmma(c[0], x[0], x[1], y[0], y[1], bl[j][h][0], bl[j][h][1]);
+                hmma(c[1], x[2], x[3], y[2], y[3], bl[j][h][0], bl[j][h][1]);
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -406,32 +462,40 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
     }
 }
 
-// The item's result over its tiles so far: head h of the group of 8, dims x
-// .. x + 3 -> put(h, x, values); the sum l and the offset of s -> stat(h, l, off).
-// Lane (g, t) holds heads 2 t and 2 t + 1, dims 8 g .. 8 g + 7 of each group
-// of 64 (4 g .. 4 g + 3 of one of 32).
-template <int NB, typename Put, typename Stat>
-__device__ __forceinline__ void result(Q4State<NB> &st, int lane, Put put, Stat stat) {
+// The item's result over its tiles so far, to dst + h * ld (heads h < heads
+// of the group of 8): with fin divided by the sum; else as it is, with the
+// offset of s and the sum behind it.  Lane (g, t) holds heads 2 t and 2 t + 1,
+// dims 8 g .. 8 g + 7 of each group of 64 (4 g .. 4 g + 3 of one of 32).
+template <int NB>
+__device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
     const int gq = lane >> 2, t = lane & 3;
     float l = st.l;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    const float l0 = __shfl_sync(0xffffffffu, l, 8 * t), l1 = __shfl_sync(0xffffffffu, l, 8 * t + 4);
-    if (t == 0) stat(gq, l, st.off);
+    if (!fin && t == 0 && gq < heads) {
+        dst[gq * ld + Q4<NB>::DH] = st.off;
+        dst[gq * ld + Q4<NB>::DH + 1] = l;
+    }
+    const float inv = fin ? 1.0f / l : 1.0f;
 #pragma unroll
-    for (int j = 0; j < Q4<NB>::NG; j++) {
-        float m = st.om[j];
-        m += __shfl_xor_sync(0xffffffffu, m, 1);
-        m += __shfl_xor_sync(0xffffffffu, m, 2);
-        const bool half = NB % 2 && j == Q4<NB>::NG - 1;
+    for (int hd = 0; hd < 2; hd++) {
+        const int from = 8 * t + 4 * hd, h = 2 * t + hd;
+        const float iv = __shfl_sync(0xffffffffu, inv, from);
 #pragma unroll
-        for (int hd = 0; hd < 2; hd++) {
-            const float mm = __shfl_sync(0xffffffffu, m, 8 * t + 4 * hd), ll = hd ? l1 : l0;
+        for (int j = 0; j < Q4<NB>::NG; j++) {
+            float m = st.om[j];
+            m += __shfl_xor_sync(0xffffffffu, m, 1);
+            m += __shfl_xor_sync(0xffffffffu, m, 2);
+            m = __shfl_sync(0xffffffffu, m, from);
+            const bool half = NB % 2 && j == Q4<NB>::NG - 1;
 #pragma unroll
             for (int k = 0; k < (half ? 1 : 2); k++) {
                 const float *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
-                const float4 v = make_float4(a[hd] + mm, fmaf(a[2 + hd], 0.0625f, mm), b[hd] + mm, fmaf(b[2 + hd], 0.0625f, mm));
-                put(2 * t + hd, 64 * j + (half ? 4 * gq : 8 * gq + 4 * k), v, ll);
+                const float4 v = make_float4((a[hd] + m) * iv, fmaf(a[2 + hd], 0.0625f, m) * iv, (b[hd] + m) * iv, fmaf(b[2 + hd], 0.0625f, m) * iv);
+                float *o = dst + h * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
+                if (h >= heads) continue;
+                if (vec) *reinterpret_cast<float4 *>(o) = v;
+                else { o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w; }
             }
         }
     }
@@ -441,7 +505,7 @@ template <int NB>
 __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Args g) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int sh_total[Q4_WARPS], desc[Q4_WARPS][2][5];  // a warp's parts: first unit of the item, b, j, first tile, end
-    constexpr int DH = Q4<NB>::DH, SLOT = Q4<NB>::SLOT;
+    constexpr int DH = Q4<NB>::DH, SLOT = Q4<NB>::SLOT, RB = Q4<NB>::RB;
     const AttnArgs &a = g.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = a.H / a.Hkv, items = a.Hkv * g.HG, GH = min(G, 8);
@@ -467,6 +531,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Ar
     const int u0 = c0 + (int)((long long)(c1 - c0) * warp / Q4_WARPS), u1 = c0 + (int)((long long)(c1 - c0) * (warp + 1) / Q4_WARPS);
     uint8_t *const ring = smem + warp * Q4<NB>::WARP_BYTES;
     float *const kdm = reinterpret_cast<float *>(ring + Q4_STAGES * Q4<NB>::STAGE), *const vdm = kdm + Q4<NB>::META;
+    uint32_t *const fresh = reinterpret_cast<uint32_t *>(vdm + Q4<NB>::META);
     float *const slots = reinterpret_cast<float *>(smem + Q4_WARPS * Q4<NB>::WARP_BYTES);  // [warp][GH][SLOT]
     const size_t hstride = (size_t)a.nsplit * (DH + 2);
 
@@ -492,93 +557,69 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Ar
             }
             before += __shfl_sync(0xffffffffu, inc, 31);
         }
-        place_at(g, in);
+        set_seq(g, in);
         const int at = u0 - before, per = g.items_only ? 1 : in.nt;
         in.j = at / per;
         in.tile = at % per;
         in.left = u1 - u0;
+        set_item<RB>(g, in);
         Place ahead = in;
         const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-#pragma unroll
-        for (int i = 0; i < Q4_STAGES - 1; i++) {
-            if (ahead.left > 0) {
-                fetch<NB>(g, ahead, ring_s + i * Q4<NB>::STAGE, lane);
-                next_tile(g, ahead);
-            } else {
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
-        }
+        int fill = 0, stage = 0, first_tile = -1, unit = u0, part = 0, phase = 0;
         Q4State<NB> st;
-        int stage = 0, fill = Q4_STAGES - 1, first_tile = -1, unit = u0, part = 0;
-        while (in.left > 0) {
-            if (first_tile < 0) {  // an item begins
-                first_tile = in.tile;
-                load_q<NB>(g, in, lane, st);
-            }
-            asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 2) : "memory");
-            __syncwarp();
+#pragma unroll 1
+        for (int skip = Q4_STAGES - 1; in.left > 0; skip--) {  // the first turns only start copies
             if (ahead.left > 0) {
                 fetch<NB>(g, ahead, ring_s + fill * Q4<NB>::STAGE, lane);
-                next_tile(g, ahead);
+                next_tile<RB>(g, ahead);
             } else {
                 asm volatile("cp.async.commit_group;" ::: "memory");
             }
             fill = fill + 1 == Q4_STAGES ? 0 : fill + 1;
-            // rows lie at the phase that they have in the cache
-            const int t0 = in.tile * Q4_TILE, kh = in.j / g.HG;
-            int phase = 0;
-            if (!a.pages) {
-                const size_t cs = a.seq ? (size_t)__ldg(a.seq + in.b) : (size_t)in.b;
-                phase = (int)(((((long long)cs * a.Hkv + kh) * a.S + t0) * Q4<NB>::RB) & 15);
+            if (skip > 0) continue;
+            if (first_tile < 0) {  // an item begins
+                first_tile = in.tile;
+                phase = a.pages ? 0 : (int)(in.off & 15);  // rows lie in the ring at the phase that they have in the cache
+                if (a.append && (g.items_only || in.left >= in.nt - in.tile)) append<NB>(g, in, fresh, lane);
+                load_q<NB>(g, in, lane, st);
             }
+            asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 1) : "memory");
+            __syncwarp();
             uint8_t *kt = ring + stage * Q4<NB>::STAGE + phase, *vt = kt + Q4<NB>::SIDE;
             stage = stage + 1 == Q4_STAGES ? 0 : stage + 1;
-            const int n = min(Q4_TILE, in.pos + 1 - t0);
+            const int n = min(Q4_TILE, in.pos + 1 - in.tile * Q4_TILE);
             const bool last = in.tile == in.nt - 1;
             if (last && a.append) {
-                append<NB>(g, in, kt + (in.pos - t0) * Q4<NB>::RB, vt + (in.pos - t0) * Q4<NB>::RB, lane);
+                for (int i = lane; i < RB / 4; i += 32) {
+                    reinterpret_cast<uint32_t *>(kt + (n - 1) * RB)[i] = fresh[i];
+                    reinterpret_cast<uint32_t *>(vt + (n - 1) * RB)[i] = fresh[RB / 4 + i];
+                }
                 __syncwarp();
             }
             tile<NB>(st, kt, vt, kdm, vdm, n, lane);
-            __syncwarp();  // the stage and (d, m) are read; they may be written again
-            const Place now = in;
-            next_tile(g, in);
-            if (last || in.left == 0) {  // the item, or this warp's part of it, ends
-                const int h0 = (now.j % g.HG) * 8, heads = min(8, G - h0);
-                if (first_tile == 0 && last) {
-                    float *out = a.out + (size_t)now.b * a.ldo + ((size_t)(now.j / g.HG) * G + h0) * DH;
-                    result<NB>(st, lane,
-                               [&](int h, int x, float4 v, float l) {
-                                   if (h >= heads) return;
-                                   float *o = out + h * DH + x;
-                                   const float4 r = make_float4(v.x / l, v.y / l, v.z / l, v.w / l);
-                                   if (g.vec) *reinterpret_cast<float4 *>(o) = r;
-                                   else { o[0] = r.x; o[1] = r.y; o[2] = r.z; o[3] = r.w; }
-                               },
-                               [&](int h, float, float) {
-                                   if (h < heads && a.nsplit > 1)  // nothing for the combine kernel to do
-                                       a.ws[((size_t)now.b * a.H + (size_t)(now.j / g.HG) * G + h0 + h) * hstride + DH + 1] = 0.0f;
-                               });
-                } else {
-                    float *slot = part ? reinterpret_cast<float *>(ring) : slots + warp * GH * SLOT;
-                    result<NB>(st, lane,
-                               [&](int h, int x, float4 v, float) { if (h < heads) *reinterpret_cast<float4 *>(slot + h * SLOT + x) = v; },
-                               [&](int h, float l, float off) {
-                                   if (h < heads) { slot[h * SLOT + DH] = off; slot[h * SLOT + DH + 1] = l; }
-                               });
-                    if (lane == 0) {
-                        int *d = desc[warp][part];
-                        d[0] = unit - now.tile;  // the item's first unit
-                        d[1] = now.b;
-                        d[2] = now.j;
-                        d[3] = first_tile;
-                        d[4] = now.tile + 1;
-                    }
+            __syncwarp();  // the stage and (d, m') are read; they may be written again
+            if (last || (!g.items_only && in.left == 1)) {  // the item, or this warp's part of it, ends
+                const int h0 = (in.j - in.kh * g.HG) * 8, heads = min(8, G - h0);
+                const size_t head = (size_t)in.kh * G + h0;
+                const bool whole = first_tile == 0 && last;
+                float *slot = part ? reinterpret_cast<float *>(ring) : slots + warp * GH * SLOT;
+                result<NB>(st, lane, whole ? a.out + (size_t)in.b * a.ldo + head * DH : slot, whole ? DH : SLOT, heads, whole, !whole || g.vec);
+                if (whole) {
+                    if (lane < heads && a.nsplit > 1)  // nothing for the combine kernel to do
+                        a.ws[((size_t)in.b * a.H + head + lane) * hstride + DH + 1] = 0.0f;
+                } else if (lane == 0) {
+                    int *d = desc[warp][part];
+                    d[0] = unit - in.tile;  // the item's first unit
+                    d[1] = in.b;
+                    d[2] = in.j;
+                    d[3] = first_tile;
+                    d[4] = in.tile + 1;
                 }
                 part = 1;
                 first_tile = -1;
             }
             unit++;
+            next_tile<RB>(g, in);
         }
     }
     __syncthreads();
@@ -633,36 +674,72 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Ar
 }
 
 // Merges the parts of each (row, query head) that several CTAs left in the
-// workspace: one warp per head.  Nothing to do when slot 0's sum is zero.
-__global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a, int batch) {
+// workspace; nothing to do when slot 0's sum is zero.  W warps (1 or 4) share
+// a head's parts: four when there are few heads, whose parts are then many
+// (131072 positions of one sequence: 56 for each of 32 heads).
+template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a, int batch) {
     pdl_wait();
     pdl_launch_dependents();
-    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, b = (int)(id / a.H), h = (int)(id % a.H), Dh = a.Dh;
+    __shared__ float sh[W == 1 ? 1 : 4][256];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long id = W == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
+    const int b = (int)(id / a.H), h = (int)(id % a.H), Dh = a.Dh;
     if (b >= batch) return;
     const int pos = a.pos[b];
     if (pos < 0 || pos >= a.S) return;
     const float *w = a.ws + ((size_t)b * a.H + h) * a.nsplit * (Dh + 2);
-    if (w[Dh + 1] == 0.0f) return;
-    float M = -INFINITY;
-    int n = 0;
-    for (bool last = false; !last; n++) {
-        const float *s = w + (size_t)n * (Dh + 2) + Dh;
-        M = fmaxf(M, s[0]);
-        last = (__float_as_uint(s[1]) >> 31) || n + 1 >= a.nsplit;
+    // offsets and sums of all slots (at most 64); slots past the last part hold anything
+    float m[2], l[2];
+    int n = a.nsplit;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int k = lane + 32 * i;
+        m[i] = k < a.nsplit ? w[(size_t)k * (Dh + 2) + Dh] : 0.0f;
+        l[i] = k < a.nsplit ? w[(size_t)k * (Dh + 2) + Dh + 1] : 0.0f;
     }
-    float L = 0.0f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < n; i++) {
-        const float *s = w + (size_t)i * (Dh + 2);
-        const float f = ex2(s[Dh] - M);
-        L = fmaf(fabsf(s[Dh + 1]), f, L);
+    if (__shfl_sync(0xffffffffu, l[0], 0) == 0.0f) return;
+#pragma unroll
+    for (int i = 1; i >= 0; i--) {
+        const unsigned last = __ballot_sync(0xffffffffu, __float_as_uint(l[i]) >> 31);
+        if (last) n = min(n, 32 * i + __ffs(last));
+    }
+    float M = fmaxf(lane < n ? m[0] : -INFINITY, lane + 32 < n ? m[1] : -INFINITY);
+    M = warp_max(M);
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) f[i] = lane + 32 * i < n ? ex2(m[i] - M) : 0.0f;
+    const float L = warp_sum((lane < n ? fabsf(l[0]) * f[0] : 0.0f) + (lane + 32 < n ? fabsf(l[1]) * f[1] : 0.0f));
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int k0 = W == 1 ? 0 : warp; k0 < n; k0 += 4 * W) {  // four parts' loads at a time
+        float v[4][8];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int k = k0 + u * W;
+                v[u][e] = k < n && lane + 32 * e < Dh ? w[(size_t)k * (Dh + 2) + lane + 32 * e] : 0.0f;
+            }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int k = k0 + u * W;
+            const float fk = __shfl_sync(0xffffffffu, (k & 32) ? f[1] : f[0], k & 31);
+            if (k < n)
+#pragma unroll
+                for (int e = 0; e < 8; e++) acc[e] = fmaf(v[u][e], fk, acc[e]);
+        }
+    }
+    float *out = a.out + (size_t)b * a.ldo + (size_t)h * Dh;
+    if constexpr (W == 1) {
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            if (lane + 32 * e < Dh) acc[e] = fmaf(s[lane + 32 * e], f, acc[e]);
-    }
+            if (lane + 32 * e < Dh) out[lane + 32 * e] = acc[e] / L;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-        if (lane + 32 * e < Dh) a.out[(size_t)b * a.ldo + (size_t)h * Dh + lane + 32 * e] = acc[e] / L;
+        for (int e = 0; e < 8; e++)
+            if (lane + 32 * e < Dh) sh[warp][lane + 32 * e] = acc[e];
+        __syncthreads();
+        for (int d = threadIdx.x; d < Dh; d += 128) out[d] = (sh[0][d] + sh[1][d] + sh[2][d] + sh[3][d]) / L;
+    }
 }
 
 template <int NB> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
@@ -700,7 +777,9 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     int (*const fn[8])(const Q4Args &, int, cudaStream_t) = {launch<1>, launch<2>, launch<3>, launch<4>, launch<5>, launch<6>, launch<7>, launch<8>};
     const int rc = fn[a.Dh / 32 - 1](g, (int)units, s);
     if (rc != LMC_OK || a.nsplit == 1) return rc;
-    LMC_LAUNCH("attention combine (4-bit rows)", k_q4_combine, lmc_cdiv((size_t)batch * a.H, 4), 128, 0, s, a, batch);
+    const size_t heads = (size_t)batch * a.H;
+    if (heads <= 1024) LMC_LAUNCH("attention combine (4-bit rows)", k_q4_combine<4>, heads, 128, 0, s, a, batch);
+    else LMC_LAUNCH("attention combine (4-bit rows)", k_q4_combine<1>, lmc_cdiv(heads, 4), 128, 0, s, a, batch);
     return LMC_OK;
 }
 
