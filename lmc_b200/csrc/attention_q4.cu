@@ -40,7 +40,15 @@ __device__ int g_attn_q4_err;  // a page id outside the pool was met (lmc_device
 
 constexpr int Q4_WARPS = 4;
 constexpr int Q4_TILE = 32;    // positions per tile
-constexpr int Q4_STAGES = 3;   // tiles in a warp's ring
+#ifndef Q4_ST
+#define Q4_ST 3
+#define Q4_MB 3
+#endif
+constexpr int Q4_STAGES = Q4_ST;   // tiles in a warp's ring
+#ifndef Q4_SETUP
+#define Q4_SETUP 2
+#endif
+constexpr int Q4_ITEM = Q4_SETUP;      // what beginning and ending an item costs, in tiles
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Q4Args {
@@ -49,6 +57,7 @@ struct Q4Args {
     int rmin;       // tiles per CTA at least (workspace slots per head: a.nsplit)
     int items_only; // 1: an item is never divided (a.nsplit is 1)
     int batch, vec; // vec: q, new rows and out can be moved 16 bytes at a time
+    int page_bytes; // of one kv head's rows of a page
 };
 
 template <int NB> struct Q4 {
@@ -71,6 +80,11 @@ __device__ __forceinline__ void hmma(float (&c)[4], uint32_t a0, uint32_t a1, ui
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void hmma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // x, y as fp16 pairs hi + lo
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -100,10 +114,14 @@ __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&c)[4]) {
 }
 
 // A place in the batch's order of tiles: sequences, their (kv head, head
-// group) items, the item's tiles.
-struct Place {
-    int b, j, tile, nt, pos, left;  // left: units still to go (tiles, or items with items_only)
-    int kh;
+// group) items, the item's tiles.  Work is divided in units: an item of nt
+// tiles has Q4_ITEM + nt of them, the first ones for what its beginning and
+// end cost, so that shares with many short items are not the last to finish
+// (with items_only one unit, an item being one CTA's then).
+struct Item {
+    int b, j, kh, nt, pos;
+    int tile, end;   // this warp's tiles of the item
+    int unit, left;  // the item's first unit; units of this warp's share from there on
     long long off;   // contiguous: byte offset of the item's row 0 in a cache
     const int *row;  // paged: the sequence's table row
 };
@@ -111,84 +129,93 @@ __device__ __forceinline__ int seq_pos(const Q4Args &g, int b) {  // position, o
     const int p = __ldg(g.a.pos + b);
     return p < 0 || p >= g.a.S ? -1 : p;
 }
-template <int RB> __device__ __forceinline__ void set_item(const Q4Args &g, Place &p) {
-    p.kh = g.HG == 1 ? p.j : p.j / g.HG;
+__device__ __forceinline__ int item_units(const Q4Args &g, int nt) { return g.items_only ? 1 : nt + Q4_ITEM; }
+// The item at (p.b, p.j), p.nt and p.pos known; its tiles up to the share's end.
+template <int RB> __device__ __forceinline__ void set_item(const Q4Args &g, Item &p) {
+    p.kh = p.j / g.HG;
+    p.end = g.items_only ? (p.left > 0 ? p.nt : 0) : min(p.nt, p.left - Q4_ITEM);
     const long long cs = g.a.seq ? __ldg(g.a.seq + p.b) : p.b;
     p.row = g.a.pages + cs * g.a.max_pages;
     p.off = (cs * g.a.Hkv + p.kh) * g.a.S * RB;
 }
-__device__ __forceinline__ void set_seq(const Q4Args &g, Place &p) {  // first sequence >= p.b with work
+__device__ __forceinline__ void set_seq(const Q4Args &g, Item &p) {  // first sequence >= p.b with work
     p.pos = -1;
     while (p.b < g.batch && (p.pos = seq_pos(g, p.b)) < 0) p.b++;
     p.nt = p.pos / Q4_TILE + 1;
 }
-template <int RB> __device__ __forceinline__ void next_tile(const Q4Args &g, Place &p) {
-    p.tile++;
-    if (!g.items_only) p.left--;
-    if (p.tile < p.nt) return;
-    p.tile = 0;
-    p.j++;
-    if (g.items_only) p.left--;
-    if (p.left <= 0) return;
-    if (p.j == g.a.Hkv * g.HG) {
-        p.j = 0;
-        p.b++;
-        set_seq(g, p);
+// The share's next item, in place (tile == end: there is none).  The items of
+// the copies and of the computation lie in shared memory: only what each tile
+// needs is kept in registers.
+template <int RB> __device__ __noinline__ void next_item(const Q4Args &g, Item *at) {
+    Item p = *at;
+    const int units = item_units(g, p.nt);
+    p.unit += units;
+    p.left -= units;
+    p.tile = p.end = 0;
+    if (p.left > 0) {
+        if (++p.j == g.a.Hkv * g.HG) {
+            p.j = 0;
+            p.b++;
+            set_seq(g, p);
+        }
+        set_item<RB>(g, p);
+        p.end = max(p.end, 0);
     }
-    set_item<RB>(g, p);
+    __syncwarp();
+    *at = p;  // (every lane the same)
+    __syncwarp();
 }
 
-// Byte offset of row t of the item in its cache; *ok: its page is in the pool (page 0 is taken if not).
-template <int RB> __device__ __forceinline__ long long row_offset(const AttnArgs &a, const Place &p, int t, bool *ok) {
-    if (!a.pages) return p.off + (long long)t * RB;
-    int pg = __ldg(p.row + (t >> a.page_shift));
-    if (pg < 0 || pg >= a.n_pages) {
+// Byte offset of row t of an item in its cache; *ok: its page is in the pool (page 0 is taken if not).
+template <int RB>
+__device__ __forceinline__ long long row_offset(const Q4Args &g, long long off, const int *row, int kh, int t, bool *ok) {
+    const AttnArgs &a = g.a;
+    if (!a.pages) return off + (long long)t * RB;
+    int pg = __ldg(row + (t >> a.page_shift));
+    if ((unsigned)pg >= (unsigned)a.n_pages) {
         atomicExch(&g_attn_q4_err, 1);
         *ok = false;
         pg = 0;
     }
-    return (((long long)pg * a.Hkv + p.kh) << a.page_shift) * RB + (t & ((1 << a.page_shift) - 1)) * RB;
+    return ((long long)pg * a.Hkv + kh) * g.page_bytes + (t & ((1 << a.page_shift) - 1)) * RB;
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t *src, int n = 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_run(uint32_t dst, const uint8_t *src, int bytes, int lane) {
     // from the 16-byte boundary at or before src; the last copy reads no byte past the run
     const int phase = (int)((uintptr_t)src & 15);
-    for (int i = 16 * lane; i < bytes + phase; i += 512) cp16(dst + i, src - phase + i, min(16, bytes + phase - i));
+    for (int i = 16 * lane; i < bytes + phase; i += 512)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i), "l"(src - phase + i), "r"(min(16, bytes + phase - i))
+                     : "memory");
 }
-// Starts the copies of a tile's rows (all but the new row) and closes their group.
-template <int NB>
-__device__ __forceinline__ void fetch(const Q4Args &g, const Place &p, uint32_t stage, int lane) {
+// Starts the copies of a tile of fewer rows (all but the new row), or of rows off the 16-byte boundaries.
+template <int NB> __device__ __noinline__ void fetch_part(const Q4Args &g, const Item *it, int tile, uint32_t stage) {
     const AttnArgs &a = g.a;
-    constexpr int RB = Q4<NB>::RB, CH = 2 * RB;  // 16-byte pieces of a whole tile
-    const int t0 = p.tile * Q4_TILE, rows = min(Q4_TILE, (a.append ? p.pos : p.pos + 1) - t0);
-    if (rows > 0) {
+    constexpr int RB = Q4<NB>::RB;
+    const int t0 = tile * Q4_TILE, rows = min(Q4_TILE, (a.append ? it->pos : it->pos + 1) - t0), lane = threadIdx.x & 31;
+    const int run = a.pages && a.page_shift == 4 ? 16 : Q4_TILE;  // rows that lie one behind the other
+    for (int r = 0; r < rows; r += run) {
         bool ok;
-        const bool two = a.pages && a.page_shift == 4;  // 16 rows to a page
-        const long long off0 = row_offset<RB>(a, p, t0, &ok);
-        const long long off1 = two && rows > 16 ? row_offset<RB>(a, p, t0 + 16, &ok) - 16 * RB : off0;
-        const uint8_t *kc = (const uint8_t *)a.k_cache, *vc = (const uint8_t *)a.v_cache;
-        if (rows == Q4_TILE && !(off0 & 15)) {
+        const long long off = row_offset<RB>(g, it->off, it->row, it->kh, t0 + r, &ok);
+        const int bytes = min(run, rows - r) * RB;
+        copy_run(stage + r * RB, (const uint8_t *)a.k_cache + off, bytes, lane);
+        copy_run(stage + Q4<NB>::SIDE + r * RB, (const uint8_t *)a.v_cache + off, bytes, lane);
+    }
+}
+// Starts the copies of a whole tile: k, v at this lane's first 16 bytes; the
+// second 16 rows lie at k + two (0 unless pages have 16 rows).
+template <int NB> __device__ __forceinline__ void fetch_tile(const uint8_t *k, long long v, long long two, uint32_t stage, int lane) {
+    constexpr int CH = 2 * Q4<NB>::RB;  // 16-byte pieces
 #pragma unroll
-            for (int i = 0; i < (CH + 31) / 32; i++) {
-                const int c = lane + 32 * i;
-                const long long at = (c < CH / 2 ? off0 : off1) + 16 * c;
-                if (c < CH) {
-                    cp16(stage + 16 * c, kc + at);
-                    cp16(stage + Q4<NB>::SIDE + 16 * c, vc + at);
-                }
-            }
-        } else {
-            for (int r = 0; r < rows; r += two ? 16 : Q4_TILE) {
-                const long long at = r ? off1 + 16 * RB : off0;
-                const int bytes = min(two ? 16 : Q4_TILE, rows - r) * RB;
-                copy_run(stage + r * RB, kc + at, bytes, lane);
-                copy_run(stage + Q4<NB>::SIDE + r * RB, vc + at, bytes, lane);
-            }
+    for (int i = 0; i < (CH + 31) / 32; i++) {
+        const int c = lane + 32 * i;
+        if (c < CH) {
+            const uint8_t *at = k + 512 * i + (32 * i + 31 < CH / 2 ? 0 : 32 * i >= CH / 2 ? two : c < CH / 2 ? 0 : two);
+            cp16(stage + 512 * i, at);
+            cp16(stage + Q4<NB>::SIDE + 512 * i, at + v);
         }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 __device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
@@ -216,14 +243,14 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 // What a warp carries through the tiles of one item.
 template <int NB> struct Q4State {
     uint32_t qa[2 * NB][4];           // q as matrix operands: head g hi, lo, hi, lo
-    float qsum[Q4<NB>::NG], qfac;     // head g: log2 e / sqrt(Dh) times sum(q_j); factor of q . c
+    float qsum[Q4<NB>::NG], qfac;     // head g: sum(q_j) and the factor of its products (q scaled to fp16's range)
     float o[2 * NB][4];               // dims x heads (see the output below)
     float om[Q4<NB>::NG], l, off, mx; // head g, this lane's positions: sum p m, sum p; offset and maximum of s
     int vexp;                         // largest exponent field of the values' d so far
 };
 
 template <int NB>
-__device__ __forceinline__ void load_q(const Q4Args &g, const Place &p, int lane, Q4State<NB> &st) {
+__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, Q4State<NB> &st) {
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH;
     const int G = a.H / a.Hkv, head = (p.j - p.kh * g.HG) * 8 + (lane >> 2), t = lane & 3;
@@ -257,7 +284,7 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Place &p, int lane
         for (int e = 0; e < 8; e++) s += x[i][e];
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        st.qsum[i / 2] += s * scale;
+        st.qsum[i / 2] += s * up;
         // nibbles (0, 4) and (2, 6) of a word meet slice 2 i, (1, 5) and (3, 7), 16 times as large, slice 2 i + 1
         const float dn = up * 0.0625f;
         split2(x[i][0] * up, x[i][4] * up, st.qa[2 * i][0], st.qa[2 * i][1]);
@@ -276,7 +303,7 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Place &p, int lane
 
 // The new K and V rows quantized into `fresh` (two rows) and, by the first
 // head group, into the cache.
-template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const Place &p, uint32_t *fresh, int lane) {
+template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const Item &p, uint32_t *fresh, int lane) {
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH, NW = DH / 8, RB = Q4<NB>::RB;
     float x[2][8];
@@ -288,7 +315,7 @@ template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const 
     }
     if (lane < NW) rope8(a, p.pos, DH, 8 * lane, x[0]);
     bool ok = true;
-    const long long off = row_offset<RB>(a, p, p.pos, &ok);
+    const long long off = row_offset<RB>(g, p.off, p.row, p.kh, p.pos, &ok);
     ok &= p.j == p.kh * g.HG;
 #pragma unroll 1
     for (int side = 0; side < 2; side++) {
@@ -308,35 +335,21 @@ template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const 
     }
 }
 
-// The NG pairs (d, m') of one row.
-template <int NG> __device__ __forceinline__ void load_dm(const float *p, float2 (&f)[NG]) {
-    if constexpr (NG % 2 == 0) {
-#pragma unroll
-        for (int j = 0; j < NG; j += 2) {
-            const float4 v = *reinterpret_cast<const float4 *>(p + 2 * j);
-            f[j] = make_float2(v.x, v.y);
-            f[j + 1] = make_float2(v.z, v.w);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < NG; j++) f[j] = *reinterpret_cast<const float2 *>(p + 2 * j);
-    }
-}
-
 // One tile: n valid rows at kt / vt (row r at r * RB); kdm, vdm: this warp's
 // (d, m) floats.  Of each 16 rows lane (g, t) holds the scores of head g at
 // rows 4 t .. 4 t + 3 (matrix column order 0, 2 | 1, 3: rows that a quarter
 // warp reads then lie in different banks).
 template <int NB>
-__device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const uint8_t *vt, float *kdm, float *vdm, int n, int lane) {
+__device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, const uint8_t *vt, float *kdm, float *vdm, int n, int lane) {
     constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, DH = Q4<NB>::DH;
     const int gq = lane >> 2, t = lane & 3;
     // (d, m') of row `lane` to floats; rows past the end: d = m' = 0
     uint32_t dmax = 0;
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        const uint32_t kw = lane < n ? *reinterpret_cast<const uint32_t *>(kt + lane * RB + DH / 2 + 4 * j) : 0u;
-        const uint32_t vw = lane < n ? *reinterpret_cast<const uint32_t *>(vt + lane * RB + DH / 2 + 4 * j) : 0u;
+        uint32_t kw = *reinterpret_cast<const uint32_t *>(kt + lane * RB + DH / 2 + 4 * j);
+        uint32_t vw = *reinterpret_cast<const uint32_t *>(vt + lane * RB + DH / 2 + 4 * j);
+        if (lane >= n) kw = vw = 0u;
         float2 kf = __half22float2(*reinterpret_cast<const __half2 *>(&kw));
         float2 vf = __half22float2(*reinterpret_cast<const __half2 *>(&vw));
         kf.y = fmaf(8.0f, kf.x, kf.y);
@@ -347,35 +360,34 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
     }
     const int vexp = min((int)(__reduce_max_sync(0xffffffffu, dmax) >> 10), 30);
     __syncwarp();
+    // scores over qfac, group by group: the 32 rows' four column sets (rows
+    // 16 h + 2 g + par) are four independent chains of products
     float s[2][4];  // [16 rows][row 4 t + r]
+    const uint32_t *const kr = reinterpret_cast<const uint32_t *>(kt + 2 * gq * RB) + t;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int j = 0; j < NG; j++) {
+        float c[4][4];
 #pragma unroll
-        for (int par = 0; par < 2; par++) {  // rows 16 h + 2 g + par are the columns
-            float c[NG][4];
+        for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
 #pragma unroll
-            for (int j = 0; j < NG; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
-            const uint32_t *kr = reinterpret_cast<const uint32_t *>(kt + (16 * h + 2 * gq + par) * RB) + t;
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
+            for (int hp = 0; hp < 4; hp++) {
                 uint32_t w[4];
-                codes8(kr[4 * i], w);
-                hmma(c[i / 2], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
-                hmma(c[i / 2], st.qa[2 * i + 1][0], st.qa[2 * i + 1][1], st.qa[2 * i + 1][2], st.qa[2 * i + 1][3], w[1], w[3]);
-            }
-#pragma unroll
-            for (int e = 0; e < 2; e++) {  // columns 2 t, 2 t + 1: rows 4 t + par, 4 t + 2 + par
-                float2 dm[NG];
-                load_dm<NG>(kdm + 2 * NG * (16 * h + 4 * t + 2 * e + par), dm);
-                float x = dm[0].x * (c[0][e] + c[0][2 + e]), y = dm[0].y * st.qsum[0];
-#pragma unroll
-                for (int j = 1; j < NG; j++) {
-                    x = fmaf(dm[j].x, c[j][e] + c[j][2 + e], x);
-                    y = fmaf(dm[j].y, st.qsum[j], y);
-                }
-                s[h][2 * e + par] = fmaf(x, st.qfac, y);
+                codes8(kr[(16 * (hp >> 1) + (hp & 1)) * (RB / 4) + 4 * i], w);
+                if (i % 2) hmma(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
+                else hmma0(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
+                hmma(c[hp], st.qa[2 * i + 1][0], st.qa[2 * i + 1][1], st.qa[2 * i + 1][2], st.qa[2 * i + 1][3], w[1], w[3]);
             }
         }
+#pragma unroll
+        for (int hp = 0; hp < 4; hp++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {  // columns 2 t, 2 t + 1: rows 4 t + par, 4 t + 2 + par
+                const int h = hp >> 1, r = 2 * e + (hp & 1);
+                const float2 dm = *reinterpret_cast<const float2 *>(kdm + 2 * (NG * (16 * h + 4 * t + r) + j));
+                const float x = c[hp][e] + c[hp][2 + e];
+                s[h][r] = j ? fmaf(dm.x, x, s[h][r]) : dm.x * x;
+                s[h][r] = fmaf(dm.y, st.qsum[j], s[h][r]);
+            }
     }
     if (n < Q4_TILE)
 #pragma unroll
@@ -387,7 +399,7 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
     float m = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = fmaxf(m, st.mx);
+    m = fmaxf(m * st.qfac, st.mx);
     const int ve = max(vexp, st.vexp);
     const float off = m - (float)(29 - ve), f = ex2(st.off - off);  // (2^-inf = 0 the first time)
     st.mx = m;
@@ -399,33 +411,25 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
     for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            s[h][r] = ex2(s[h][r] - off);
+            s[h][r] = ex2(fmaf(s[h][r], st.qfac, -off));
             st.l += s[h][r];
         }
-    uint32_t bh[NG][2][2], bl[NG][2][2];  // p d of the 16 rows of each half: hi, lo
-#pragma unroll
-    for (int j = 0; j < NG; j++) st.om[j] *= f;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        float w[NG][4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            float2 dm[NG];
-            load_dm<NG>(vdm + 2 * NG * (16 * h + 4 * t + r), dm);
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                w[j][r] = s[h][r] * dm[j].x;
-                st.om[j] = fmaf(s[h][r], dm[j].y, st.om[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            split2(w[j][0], w[j][2], bh[j][h][0], bl[j][h][0]);
-            split2(w[j][1], w[j][3], bh[j][h][1], bl[j][h][1]);
-        }
-    }
 #pragma unroll
     for (int j = 0; j < NG; j++) {
+        uint32_t bh[2][2], bl[2][2];  // p d of the 16 rows of each half: hi, lo
+        st.om[j] *= f;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float2 dm = *reinterpret_cast<const float2 *>(vdm + 2 * (NG * (16 * h + 4 * t + r) + j));
+                w[r] = s[h][r] * dm.x;
+                st.om[j] = fmaf(s[h][r], dm.y, st.om[j]);
+            }
+            split2(w[0], w[2], bh[h][0], bl[h][0]);
+            split2(w[1], w[3], bh[h][1], bl[h][1]);
+        }
         // this lane's dims: word g of the group, or half a word of a group of 32
         const bool half = NB % 2 && j == NG - 1;
         const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
@@ -440,16 +444,19 @@ __device__ __forceinline__ void tile(Q4State<NB> &st, const uint8_t *kt, const u
             const int i = 4 * j + 2 * k;
             float c[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) c[0][e] = c[1][e] = 0.0f;
-#pragma unroll
             for (int h = 0; h < 2; h++) {
                 uint32_t x[4], y[4];  // rows 4 t + (0, 2) and (1, 3)
                 codes8(__byte_perm(cw[h][0], cw[h][2], sel), x);
                 codes8(__byte_perm(cw[h][1], cw[h][3], sel), y);
-                hmma(c[0], x[0], x[1], y[0], y[1], bh[j][h][0], bh[j][h][1]);
-                hmma(c[1], x[2], x[3], y[2], y[3], bh[j][h][0], bh[j][h][1]);
-                hmma(c[0], x[0], x[1], y[0], y[1], bl[j][h][0], bl[j][h][1]);
-                hmma(c[1], x[2], x[3], y[2], y[3], bl[j][h][0], bl[j][h][1]);
+                if (h) {
+                    hmma(c[0], x[0], x[1], y[0], y[1], bh[h][0], bh[h][1]);
+                    hmma(c[1], x[2], x[3], y[2], y[3], bh[h][0], bh[h][1]);
+                } else {
+                    hmma0(c[0], x[0], x[1], y[0], y[1], bh[h][0], bh[h][1]);
+                    hmma0(c[1], x[2], x[3], y[2], y[3], bh[h][0], bh[h][1]);
+                }
+                hmma(c[0], x[0], x[1], y[0], y[1], bl[h][0], bl[h][1]);
+                hmma(c[1], x[2], x[3], y[2], y[3], bl[h][0], bl[h][1]);
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -502,8 +509,9 @@ __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *d
 }
 
 template <int NB>
-__global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Args g) {
+__global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? Q4_MB : 2) k_attn_q4(const __grid_constant__ Q4Args g) {
     extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ Item sh_item[Q4_WARPS][2];  // of the copies, of the computation
     __shared__ int sh_total[Q4_WARPS], desc[Q4_WARPS][2][5];  // a warp's parts: first unit of the item, b, j, first tile, end
     constexpr int DH = Q4<NB>::DH, SLOT = Q4<NB>::SLOT, RB = Q4<NB>::RB;
     const AttnArgs &a = g.a;
@@ -514,7 +522,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Ar
     // units (tiles) of the whole batch, and this CTA's and this warp's share
     auto units_of = [&](int b) -> int {
         const int p = seq_pos(g, b);
-        return p < 0 ? 0 : g.items_only ? items : (p / Q4_TILE + 1) * items;
+        return p < 0 ? 0 : item_units(g, p / Q4_TILE + 1) * items;
     };
     int sum = 0;
     for (int b = threadIdx.x; b < g.batch; b += 32 * Q4_WARPS) sum += units_of(b);
@@ -537,8 +545,8 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Ar
 
     if (u0 < u1) {
         // where unit u0 lies
-        Place in;
-        in.b = 0;
+        Item p;
+        p.b = 0;
         int before = 0;
         for (int b0 = 0; b0 < g.batch; b0 += 32) {
             const int mine = b0 + lane < g.batch ? units_of(b0 + lane) : 0;
@@ -551,75 +559,135 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Ar
             const unsigned hit = __ballot_sync(0xffffffffu, before + inc > u0);
             if (hit) {
                 const int w = __ffs(hit) - 1;
-                in.b = b0 + w;
+                p.b = b0 + w;
                 before += __shfl_sync(0xffffffffu, inc - mine, w);
                 break;
             }
             before += __shfl_sync(0xffffffffu, inc, 31);
         }
-        set_seq(g, in);
-        const int at = u0 - before, per = g.items_only ? 1 : in.nt;
-        in.j = at / per;
-        in.tile = at % per;
-        in.left = u1 - u0;
-        set_item<RB>(g, in);
-        Place ahead = in;
-        const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-        int fill = 0, stage = 0, first_tile = -1, unit = u0, part = 0, phase = 0;
+        set_seq(g, p);
+        const int at = u0 - before, per = item_units(g, p.nt);
+        p.j = at / per;
+        p.unit = u0 - at % per;
+        p.left = u1 - p.unit;
+        p.tile = g.items_only ? 0 : max(0, at % per - Q4_ITEM);
+        set_item<RB>(g, p);
+        Item *const ia = &sh_item[warp][0], *const ii = &sh_item[warp][1];
+        *ia = p;
+        *ii = p;
+        __syncwarp();
+        // the copies' place: tiles [tile, end) of an item, the first `whole` of it without special cases
+        const uint8_t *const kc = (const uint8_t *)a.k_cache + 16 * lane;
+        const long long kv = (const uint8_t *)a.v_cache - (const uint8_t *)a.k_cache;
+        const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
+        const bool two = a.pages && a.page_shift == 4;
+        int a_tile, a_end, a_whole, a_kh, a_pg = 0, a_pg2 = 0, fill = 0;  // (pages looked up one tile ahead)
+        const uint8_t *a_src = nullptr;  // contiguous: this lane's first piece of tile a_tile
+        const int *a_row;
+        auto look_up = [&]() {
+            if (a_tile < a_whole) {
+                a_pg = __ldg(a_row + (a_tile * Q4_TILE >> a.page_shift));
+                if (two) a_pg2 = __ldg(a_row + 2 * a_tile + 1);
+            }
+        };
+        auto item_ahead = [&]() {
+            a_tile = ia->tile;
+            a_end = ia->end;
+            a_kh = ia->kh;
+            a_row = ia->row;
+            const int rows = a.append ? ia->pos : ia->pos + 1;
+            if (a.pages) {
+                a_whole = min(rows / Q4_TILE, a_end);
+                look_up();
+            } else {
+                a_whole = ia->off & 15 ? 0 : min(rows / Q4_TILE, a_end);
+                a_src = kc + ia->off + (long long)a_tile * (Q4_TILE * RB);
+            }
+        };
+        auto page_at = [&](int pg) -> const uint8_t * {  // this lane's first piece of a page's rows
+            if ((unsigned)pg >= (unsigned)a.n_pages) {
+                atomicExch(&g_attn_q4_err, 1);
+                pg = 0;
+            }
+            return kc + ((long long)pg * a.Hkv + a_kh) * g.page_bytes;
+        };
+        item_ahead();
+        int tile = p.tile, end = p.end, nt = p.nt, phase = 0, stage = 0, part = 0;
+        bool begin = true;
         Q4State<NB> st;
 #pragma unroll 1
-        for (int skip = Q4_STAGES - 1; in.left > 0; skip--) {  // the first turns only start copies
-            if (ahead.left > 0) {
-                fetch<NB>(g, ahead, ring_s + fill * Q4<NB>::STAGE, lane);
-                next_tile<RB>(g, ahead);
-            } else {
-                asm volatile("cp.async.commit_group;" ::: "memory");
+        for (int skip = Q4_STAGES - 1; tile < end; skip--) {  // the first turns only start copies
+            if (a_tile < a_end) {
+                if (a_tile < a_whole) {
+                    long long o2 = 0;
+                    if (a.pages) {
+                        a_src = page_at(a_pg) + ((a_tile * Q4_TILE) & ((1 << a.page_shift) - 1)) * RB;
+                        if (two) o2 = page_at(a_pg2) - 16 * RB - a_src;
+                    }
+                    fetch_tile<NB>(a_src, kv, o2, ring_s + fill, lane);
+                } else {
+                    fetch_part<NB>(g, ia, a_tile, ring_s - 16 * lane + fill);
+                }
+                a_tile++;
+                a_src += Q4_TILE * RB;
+                if (a_tile == a_end) {
+                    next_item<RB>(g, ia);
+                    item_ahead();
+                } else if (a.pages) {
+                    look_up();
+                }
             }
-            fill = fill + 1 == Q4_STAGES ? 0 : fill + 1;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            fill = fill == (Q4_STAGES - 1) * Q4<NB>::STAGE ? 0 : fill + Q4<NB>::STAGE;
             if (skip > 0) continue;
-            if (first_tile < 0) {  // an item begins
-                first_tile = in.tile;
-                phase = a.pages ? 0 : (int)(in.off & 15);  // rows lie in the ring at the phase that they have in the cache
-                if (a.append && (g.items_only || in.left >= in.nt - in.tile)) append<NB>(g, in, fresh, lane);
-                load_q<NB>(g, in, lane, st);
+            if (begin) {
+                phase = a.pages ? 0 : (int)(ii->off & 15);  // rows lie in the ring at the phase that they have in the cache
+                if (a.append && end == nt) append<NB>(g, *ii, fresh, lane);
+                load_q<NB>(g, *ii, lane, st);
+                begin = false;
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 1) : "memory");
             __syncwarp();
-            uint8_t *kt = ring + stage * Q4<NB>::STAGE + phase, *vt = kt + Q4<NB>::SIDE;
-            stage = stage + 1 == Q4_STAGES ? 0 : stage + 1;
-            const int n = min(Q4_TILE, in.pos + 1 - in.tile * Q4_TILE);
-            const bool last = in.tile == in.nt - 1;
-            if (last && a.append) {
-                for (int i = lane; i < RB / 4; i += 32) {
-                    reinterpret_cast<uint32_t *>(kt + (n - 1) * RB)[i] = fresh[i];
-                    reinterpret_cast<uint32_t *>(vt + (n - 1) * RB)[i] = fresh[RB / 4 + i];
+            uint8_t *kt = ring + stage + phase;
+            stage = stage == (Q4_STAGES - 1) * Q4<NB>::STAGE ? 0 : stage + Q4<NB>::STAGE;
+            int n = Q4_TILE;
+            if (tile == nt - 1) {  // the item's last tile: fewer rows, the new row among them
+                n = ii->pos + 1 - tile * Q4_TILE;
+                if (a.append) {
+                    for (int i = lane; i < RB / 4; i += 32) {
+                        reinterpret_cast<uint32_t *>(kt + (n - 1) * RB)[i] = fresh[i];
+                        reinterpret_cast<uint32_t *>(kt + Q4<NB>::SIDE + (n - 1) * RB)[i] = fresh[RB / 4 + i];
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-            tile<NB>(st, kt, vt, kdm, vdm, n, lane);
+            attend_tile<NB>(st, kt, kt + Q4<NB>::SIDE, kdm, vdm, n, lane);
             __syncwarp();  // the stage and (d, m') are read; they may be written again
-            if (last || (!g.items_only && in.left == 1)) {  // the item, or this warp's part of it, ends
-                const int h0 = (in.j - in.kh * g.HG) * 8, heads = min(8, G - h0);
-                const size_t head = (size_t)in.kh * G + h0;
-                const bool whole = first_tile == 0 && last;
+            if (++tile == end) {  // the item, or this warp's part of it, ends
+                const int b = ii->b, j = ii->j, kh = ii->kh, first = ii->tile;
+                const int h0 = (j - kh * g.HG) * 8, heads = min(8, G - h0);
+                const size_t head = (size_t)kh * G + h0;
+                const bool whole = first == 0 && end == nt;
                 float *slot = part ? reinterpret_cast<float *>(ring) : slots + warp * GH * SLOT;
-                result<NB>(st, lane, whole ? a.out + (size_t)in.b * a.ldo + head * DH : slot, whole ? DH : SLOT, heads, whole, !whole || g.vec);
+                result<NB>(st, lane, whole ? a.out + (size_t)b * a.ldo + head * DH : slot, whole ? DH : SLOT, heads, whole, !whole || g.vec);
                 if (whole) {
                     if (lane < heads && a.nsplit > 1)  // nothing for the combine kernel to do
-                        a.ws[((size_t)in.b * a.H + head + lane) * hstride + DH + 1] = 0.0f;
+                        a.ws[((size_t)b * a.H + head + lane) * hstride + DH + 1] = 0.0f;
                 } else if (lane == 0) {
                     int *d = desc[warp][part];
-                    d[0] = unit - in.tile;  // the item's first unit
-                    d[1] = in.b;
-                    d[2] = in.j;
-                    d[3] = first_tile;
-                    d[4] = in.tile + 1;
+                    d[0] = ii->unit;
+                    d[1] = b;
+                    d[2] = j;
+                    d[3] = first;
+                    d[4] = end;
                 }
                 part = 1;
-                first_tile = -1;
+                next_item<RB>(g, ii);
+                tile = ii->tile;
+                end = ii->end;
+                nt = ii->nt;
+                begin = true;
             }
-            unit++;
-            next_tile<RB>(g, in);
         }
     }
     __syncthreads();
@@ -639,7 +707,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? 3 : 2) k_attn_q4(Q4Ar
         const int pos = seq_pos(g, b), nt = pos / Q4_TILE + 1;
         const bool whole = d[3] == 0 && desc[e / 2][e % 2][4] == nt;
         // the CTAs that hold the item's first and last tile
-        const int ca = (int)(((long long)(d[0] + 1) * nC - 1) / total), cb = (int)(((long long)(d[0] + nt) * nC - 1) / total);
+        const int ca = (int)(((long long)(d[0] + Q4_ITEM + 1) * nC - 1) / total), cb = (int)(((long long)(d[0] + Q4_ITEM + nt) * nC - 1) / total);
         for (int i = threadIdx.x; i < heads * DH; i += 32 * Q4_WARPS) {
             const int h = i / DH, x = i % DH;
             float M = -INFINITY, L = 0.0f, acc = 0.0f;
@@ -746,7 +814,7 @@ template <int NB> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
     const int GH = g.a.H / g.a.Hkv < 8 ? g.a.H / g.a.Hkv : 8;
     const size_t smem = (size_t)Q4_WARPS * Q4<NB>::WARP_BYTES + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
     LMC_CUDA_TRY(cudaFuncSetAttribute(k_attn_q4<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int fit = (int)(227 * 1024 / (smem + 1536)), per_sm = fit < (NB <= 4 ? 3 : 2) ? fit : (NB <= 4 ? 3 : 2);
+    const int fit = (int)(227 * 1024 / (smem + 1536)), per_sm = fit < (NB <= 4 ? Q4_MB : 2) ? fit : (NB <= 4 ? Q4_MB : 2);
     const int most = lmc_sm_count() * (per_sm > 0 ? per_sm : 1), want = max_units / g.rmin;
     LMC_LAUNCH("attention (4-bit rows)", k_attn_q4<NB>, want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);
     return LMC_OK;
@@ -772,7 +840,8 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     g.rmin = g.items_only || NT < 2 ? 1 : (NT - 2) / (a.nsplit - 1) + 1;
     g.vec = (((uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.out) & 15) == 0 && a.ldq % 4 == 0 &&
             a.ldkv % 4 == 0 && a.ldo % 4 == 0;
-    const long long units = (long long)batch * a.Hkv * g.HG * (g.items_only ? 1 : NT);
+    g.page_bytes = kv_q4_row_bytes(a.Dh) << a.page_shift;
+    const long long units = (long long)batch * a.Hkv * g.HG * (g.items_only ? 1 : NT + Q4_ITEM);
     if (units > 0x7fffffffLL) return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: batch %d x context %d is too large", batch, a.S);
     int (*const fn[8])(const Q4Args &, int, cudaStream_t) = {launch<1>, launch<2>, launch<3>, launch<4>, launch<5>, launch<6>, launch<7>, launch<8>};
     const int rc = fn[a.Dh / 32 - 1](g, (int)units, s);
