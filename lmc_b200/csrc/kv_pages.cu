@@ -14,6 +14,7 @@ namespace {
 __device__ int g_kv_pages_err;  // an index outside its range was met (lmc_device_status)
 
 constexpr int PLAN_THREADS = 1024;
+constexpr int COPY_VECS = 1024;  // 16-byte words that a CTA copies at a time, four loads a thread in flight
 constexpr int MAX_POOLS = 256;  // pool addresses passed in one launch (2 KiB of parameters)
 
 // Workspace: [0] pages to copy, then from WS_LIST on pairs (source, destination),
@@ -52,32 +53,44 @@ __device__ __forceinline__ int block_scan(int v, int *part, int *total) {
     return part[warp] + x - v;
 }
 
-// Column stripe of the table: every row's entries of C columns are read
-// before any is written, so parents may be any mapping.
+// Column stripe of the table: every row's entries of 2^cs columns are read
+// before any is written, so parents may be any mapping.  What a call changes
+// in the counts of row r's old entries is the same in every column: one more
+// for each other row that copies r, one less when r itself is replaced; so one
+// atomic addition per entry of a row where that is not 0 (and none per copy).
 __global__ void __launch_bounds__(256) k_pages_fork(int *pages, int n_seqs, int max_pages, int *refs, int n_pages,
-                                                    const int *parent, int C) {
-    extern __shared__ int tile[];  // [n_seqs][C]
+                                                    const int *parent, int cs) {
+    extern __shared__ int tile[];  // [n_seqs][2^cs], then parent[n_seqs], change[n_seqs]
+    int *const par = tile + ((size_t)n_seqs << cs), *const change = par + n_seqs;
     pdl_wait();
     pdl_launch_dependents();
-    const int c0 = blockIdx.x * C, nc = min(C, max_pages - c0);
-    for (int i = threadIdx.x; i < n_seqs * C; i += 256) {
-        const int b = i / C, j = i % C;
-        if (j < nc) tile[i] = pages[(size_t)b * max_pages + c0 + j];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_seqs * C; i += 256) {
-        const int b = i / C, j = i % C, p = parent[b];
-        if (j >= nc || p == b) continue;
+    const int c0 = blockIdx.x << cs, nc = min(1 << cs, max_pages - c0), mask = (1 << cs) - 1;
+    for (int b = threadIdx.x; b < n_seqs; b += 256) {
+        int p = parent[b];
         if (p >= n_seqs) {
             atomicExch(&g_kv_pages_err, 1);
-            continue;
+            p = b;
         }
-        const int was = tile[i], now = p < 0 ? -1 : tile[p * C + j];
-        if (was >= n_pages || now >= n_pages) atomicExch(&g_kv_pages_err, 1);
-        if (was == now) continue;
-        if (was >= 0 && was < n_pages) atomicSub(refs + was, 1);
-        if (now >= 0 && now < n_pages) atomicAdd(refs + now, 1);
-        pages[(size_t)b * max_pages + c0 + j] = now;
+        par[b] = p;
+        change[b] = p == b ? 0 : -1;
+    }
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n_seqs << cs; i += 256)
+        if ((i & mask) < nc) tile[i] = pages[(size_t)(i >> cs) * max_pages + c0 + (i & mask)];
+    __syncthreads();
+    for (int b = threadIdx.x; b < n_seqs; b += 256)
+        if (par[b] >= 0 && par[b] != b) atomicAdd(change + par[b], 1);
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n_seqs << cs; i += 256) {
+        const int b = i >> cs, j = i & mask, p = par[b], was = tile[i], d = change[b];
+        if (j >= nc) continue;
+        if (was >= n_pages) atomicExch(&g_kv_pages_err, 1);
+        if (d != 0 && was >= 0 && was < n_pages) atomicAdd(refs + was, d);
+        if (p != b) {
+            const int now = p < 0 ? -1 : tile[(p << cs) + j];
+            if (now != was) pages[(size_t)b * max_pages + c0 + j] = now;
+        }
     }
 }
 
@@ -226,11 +239,22 @@ __global__ void __launch_bounds__(256) k_pages_copy(Pools pools, int n_pools, in
         const int n_live = *d_n_live;
         for (long long i = tid; i < entries; i += nthr) rename_entry(pages + i, n_live, n_pages, ws + WS_LIST + n_pages + 2);
     }
-    for (long long item = blockIdx.x; item < (long long)n * n_pools; item += gridDim.x) {
-        const int k = (int)(item / n_pools), pool = (int)(item % n_pools);
-        const uint4 *src = pools.p[pool] + (size_t)ws[WS_LIST + 2 * k] * vecs;
-        uint4 *dst = pools.p[pool] + (size_t)ws[WS_LIST + 2 * k + 1] * vecs;
-        for (int i = threadIdx.x; i < vecs; i += 256) dst[i] = src[i];
+    // piece = COPY_VECS neighbouring 16-byte words of one page in one pool; pools innermost, so that the
+    // CTAs at work spread over the memory
+    const int pieces = (vecs + COPY_VECS - 1) / COPY_VECS;
+    const long long items = (long long)n * pieces * n_pools;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const int pool = (int)(item % n_pools), at = (int)(item / n_pools % pieces) * COPY_VECS, k = (int)(item / n_pools / pieces);
+        const uint4 *src = pools.p[pool] + (size_t)ws[WS_LIST + 2 * k] * vecs + at;
+        uint4 *dst = pools.p[pool] + (size_t)ws[WS_LIST + 2 * k + 1] * vecs + at;
+        const int m = min(COPY_VECS, vecs - at);
+        uint4 v[COPY_VECS / 256];
+#pragma unroll
+        for (int u = 0; u < COPY_VECS / 256; u++)
+            if (threadIdx.x + 256 * u < m) v[u] = __ldg(src + threadIdx.x + 256 * u);
+#pragma unroll
+        for (int u = 0; u < COPY_VECS / 256; u++)
+            if (threadIdx.x + 256 * u < m) dst[threadIdx.x + 256 * u] = v[u];
     }
 }
 
@@ -267,16 +291,19 @@ extern "C" size_t lmc_kv_pages_workspace_bytes(int n_seqs, int n_pages) {
 extern "C" int lmc_kv_pages_fork(int *d_pages, int n_seqs, int max_pages, int *d_refs, int n_pages, const int *d_parent,
                                  void *stream) {
     if (!d_pages || !d_refs || !d_parent) return lmc_set_error(LMC_ERR_INVALID, "kv_pages_fork: null pointer");
-    if (n_seqs <= 0 || max_pages <= 0 || n_pages <= 0 || n_seqs > 32768)
-        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_fork: %d sequences x %d entries, %d pages (at most 32768 "
+    if (n_seqs <= 0 || max_pages <= 0 || n_pages <= 0 || n_seqs > 16384)
+        return lmc_set_error(LMC_ERR_INVALID, "kv_pages_fork: %d sequences x %d entries, %d pages (at most 16384 "
                              "sequences)", n_seqs, max_pages, n_pages);
-    int C = 32;
-    while (C > 1 && (size_t)n_seqs * C * sizeof(int) > 128 * 1024) C /= 2;
-    const size_t smem = (size_t)n_seqs * C * sizeof(int);
+    // 32 columns (128 bytes of a row) to a CTA; down to 8 (a 32-byte sector)
+    // while that gives fewer than two CTAs an SM, and as few as fit in shared memory
+    int cs = 5;
+    while (cs > 3 && (max_pages >> cs) < 2 * lmc_sm_count()) cs--;
+    while (cs > 0 && ((size_t)n_seqs << cs) * sizeof(int) > 128 * 1024) cs--;
+    const size_t smem = (((size_t)n_seqs << cs) + 2 * (size_t)n_seqs) * sizeof(int);
     if (smem > 48 * 1024)
-        LMC_CUDA_TRY(cudaFuncSetAttribute(k_pages_fork, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
-    LMC_LAUNCH("kv pages fork", k_pages_fork, lmc_cdiv(max_pages, C), 256, smem, lmc_stream(stream), d_pages, n_seqs,
-               max_pages, d_refs, n_pages, d_parent, C);
+        LMC_CUDA_TRY(cudaFuncSetAttribute(k_pages_fork, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    LMC_LAUNCH("kv pages fork", k_pages_fork, lmc_cdiv(max_pages, (size_t)1 << cs), 256, smem, lmc_stream(stream), d_pages,
+               n_seqs, max_pages, d_refs, n_pages, d_parent, cs);
     return LMC_OK;
 }
 

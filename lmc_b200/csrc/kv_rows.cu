@@ -2,11 +2,13 @@
 // any row form, contiguous or paged.
 //
 // Both stream: append reads 4 Dh bytes per row and side and writes the row's
-// form, read the reverse, so HBM bounds them.  4-bit rows: LPR = 4 .. 32
-// lanes per row, one lane per word of eight codes (two 16-byte loads of
-// fp32), so every lane of a warp has work at each head size that is a power
-// of two and a group's minimum and maximum take three shuffles; the other
-// forms take a warp per row.
+// form, read the reverse, so HBM bounds them, and close behind it the
+// instructions per value; a thread therefore has the K and the V side of its
+// rows, whose place in the cache it works out once, and starts all loads
+// before it uses the first.  4-bit rows: LPR = 4 .. 32 lanes per row, eight
+// dims a lane; append takes neighbouring dims (a word of codes, three shuffles
+// for a group's minimum and maximum), read two runs of four (stores without
+// gaps).  The other forms take a warp per row and side.
 #include "attention.cuh"
 #include "kv_q4.cuh"
 #include "lmc_common.cuh"
@@ -58,69 +60,106 @@ __device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
     }
 }
 
-__device__ __forceinline__ void store8(float *p, bool vec, const float (&x)[8]) {
-    if (vec) {
-        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = x[i];
-    }
-}
-
-// blockIdx.y: 0 = K, 1 = V.  Item = (row, kv head), heads innermost.
-template <int LPR>
-__global__ void __launch_bounds__(128) k_append_q4(RowArgs a) {
+// Item = (row, kv head), heads innermost; a CTA has U x 128 / LPR neighbouring
+// items, a thread items 128 / LPR apart.
+template <int LPR, int U> __global__ void __launch_bounds__(128) k_append_q4(RowArgs a) {
     pdl_wait();
     pdl_launch_dependents();
-    const bool is_v = blockIdx.y;
-    const float *src = is_v ? a.v : a.k;
-    if (!src) return;
-    const long long item = ((long long)blockIdx.x * 128 + threadIdx.x) / LPR;
-    const int w = threadIdx.x % LPR, r = (int)(item / a.Hkv), kh = (int)(item % a.Hkv);
-    const long long off = r < a.rows ? row_offset(a, r, kh) : -1;
-    const bool active = off >= 0 && w < a.Dh / 8;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (active) {
-        load8(src + (size_t)r * (is_v ? a.ldv : a.ldk) + (size_t)kh * a.Dh + 8 * w, a.vec, x);
-        if (!is_v && a.rope_cos) {  // pairs (2 d, 2 d + 1) (src/ops_llama.c:39-48)
+    const int w = threadIdx.x % LPR;
+    const unsigned first = blockIdx.x * (U * 128u / LPR) + threadIdx.x / LPR;
+    float x[U][2][8];
+    long long off[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const unsigned item = first + u * (128 / LPR), r = item / a.Hkv, kh = item - r * a.Hkv;
+        off[u] = r < (unsigned)a.rows && w < a.Dh / 8 ? row_offset(a, r, kh) : -1;
+        const size_t at = (size_t)kh * a.Dh + 8 * w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[u][0][i] = x[u][1][i] = 0.0f;
+        if (off[u] < 0) continue;
+        if (a.k) load8(a.k + (size_t)r * a.ldk + at, a.vec, x[u][0]);
+        if (a.v) load8(a.v + (size_t)r * a.ldv + at, a.vec, x[u][1]);
+        if (a.k && a.rope_cos) {  // pairs (2 d, 2 d + 1) (src/ops_llama.c:39-48)
             const size_t t = (size_t)a.pos[r] * (a.Dh / 2) + 4 * w;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float c = a.rope_cos[t + i], s = a.rope_sin[t + i], x0 = x[2 * i], x1 = x[2 * i + 1];
-                x[2 * i] = x0 * c - x1 * s;
-                x[2 * i + 1] = x0 * s + x1 * c;
+                const float c = a.rope_cos[t + i], s = a.rope_sin[t + i], x0 = x[u][0][2 * i], x1 = x[u][0][2 * i + 1];
+                x[u][0][2 * i] = x0 * c - x1 * s;
+                x[u][0][2 * i + 1] = x0 * s + x1 * c;
             }
         }
     }
-    uint32_t codes, dm;
-    kv_q4_quantize<LPR>(x, active, codes, dm);
-    if (!active) return;
-    uint32_t *row = reinterpret_cast<uint32_t *>((is_v ? a.vc : a.kc) + off);
-    row[w] = codes;
-    if (w % 8 == 0) row[a.Dh / 8 + w / 8] = dm;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+            if (!(side ? a.v : a.k)) continue;
+            uint32_t codes, dm;
+            kv_q4_quantize<LPR>(x[u][side], off[u] >= 0, codes, dm);
+            if (off[u] < 0) continue;
+            uint32_t *to = reinterpret_cast<uint32_t *>((side ? a.vc : a.kc) + off[u]);
+            to[w] = codes;
+            if (w % 8 == 0) to[a.Dh / 8 + w / 8] = dm;
+        }
 }
 
-template <int LPR>
-__global__ void __launch_bounds__(128) k_read_q4(RowArgs a) {
+template <int LPR, int U> __global__ void __launch_bounds__(128) k_read_q4(RowArgs a) {
     pdl_wait();
     pdl_launch_dependents();
-    const bool is_v = blockIdx.y;
-    float *dst = is_v ? a.v : a.k;
-    if (!dst) return;
-    const long long item = ((long long)blockIdx.x * 128 + threadIdx.x) / LPR;
-    const int w = threadIdx.x % LPR, r = (int)(item / a.Hkv), kh = (int)(item % a.Hkv);
-    if (r >= a.rows || w >= a.Dh / 8) return;
-    const long long off = row_offset(a, r, kh);
-    if (off < 0) return;
-    const uint32_t *row = reinterpret_cast<const uint32_t *>((is_v ? a.vc : a.kc) + off);
-    const uint32_t codes = row[w], dm = row[a.Dh / 8 + w / 8];
-    const float d = __half2float(__ushort_as_half((unsigned short)(dm & 0xffff)));
-    const float m = __half2float(__ushort_as_half((unsigned short)(dm >> 16)));
-    float x[8];
+    const int w = threadIdx.x % LPR, half = a.Dh / 8;  // quads w and w + half
+    if (w >= half) return;
+    const unsigned first = blockIdx.x * (U * 128u / LPR) + threadIdx.x / LPR;
+    uint32_t codes[U][2][2], dm[U][2][2];
+    long long off[U];
+    unsigned row[U], head[U];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = fmaf(d, (float)((codes >> (4 * i)) & 15u), m);
-    store8(dst + (size_t)r * (is_v ? a.ldv : a.ldk) + (size_t)kh * a.Dh + 8 * w, a.vec, x);
+    for (int u = 0; u < U; u++) {
+        const unsigned item = first + u * (128 / LPR), r = item / a.Hkv, kh = item - r * a.Hkv;
+        off[u] = r < (unsigned)a.rows ? row_offset(a, r, kh) : -1;
+        row[u] = r;
+        head[u] = kh;
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+            if (off[u] < 0 || !(side ? a.v : a.k)) continue;
+            const uint8_t *p = (side ? a.vc : a.kc) + off[u];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                codes[u][side][i] = reinterpret_cast<const uint16_t *>(p)[w + i * half];
+                dm[u][side][i] = reinterpret_cast<const uint32_t *>(p)[half + (w + i * half) / 16];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+            if (off[u] < 0 || !(side ? a.v : a.k)) continue;
+            float *to = (side ? a.v + (size_t)row[u] * a.ldv : a.k + (size_t)row[u] * a.ldk) + (size_t)head[u] * a.Dh + 4 * w;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float d = __half2float(__ushort_as_half((unsigned short)(dm[u][side][i] & 0xffff)));
+                const float m = __half2float(__ushort_as_half((unsigned short)(dm[u][side][i] >> 16)));
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)  // 2^23 | code is the number 2^23 + code
+                    x[e] = fmaf(d, __uint_as_float(0x4b000000u | ((codes[u][side][i] >> (4 * e)) & 15u)) - 8388608.0f, m);
+                float *p = to + 4 * half * i;
+                if (a.vec) *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; e++) p[e] = x[e];
+            }
+        }
+}
+
+template <int LPR, int U> int launch_q4(const char *name, const RowArgs &a, bool read, cudaStream_t s) {
+    LMC_LAUNCH(name, (read ? k_read_q4<LPR, U> : k_append_q4<LPR, U>), lmc_cdiv((size_t)a.rows * a.Hkv, U * 128 / LPR), 128, 0, s, a);
+    return LMC_OK;
+}
+// Two items a thread when that still gives every SM eight CTAs, else one.
+template <int LPR> int launch_q4(const char *name, const RowArgs &a, bool read, cudaStream_t s) {
+    const bool many = (long long)a.rows * a.Hkv * LPR >= 2ll * 128 * 8 * lmc_sm_count();
+    return many ? launch_q4<LPR, 2>(name, a, read, s) : launch_q4<LPR, 1>(name, a, read, s);
 }
 
 // One warp per (row, kv head, side) for the other row forms.
@@ -131,8 +170,8 @@ __global__ void __launch_bounds__(128) k_rows(RowArgs a) {
     const bool is_v = blockIdx.y;
     float *f = is_v ? a.v : a.k;
     if (!f) return;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, r = (int)(item / a.Hkv), kh = (int)(item % a.Hkv);
+    const unsigned item = blockIdx.x * 4u + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, r = (int)((unsigned)item / a.Hkv), kh = (int)((unsigned)item % a.Hkv);
     if (r >= a.rows) return;
     const long long off = row_offset(a, r, kh);
     if (off < 0) return;
@@ -156,12 +195,11 @@ __global__ void __launch_bounds__(128) k_rows(RowArgs a) {
 int rows_launch(const char *name, const RowArgs &a, int kv_dtype, bool read, cudaStream_t s) {
     const long long items = (long long)a.rows * a.Hkv;
     if (kv_dtype == LMC_KV_Q4) {
-        const int words = a.Dh / 8, lpr = words <= 4 ? 4 : words <= 8 ? 8 : words <= 16 ? 16 : 32;
-        const dim3 grid(lmc_cdiv(items, 128 / lpr), 2);
-        void (*fn)(RowArgs) = read ? (lpr == 4 ? k_read_q4<4> : lpr == 8 ? k_read_q4<8> : lpr == 16 ? k_read_q4<16> : k_read_q4<32>)
-                                   : (lpr == 4 ? k_append_q4<4> : lpr == 8 ? k_append_q4<8> : lpr == 16 ? k_append_q4<16> : k_append_q4<32>);
-        LMC_LAUNCH(name, fn, grid, 128, 0, s, a);
-        return LMC_OK;
+        const int words = a.Dh / 8;
+        return words <= 4    ? launch_q4<4>(name, a, read, s)
+               : words <= 8  ? launch_q4<8>(name, a, read, s)
+               : words <= 16 ? launch_q4<16>(name, a, read, s)
+                             : launch_q4<32>(name, a, read, s);
     }
     const dim3 grid(lmc_cdiv(items, 4), 2);
     void (*fn)(RowArgs) = kv_dtype == LMC_KV_F32   ? (read ? k_rows<float, true> : k_rows<float, false>)
@@ -182,7 +220,7 @@ int rows_args(const char *name, RowArgs *a, const float *k, const float *v, int 
     if (rows < 0 || n_seqs <= 0 || Hkv <= 0 || Dh <= 0 || Dh % 32 || Dh > 256 || S <= 0 || (long long)Hkv * Dh > ld)
         return lmc_set_error(LMC_ERR_INVALID, "%s: rows=%d n_seqs=%d Hkv=%d Dh=%d S=%d ld=%d (need Dh%%32==0, "
                              "Dh<=256, ld>=Hkv*Dh)", name, rows, n_seqs, Hkv, Dh, S, ld);
-    if ((long long)rows * Hkv > (1ll << 31))
+    if ((long long)rows * Hkv > (1ll << 30))
         return lmc_set_error(LMC_ERR_INVALID, "%s: %d rows of %d heads in one call", name, rows, Hkv);
     if (((uintptr_t)(k ? kc : nullptr) | (uintptr_t)(v ? vc : nullptr)) & 15)
         return lmc_set_error(LMC_ERR_INVALID, "%s: the cache must start on a 16-byte boundary", name);

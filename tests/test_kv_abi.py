@@ -94,7 +94,7 @@ def test_page_operator_refusals():
     com = lambda **k: ("lmc_kv_pages_compact", *{**dict(h=one, k=1, by=4096, t=P, n=4, w=8, r=P, np=100, nl=P, ws=P,
                                                         wb=ws), **k}.values(), None)
     cases = [(fork(t=None), b"null"), (fork(r=None), b"null"), (fork(p=None), b"null"), (fork(n=0), b"0 sequences"),
-             (fork(n=32769), b"32768"), (fork(w=0), b"x 0 entries"), (fork(np=0), b"0 pages"),
+             (fork(n=16385), b"16384"), (fork(w=0), b"x 0 entries"), (fork(np=0), b"0 pages"),
              (res(pos=None), b"null"), (res(sh=None), b"null"), (res(ws=None), b"null"), (res(ps=24), b"24 positions"),
              (res(ps=8), b"8 positions"), (res(n=-1), b"-1 sequences"), (com(nl=None), b"null"), (com(np=-5), b"-5 pages")]
     for f in (res, com):
