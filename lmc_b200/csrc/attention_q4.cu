@@ -22,13 +22,16 @@
 // truncates its sums, so a tile's products go to fresh accumulators that are
 // added to the running ones in rounded fp32.
 //
-// Work: tiles of 32 positions of one (sequence, kv head, 8 query heads).  All
-// tiles of the batch, in order, are divided evenly over the CTAs and within a
-// CTA over its four warps, so ragged batches and single long sequences load
-// every SM alike.  A warp streams its tiles through its own ring in shared
-// memory (16-byte asynchronous copies, two tiles ahead) with a running
-// softmax; parts of one item that lie in one CTA are merged in shared memory,
-// parts in several CTAs through the workspace by k_q4_combine.
+// Work: tiles of 64 positions (32 from head size 160 on) of one (sequence, kv
+// head, 8 query heads).  All tiles of the batch, in order, are divided evenly
+// over the CTAs and within a CTA over its four warps, so ragged batches and
+// single long sequences load every SM alike.  A warp streams its tiles through
+// its own ring in shared memory (bulk copies of the runs of rows that lie
+// together, one lane each; 16-byte asynchronous copies where a contiguous
+// cache's context is no multiple of 4 positions, which puts rows off the
+// 16-byte boundaries) with a running softmax; parts of one item that lie in
+// one CTA are merged in shared memory, parts in several CTAs through the
+// workspace by k_q4_combine.
 #include "attention.cuh"
 #include "kv_q4.cuh"
 #include "lmc_common.cuh"
@@ -36,20 +39,16 @@
 
 namespace {
 
-__device__ int g_attn_q4_err;  // a page id outside the pool was met (lmc_device_status)
+__device__ int g_attn_q4_err;  // bit 0: a page id outside the pool, bit 1: a wait ran out (lmc_device_status)
 
 constexpr int Q4_WARPS = 4;
-constexpr int Q4_TILE = 32;    // positions per tile
-#ifndef Q4_ST
-#define Q4_ST 3
-#define Q4_MB 3
-#endif
-constexpr int Q4_STAGES = Q4_ST;   // tiles in a warp's ring
-#ifndef Q4_SETUP
-#define Q4_SETUP 2
-#endif
-constexpr int Q4_ITEM = Q4_SETUP;      // what beginning and ending an item costs, in tiles
+constexpr int Q4_STAGES = 2;  // tiles in a warp's ring
+constexpr int Q4_ITEM = 1;    // what beginning and ending an item costs, in tiles
 constexpr float LOG2E = 1.4426950408889634f;
+// Limit of a wait for bulk copies (nanoseconds of %globaltimer).
+__device__ long long g_attn_q4_wait_ns = 1000000000ll;
+
+constexpr int q4_tile(int NB) { return NB <= 4 ? 64 : 32; }  // positions per tile (registers and shared memory)
 
 struct Q4Args {
     AttnArgs a;
@@ -57,14 +56,16 @@ struct Q4Args {
     int rmin;       // tiles per CTA at least (workspace slots per head: a.nsplit)
     int items_only; // 1: an item is never divided (a.nsplit is 1)
     int batch, vec; // vec: q, new rows and out can be moved 16 bytes at a time
+    int bulk;       // every run of rows starts on a 16-byte boundary, four rows are whole 16-byte pieces
+    int run;        // rows that lie together: a page's, at most a tile's
     int page_bytes; // of one kv head's rows of a page
 };
 
 template <int NB> struct Q4 {
-    static constexpr int DH = 32 * NB, NG = kv_q4_groups(DH), RB = kv_q4_row_bytes(DH);
-    static constexpr int SIDE = Q4_TILE * RB + 16;        // a tile's K or V rows, from any 4-byte phase
+    static constexpr int T = q4_tile(NB), DH = 32 * NB, NG = kv_q4_groups(DH), RB = kv_q4_row_bytes(DH);
+    static constexpr int SIDE = T * RB + 16;              // a tile's K or V rows, from any 4-byte phase
     static constexpr int STAGE = 2 * SIDE;
-    static constexpr int META = Q4_TILE * NG * 2;         // floats: (d, m) of a tile's rows, one side
+    static constexpr int META = T * NG * 2;               // floats: (d, m') of a tile's rows, one side
     static constexpr int FRESH = (2 * RB + 15) / 16 * 16; // the new K and V rows
     static constexpr int WARP_BYTES = Q4_STAGES * STAGE + 2 * META * 4 + FRESH;
     static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, offset, sum)
@@ -86,13 +87,61 @@ __device__ __forceinline__ void hmma0(float (&c)[4], uint32_t a0, uint32_t a1, u
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
+// Two fp32 numbers, one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
+          "l"(reinterpret_cast<unsigned long long &>(c)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
 // x, y as fp16 pairs hi + lo
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    float rx, ry;  // hi - x, hi - y
+    asm("sub.f32.f16 %0, %1, %2;" : "=f"(rx) : "h"(__half_as_ushort(__low2half(h))), "f"(x));
+    asm("sub.f32.f16 %0, %1, %2;" : "=f"(ry) : "h"(__half_as_ushort(__high2half(h))), "f"(y));
+    const __half2 l = __floats2half2_rn(-rx, -ry);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// Barrier of a stage's bulk copies.
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+// Bounded: false (and the time-out is recorded) when the copies have not landed within the limit.
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity) {
+    long long t0, t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    do {
+        if (bar_try(bar, parity)) return true;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    } while (t - t0 < g_attn_q4_wait_ns);
+    atomicOr(&g_attn_q4_err, 2);
+    return false;
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const uint8_t *src, int bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 // Eight codes of a word, less 8, as fp16 pairs: nibbles (0, 4), 16 x (1, 5), (2, 6), 16 x (3, 7).
@@ -131,22 +180,22 @@ __device__ __forceinline__ int seq_pos(const Q4Args &g, int b) {  // position, o
 }
 __device__ __forceinline__ int item_units(const Q4Args &g, int nt) { return g.items_only ? 1 : nt + Q4_ITEM; }
 // The item at (p.b, p.j), p.nt and p.pos known; its tiles up to the share's end.
-template <int RB> __device__ __forceinline__ void set_item(const Q4Args &g, Item &p) {
+template <int NB> __device__ __forceinline__ void set_item(const Q4Args &g, Item &p) {
     p.kh = p.j / g.HG;
     p.end = g.items_only ? (p.left > 0 ? p.nt : 0) : min(p.nt, p.left - Q4_ITEM);
     const long long cs = g.a.seq ? __ldg(g.a.seq + p.b) : p.b;
     p.row = g.a.pages + cs * g.a.max_pages;
-    p.off = (cs * g.a.Hkv + p.kh) * g.a.S * RB;
+    p.off = (cs * g.a.Hkv + p.kh) * g.a.S * Q4<NB>::RB;
 }
-__device__ __forceinline__ void set_seq(const Q4Args &g, Item &p) {  // first sequence >= p.b with work
+template <int NB> __device__ __forceinline__ void set_seq(const Q4Args &g, Item &p) {  // first sequence >= p.b with work
     p.pos = -1;
     while (p.b < g.batch && (p.pos = seq_pos(g, p.b)) < 0) p.b++;
-    p.nt = p.pos / Q4_TILE + 1;
+    p.nt = p.pos / Q4<NB>::T + 1;
 }
 // The share's next item, in place (tile == end: there is none).  The items of
 // the copies and of the computation lie in shared memory: only what each tile
 // needs is kept in registers.
-template <int RB> __device__ __noinline__ void next_item(const Q4Args &g, Item *at) {
+template <int NB> __device__ __noinline__ void next_item(const Q4Args &g, Item *at) {
     Item p = *at;
     const int units = item_units(g, p.nt);
     p.unit += units;
@@ -156,9 +205,9 @@ template <int RB> __device__ __noinline__ void next_item(const Q4Args &g, Item *
         if (++p.j == g.a.Hkv * g.HG) {
             p.j = 0;
             p.b++;
-            set_seq(g, p);
+            set_seq<NB>(g, p);
         }
-        set_item<RB>(g, p);
+        set_item<NB>(g, p);
         p.end = max(p.end, 0);
     }
     __syncwarp();
@@ -166,55 +215,30 @@ template <int RB> __device__ __noinline__ void next_item(const Q4Args &g, Item *
     __syncwarp();
 }
 
-// Byte offset of row t of an item in its cache; *ok: its page is in the pool (page 0 is taken if not).
-template <int RB>
-__device__ __forceinline__ long long row_offset(const Q4Args &g, long long off, const int *row, int kh, int t, bool *ok) {
+__device__ __forceinline__ int checked_page(const AttnArgs &a, int pg, bool *ok) {  // page 0 for one outside the pool
+    if ((unsigned)pg < (unsigned)a.n_pages) return pg;
+    atomicOr(&g_attn_q4_err, 1);
+    *ok = false;
+    return 0;
+}
+// Byte offset of row t of an item in its cache; *ok: its page is in the pool.
+template <int NB> __device__ __forceinline__ long long row_offset(const Q4Args &g, const Item &it, int t, bool *ok) {
     const AttnArgs &a = g.a;
-    if (!a.pages) return off + (long long)t * RB;
-    int pg = __ldg(row + (t >> a.page_shift));
-    if ((unsigned)pg >= (unsigned)a.n_pages) {
-        atomicExch(&g_attn_q4_err, 1);
-        *ok = false;
-        pg = 0;
-    }
-    return ((long long)pg * a.Hkv + kh) * g.page_bytes + (t & ((1 << a.page_shift) - 1)) * RB;
+    if (!a.pages) return it.off + (long long)t * Q4<NB>::RB;
+    const int pg = checked_page(a, __ldg(it.row + (t >> a.page_shift)), ok);
+    return ((long long)pg * a.Hkv + it.kh) * g.page_bytes + (t & ((1 << a.page_shift) - 1)) * Q4<NB>::RB;
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_run(uint32_t dst, const uint8_t *src, int bytes, int lane) {
-    // from the 16-byte boundary at or before src; the last copy reads no byte past the run
-    const int phase = (int)((uintptr_t)src & 15);
-    for (int i = 16 * lane; i < bytes + phase; i += 512)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i), "l"(src - phase + i), "r"(min(16, bytes + phase - i))
-                     : "memory");
-}
-// Starts the copies of a tile of fewer rows (all but the new row), or of rows off the 16-byte boundaries.
-template <int NB> __device__ __noinline__ void fetch_part(const Q4Args &g, const Item *it, int tile, uint32_t stage) {
-    const AttnArgs &a = g.a;
-    constexpr int RB = Q4<NB>::RB;
-    const int t0 = tile * Q4_TILE, rows = min(Q4_TILE, (a.append ? it->pos : it->pos + 1) - t0), lane = threadIdx.x & 31;
-    const int run = a.pages && a.page_shift == 4 ? 16 : Q4_TILE;  // rows that lie one behind the other
-    for (int r = 0; r < rows; r += run) {
-        bool ok;
-        const long long off = row_offset<RB>(g, it->off, it->row, it->kh, t0 + r, &ok);
-        const int bytes = min(run, rows - r) * RB;
-        copy_run(stage + r * RB, (const uint8_t *)a.k_cache + off, bytes, lane);
-        copy_run(stage + Q4<NB>::SIDE + r * RB, (const uint8_t *)a.v_cache + off, bytes, lane);
-    }
-}
-// Starts the copies of a whole tile: k, v at this lane's first 16 bytes; the
-// second 16 rows lie at k + two (0 unless pages have 16 rows).
-template <int NB> __device__ __forceinline__ void fetch_tile(const uint8_t *k, long long v, long long two, uint32_t stage, int lane) {
-    constexpr int CH = 2 * Q4<NB>::RB;  // 16-byte pieces
-#pragma unroll
-    for (int i = 0; i < (CH + 31) / 32; i++) {
-        const int c = lane + 32 * i;
-        if (c < CH) {
-            const uint8_t *at = k + 512 * i + (32 * i + 31 < CH / 2 ? 0 : 32 * i >= CH / 2 ? two : c < CH / 2 ? 0 : two);
-            cp16(stage + 512 * i, at);
-            cp16(stage + Q4<NB>::SIDE + 512 * i, at + v);
-        }
+// Starts the copies of a tile's rows, from any 4-byte phase: from the 16-byte
+// boundary at or before the first row; the last copy reads no byte past the run.
+template <int NB> __device__ __noinline__ void fetch_unaligned(const Q4Args &g, const Item *it, int tile, int rows, uint32_t stage) {
+    bool ok;
+    const long long off = row_offset<NB>(g, *it, tile * Q4<NB>::T, &ok);
+    const int phase = (int)(off & 15), bytes = rows * Q4<NB>::RB + phase;  // (the caches themselves are aligned)
+    const uint8_t *k = (const uint8_t *)g.a.k_cache + off - phase, *v = (const uint8_t *)g.a.v_cache + off - phase;
+    for (int i = 16 * (threadIdx.x & 31); i < bytes; i += 512) {
+        const int n = min(16, bytes - i);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + i), "l"(k + i), "r"(n) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + Q4<NB>::SIDE + i), "l"(v + i), "r"(n) : "memory");
     }
 }
 
@@ -244,8 +268,9 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 template <int NB> struct Q4State {
     uint32_t qa[2 * NB][4];           // q as matrix operands: head g hi, lo, hi, lo
     float qsum[Q4<NB>::NG], qfac;     // head g: sum(q_j) and the factor of its products (q scaled to fp16's range)
-    float o[2 * NB][4];               // dims x heads (see the output below)
-    float om[Q4<NB>::NG], l, off, mx; // head g, this lane's positions: sum p m, sum p; offset and maximum of s
+    float2 o[2 * NB][2];              // dims x heads (see the output below)
+    float2 om[Q4<NB>::NG], l;         // head g, this lane's positions (two sums each): p m', p
+    float off, mx;                    // offset and maximum of s
     int vexp;                         // largest exponent field of the values' d so far
 };
 
@@ -293,10 +318,10 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
         split2(x[i][3] * dn, x[i][7] * dn, st.qa[2 * i + 1][2], st.qa[2 * i + 1][3]);
     }
 #pragma unroll
-    for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = st.o[i][2] = st.o[i][3] = 0.0f;
+    for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < Q4<NB>::NG; i++) st.om[i] = 0.0f;
-    st.l = 0.0f;
+    for (int i = 0; i < Q4<NB>::NG; i++) st.om[i] = make_float2(0.0f, 0.0f);
+    st.l = make_float2(0.0f, 0.0f);
     st.off = st.mx = -INFINITY;
     st.vexp = 0;
 }
@@ -315,7 +340,7 @@ template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const 
     }
     if (lane < NW) rope8(a, p.pos, DH, 8 * lane, x[0]);
     bool ok = true;
-    const long long off = row_offset<RB>(g, p.off, p.row, p.kh, p.pos, &ok);
+    const long long off = row_offset<NB>(g, p, p.pos, &ok);
     ok &= p.j == p.kh * g.HG;
 #pragma unroll 1
     for (int side = 0; side < 2; side++) {
@@ -336,67 +361,77 @@ template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const 
 }
 
 // One tile: n valid rows at kt / vt (row r at r * RB); kdm, vdm: this warp's
-// (d, m) floats.  Of each 16 rows lane (g, t) holds the scores of head g at
-// rows 4 t .. 4 t + 3 (matrix column order 0, 2 | 1, 3: rows that a quarter
-// warp reads then lie in different banks).
+// (d, m') floats.  Of each 16 rows (h) lane (g, t) holds the scores of head g
+// at rows 4 t + 2 e + par, as pairs over e: matrix columns then are rows 2 g
+// + par (QK) and 4 t + (0, 2 | 1, 3) (PV), which lie in different banks.  The
+// factors of a pair of rows are one 16-byte word: d, d, m', m'.
 template <int NB>
 __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, const uint8_t *vt, float *kdm, float *vdm, int n, int lane) {
-    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, DH = Q4<NB>::DH;
+    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, DH = Q4<NB>::DH, T = Q4<NB>::T, NH = T / 16;
     const int gq = lane >> 2, t = lane & 3;
-    // (d, m') of row `lane` to floats; rows past the end: d = m' = 0
+    // factors of rows `lane`, lane + 32; rows past the end: d = m' = 0
     uint32_t dmax = 0;
 #pragma unroll
-    for (int j = 0; j < NG; j++) {
-        uint32_t kw = *reinterpret_cast<const uint32_t *>(kt + lane * RB + DH / 2 + 4 * j);
-        uint32_t vw = *reinterpret_cast<const uint32_t *>(vt + lane * RB + DH / 2 + 4 * j);
-        if (lane >= n) kw = vw = 0u;
-        float2 kf = __half22float2(*reinterpret_cast<const __half2 *>(&kw));
-        float2 vf = __half22float2(*reinterpret_cast<const __half2 *>(&vw));
-        kf.y = fmaf(8.0f, kf.x, kf.y);
-        vf.y = fmaf(8.0f, vf.x, vf.y);
-        *reinterpret_cast<float2 *>(kdm + 2 * (lane * NG + j)) = kf;
-        *reinterpret_cast<float2 *>(vdm + 2 * (lane * NG + j)) = vf;
-        dmax = max(dmax, vw & 0xffffu);
+    for (int r = 0; r < T; r += 32) {
+        const int to = 4 * ((lane >> 1 & 14) | (lane & 1)) + (lane >> 1 & 1) + 2 * r;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            uint32_t kw = *reinterpret_cast<const uint32_t *>(kt + (r + lane) * RB + DH / 2 + 4 * j);
+            uint32_t vw = *reinterpret_cast<const uint32_t *>(vt + (r + lane) * RB + DH / 2 + 4 * j);
+            if (r + lane >= n) kw = vw = 0u;
+            const float2 kf = __half22float2(*reinterpret_cast<const __half2 *>(&kw));
+            const float2 vf = __half22float2(*reinterpret_cast<const __half2 *>(&vw));
+            kdm[to + 2 * T * j] = kf.x;
+            kdm[to + 2 * T * j + 2] = fmaf(8.0f, kf.x, kf.y);
+            vdm[to + 2 * T * j] = vf.x;
+            vdm[to + 2 * T * j + 2] = fmaf(8.0f, vf.x, vf.y);
+            dmax = max(dmax, vw & 0xffffu);
+        }
     }
     const int vexp = min((int)(__reduce_max_sync(0xffffffffu, dmax) >> 10), 30);
     __syncwarp();
-    // scores over qfac, group by group: the 32 rows' four column sets (rows
-    // 16 h + 2 g + par) are four independent chains of products
-    float s[2][4];  // [16 rows][row 4 t + r]
+    // scores over qfac, group by group; four column sets at a time are independent chains of products
+    float2 s[NH][2];  // [16 rows][par]
     const uint32_t *const kr = reinterpret_cast<const uint32_t *>(kt + 2 * gq * RB) + t;
 #pragma unroll
-    for (int j = 0; j < NG; j++) {
-        float c[4][4];
+    for (int h0 = 0; h0 < NH; h0 += 2) {
 #pragma unroll
-        for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
+        for (int j = 0; j < NG; j++) {
+            float c[4][4];
 #pragma unroll
-            for (int hp = 0; hp < 4; hp++) {
-                uint32_t w[4];
-                codes8(kr[(16 * (hp >> 1) + (hp & 1)) * (RB / 4) + 4 * i], w);
-                if (i % 2) hmma(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
-                else hmma0(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
-                hmma(c[hp], st.qa[2 * i + 1][0], st.qa[2 * i + 1][1], st.qa[2 * i + 1][2], st.qa[2 * i + 1][3], w[1], w[3]);
+            for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
+#pragma unroll
+                for (int hp = 0; hp < 4; hp++) {
+                    uint32_t w[4];
+                    codes8(kr[(16 * (h0 + (hp >> 1)) + (hp & 1)) * (RB / 4) + 4 * i], w);
+                    if (i % 2) hmma(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
+                    else hmma0(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
+                    hmma(c[hp], st.qa[2 * i + 1][0], st.qa[2 * i + 1][1], st.qa[2 * i + 1][2], st.qa[2 * i + 1][3], w[1], w[3]);
+                }
+            }
+#pragma unroll
+            for (int hp = 0; hp < 4; hp++) {  // columns 2 t, 2 t + 1: rows 4 t + par, 4 t + 2 + par
+                const int h = h0 + (hp >> 1), par = hp & 1;
+                const float4 dm = *reinterpret_cast<const float4 *>(kdm + 4 * (2 * (4 * h + t) + par) + 2 * T * j);
+                const float2 d = make_float2(dm.x, dm.y), m = make_float2(dm.z, dm.w);
+                const float2 x = add2(make_float2(c[hp][0], c[hp][1]), make_float2(c[hp][2], c[hp][3]));
+                s[h][par] = j ? fma2(d, x, s[h][par]) : mul2(d, x);
+                s[h][par] = fma2(m, make_float2(st.qsum[j], st.qsum[j]), s[h][par]);
             }
         }
-#pragma unroll
-        for (int hp = 0; hp < 4; hp++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {  // columns 2 t, 2 t + 1: rows 4 t + par, 4 t + 2 + par
-                const int h = hp >> 1, r = 2 * e + (hp & 1);
-                const float2 dm = *reinterpret_cast<const float2 *>(kdm + 2 * (NG * (16 * h + 4 * t + r) + j));
-                const float x = c[hp][e] + c[hp][2 + e];
-                s[h][r] = j ? fmaf(dm.x, x, s[h][r]) : dm.x * x;
-                s[h][r] = fmaf(dm.y, st.qsum[j], s[h][r]);
-            }
     }
-    if (n < Q4_TILE)
+    if (n < T)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < NH; h++)
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (16 * h + 4 * t + r >= n) s[h][r] = -INFINITY;
+            for (int par = 0; par < 2; par++) {
+                if (16 * h + 4 * t + par >= n) s[h][par].x = -INFINITY;
+                if (16 * h + 4 * t + 2 + par >= n) s[h][par].y = -INFINITY;
+            }
     // running maximum of head g and exponent of the values' scales
-    float m = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    float m = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < NH; h++) m = fmaxf(m, fmaxf(fmaxf(s[h][0].x, s[h][0].y), fmaxf(s[h][1].x, s[h][1].y)));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     m = fmaxf(m * st.qfac, st.mx);
@@ -405,49 +440,44 @@ __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, 
     st.mx = m;
     st.off = off;
     st.vexp = ve;
-    st.l *= f;
-    const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+    const float2 ff = make_float2(__shfl_sync(0xffffffffu, f, 8 * t), __shfl_sync(0xffffffffu, f, 8 * t + 4));
+    st.l = mul2(st.l, make_float2(f, f));
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int h = 0; h < NH; h++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            s[h][r] = ex2(fmaf(s[h][r], st.qfac, -off));
-            st.l += s[h][r];
+        for (int par = 0; par < 2; par++) {
+            const float2 e = fma2(s[h][par], make_float2(st.qfac, st.qfac), make_float2(-off, -off));
+            s[h][par] = make_float2(ex2(e.x), ex2(e.y));
+            st.l = add2(st.l, s[h][par]);
         }
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        uint32_t bh[2][2], bl[2][2];  // p d of the 16 rows of each half: hi, lo
-        st.om[j] *= f;
+        uint32_t bh[NH][2], bl[NH][2];  // p d of the 16 rows of each set: hi, lo
+        st.om[j] = mul2(st.om[j], make_float2(f, f));
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float w[4];
+        for (int h = 0; h < NH; h++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float2 dm = *reinterpret_cast<const float2 *>(vdm + 2 * (NG * (16 * h + 4 * t + r) + j));
-                w[r] = s[h][r] * dm.x;
-                st.om[j] = fmaf(s[h][r], dm.y, st.om[j]);
+            for (int par = 0; par < 2; par++) {
+                const float4 dm = *reinterpret_cast<const float4 *>(vdm + 4 * (2 * (4 * h + t) + par) + 2 * T * j);
+                const float2 w = mul2(s[h][par], make_float2(dm.x, dm.y));
+                st.om[j] = fma2(s[h][par], make_float2(dm.z, dm.w), st.om[j]);
+                split2(w.x, w.y, bh[h][par], bl[h][par]);
             }
-            split2(w[0], w[2], bh[h][0], bl[h][0]);
-            split2(w[1], w[3], bh[h][1], bl[h][1]);
-        }
         // this lane's dims: word g of the group, or half a word of a group of 32
         const bool half = NB % 2 && j == NG - 1;
         const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
-        uint32_t cw[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) cw[h][r] = *reinterpret_cast<const uint32_t *>(vr + (16 * h + r) * RB);
 #pragma unroll
         for (int k = 0; k < (half ? 1 : 2); k++) {  // nibbles 0-3, 4-7 of the words (or the half word's four)
             const uint32_t sel = half ? ((gq & 1) ? 0x7632u : 0x5410u) : (k ? 0x7632u : 0x5410u);
             const int i = 4 * j + 2 * k;
             float c[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t x[4], y[4];  // rows 4 t + (0, 2) and (1, 3)
-                codes8(__byte_perm(cw[h][0], cw[h][2], sel), x);
-                codes8(__byte_perm(cw[h][1], cw[h][3], sel), y);
+            for (int h = 0; h < NH; h++) {
+                uint32_t cw[4], x[4], y[4];  // rows 4 t + (0, 2) and (1, 3)
+#pragma unroll
+                for (int r = 0; r < 4; r++) cw[r] = *reinterpret_cast<const uint32_t *>(vr + (16 * h + r) * RB);
+                codes8(__byte_perm(cw[0], cw[2], sel), x);
+                codes8(__byte_perm(cw[1], cw[3], sel), y);
                 if (h) {
                     hmma(c[0], x[0], x[1], y[0], y[1], bh[h][0], bh[h][1]);
                     hmma(c[1], x[2], x[3], y[2], y[3], bh[h][0], bh[h][1]);
@@ -460,10 +490,8 @@ __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, 
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                st.o[i + e][0] = fmaf(st.o[i + e][0], f0, c[e][0]);
-                st.o[i + e][1] = fmaf(st.o[i + e][1], f1, c[e][1]);
-                st.o[i + e][2] = fmaf(st.o[i + e][2], f0, c[e][2]);
-                st.o[i + e][3] = fmaf(st.o[i + e][3], f1, c[e][3]);
+                st.o[i + e][0] = fma2(st.o[i + e][0], ff, make_float2(c[e][0], c[e][1]));
+                st.o[i + e][1] = fma2(st.o[i + e][1], ff, make_float2(c[e][2], c[e][3]));
             }
         }
     }
@@ -476,7 +504,7 @@ __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, 
 template <int NB>
 __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
     const int gq = lane >> 2, t = lane & 3;
-    float l = st.l;
+    float l = st.l.x + st.l.y;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (!fin && t == 0 && gq < heads) {
@@ -490,15 +518,16 @@ __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *d
         const float iv = __shfl_sync(0xffffffffu, inv, from);
 #pragma unroll
         for (int j = 0; j < Q4<NB>::NG; j++) {
-            float m = st.om[j];
+            float m = st.om[j].x + st.om[j].y;
             m += __shfl_xor_sync(0xffffffffu, m, 1);
             m += __shfl_xor_sync(0xffffffffu, m, 2);
             m = __shfl_sync(0xffffffffu, m, from);
             const bool half = NB % 2 && j == Q4<NB>::NG - 1;
 #pragma unroll
             for (int k = 0; k < (half ? 1 : 2); k++) {
-                const float *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
-                const float4 v = make_float4((a[hd] + m) * iv, fmaf(a[2 + hd], 0.0625f, m) * iv, (b[hd] + m) * iv, fmaf(b[2 + hd], 0.0625f, m) * iv);
+                const float2 *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];  // (pairs over the heads)
+                const float4 v = make_float4(((hd ? a[0].y : a[0].x) + m) * iv, fmaf(hd ? a[1].y : a[1].x, 0.0625f, m) * iv,
+                                             ((hd ? b[0].y : b[0].x) + m) * iv, fmaf(hd ? b[1].y : b[1].x, 0.0625f, m) * iv);
                 float *o = dst + h * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
                 if (h >= heads) continue;
                 if (vec) *reinterpret_cast<float4 *>(o) = v;
@@ -509,11 +538,12 @@ __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *d
 }
 
 template <int NB>
-__global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? Q4_MB : 2) k_attn_q4(const __grid_constant__ Q4Args g) {
+__global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_constant__ Q4Args g) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Item sh_item[Q4_WARPS][2];  // of the copies, of the computation
+    __shared__ __align__(8) uint64_t sh_bar[Q4_WARPS][Q4_STAGES];
     __shared__ int sh_total[Q4_WARPS], desc[Q4_WARPS][2][5];  // a warp's parts: first unit of the item, b, j, first tile, end
-    constexpr int DH = Q4<NB>::DH, SLOT = Q4<NB>::SLOT, RB = Q4<NB>::RB;
+    constexpr int DH = Q4<NB>::DH, SLOT = Q4<NB>::SLOT, RB = Q4<NB>::RB, T = Q4<NB>::T;
     const AttnArgs &a = g.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = a.H / a.Hkv, items = a.Hkv * g.HG, GH = min(G, 8);
@@ -522,7 +552,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? Q4_MB : 2) k_attn_q4(
     // units (tiles) of the whole batch, and this CTA's and this warp's share
     auto units_of = [&](int b) -> int {
         const int p = seq_pos(g, b);
-        return p < 0 ? 0 : item_units(g, p / Q4_TILE + 1) * items;
+        return p < 0 ? 0 : item_units(g, p / T + 1) * items;
     };
     int sum = 0;
     for (int b = threadIdx.x; b < g.batch; b += 32 * Q4_WARPS) sum += units_of(b);
@@ -530,6 +560,9 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? Q4_MB : 2) k_attn_q4(
     if (lane == 0) {
         sh_total[warp] = sum;
         desc[warp][0][0] = desc[warp][1][0] = -1;
+        for (int i = 0; i < Q4_STAGES; i++)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&sh_bar[warp][i])));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     const int total = sh_total[0] + sh_total[1] + sh_total[2] + sh_total[3];
@@ -565,99 +598,103 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? Q4_MB : 2) k_attn_q4(
             }
             before += __shfl_sync(0xffffffffu, inc, 31);
         }
-        set_seq(g, p);
+        set_seq<NB>(g, p);
         const int at = u0 - before, per = item_units(g, p.nt);
         p.j = at / per;
         p.unit = u0 - at % per;
         p.left = u1 - p.unit;
         p.tile = g.items_only ? 0 : max(0, at % per - Q4_ITEM);
-        set_item<RB>(g, p);
+        set_item<NB>(g, p);
         Item *const ia = &sh_item[warp][0], *const ii = &sh_item[warp][1];
         *ia = p;
         *ii = p;
         __syncwarp();
-        // the copies' place: tiles [tile, end) of an item, the first `whole` of it without special cases
-        const uint8_t *const kc = (const uint8_t *)a.k_cache + 16 * lane;
-        const long long kv = (const uint8_t *)a.v_cache - (const uint8_t *)a.k_cache;
-        const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
-        const bool two = a.pages && a.page_shift == 4;
-        int a_tile, a_end, a_whole, a_kh, a_pg = 0, a_pg2 = 0, fill = 0;  // (pages looked up one tile ahead)
-        const uint8_t *a_src = nullptr;  // contiguous: this lane's first piece of tile a_tile
-        const int *a_row;
+        // The copies' place: tiles [a_tile, a_end) of an item of which a_rows
+        // rows are copied.  Lanes 0-3 copy the K rows' runs, lanes 4-7 the V
+        // rows'; a lane looks its page up one tile ahead.
+        const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring), bar = (uint32_t)__cvta_generic_to_shared(&sh_bar[warp][0]);
+        const uint8_t *const cache = (const uint8_t *)(lane & 4 ? a.v_cache : a.k_cache);
+        const int r0 = (lane & 3) * g.run;  // first row of this lane's run; T or more: it has none
+        const uint32_t to = (lane & 4 ? Q4<NB>::SIDE : 0) + r0 * RB;
+        int a_tile, a_end, a_rows, a_pg = 0;
         auto look_up = [&]() {
-            if (a_tile < a_whole) {
-                a_pg = __ldg(a_row + (a_tile * Q4_TILE >> a.page_shift));
-                if (two) a_pg2 = __ldg(a_row + 2 * a_tile + 1);
-            }
+            if (a.pages && a_tile * T + r0 < a_rows && r0 < T) a_pg = __ldg(ia->row + ((a_tile * T + r0) >> a.page_shift));
         };
         auto item_ahead = [&]() {
             a_tile = ia->tile;
             a_end = ia->end;
-            a_kh = ia->kh;
-            a_row = ia->row;
-            const int rows = a.append ? ia->pos : ia->pos + 1;
-            if (a.pages) {
-                a_whole = min(rows / Q4_TILE, a_end);
-                look_up();
-            } else {
-                a_whole = ia->off & 15 ? 0 : min(rows / Q4_TILE, a_end);
-                a_src = kc + ia->off + (long long)a_tile * (Q4_TILE * RB);
-            }
+            a_rows = a.append ? ia->pos : ia->pos + 1;
+            look_up();
         };
-        auto page_at = [&](int pg) -> const uint8_t * {  // this lane's first piece of a page's rows
-            if ((unsigned)pg >= (unsigned)a.n_pages) {
-                atomicExch(&g_attn_q4_err, 1);
-                pg = 0;
+        auto fetch = [&](int i) {  // tile a_tile into stage i
+            const int rows = min(T, a_rows - a_tile * T);
+            const uint32_t stage = ring_s + i * Q4<NB>::STAGE;
+            if (!g.bulk) {
+                if (rows > 0) fetch_unaligned<NB>(g, ia, a_tile, rows, stage);
+                return;
             }
-            return kc + ((long long)pg * a.Hkv + a_kh) * g.page_bytes;
+            const int some = rows > 0 ? (rows + 3) & ~3 : 0;  // (at most three rows more, of the same page or cache)
+            if (lane == 0) bar_expect(bar + 8 * i, 2 * some * RB);
+            __syncwarp();
+            if (lane < 8 && r0 < some) {
+                long long off;
+                if (a.pages) {
+                    bool ok;
+                    off = ((long long)checked_page(a, a_pg, &ok) * a.Hkv + ia->kh) * g.page_bytes +
+                          ((a_tile * T + r0) & ((1 << a.page_shift) - 1)) * RB;
+                } else {
+                    off = ia->off + (long long)a_tile * (T * RB);
+                }
+                bulk_copy(stage + to, cache + off, min(g.run, some - r0) * RB, bar + 8 * i);
+            }
         };
         item_ahead();
-        int tile = p.tile, end = p.end, nt = p.nt, phase = 0, stage = 0, part = 0;
+        int tile = p.tile, end = p.end, nt = p.nt, phase = 0, part = 0, stage = 0, fill = 0;
+        uint32_t parity = 0, flying = 0;  // phase bits of the stages' barriers; stages whose copies are not waited for
         bool begin = true;
         Q4State<NB> st;
 #pragma unroll 1
         for (int skip = Q4_STAGES - 1; tile < end; skip--) {  // the first turns only start copies
             if (a_tile < a_end) {
-                if (a_tile < a_whole) {
-                    long long o2 = 0;
-                    if (a.pages) {
-                        a_src = page_at(a_pg) + ((a_tile * Q4_TILE) & ((1 << a.page_shift) - 1)) * RB;
-                        if (two) o2 = page_at(a_pg2) - 16 * RB - a_src;
-                    }
-                    fetch_tile<NB>(a_src, kv, o2, ring_s + fill, lane);
-                } else {
-                    fetch_part<NB>(g, ia, a_tile, ring_s - 16 * lane + fill);
-                }
-                a_tile++;
-                a_src += Q4_TILE * RB;
-                if (a_tile == a_end) {
-                    next_item<RB>(g, ia);
+                fetch(fill);
+                flying |= 1u << fill;
+                if (++a_tile == a_end) {
+                    next_item<NB>(g, ia);
                     item_ahead();
-                } else if (a.pages) {
+                } else {
                     look_up();
                 }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            fill = fill == (Q4_STAGES - 1) * Q4<NB>::STAGE ? 0 : fill + Q4<NB>::STAGE;
+            if (!g.bulk) asm volatile("cp.async.commit_group;" ::: "memory");
+            fill = fill + 1 == Q4_STAGES ? 0 : fill + 1;
             if (skip > 0) continue;
             if (begin) {
-                phase = a.pages ? 0 : (int)(ii->off & 15);  // rows lie in the ring at the phase that they have in the cache
+                phase = g.bulk ? 0 : (int)(ii->off & 15);  // rows lie in the ring at the phase that they have in the cache
                 if (a.append && end == nt) append<NB>(g, *ii, fresh, lane);
                 load_q<NB>(g, *ii, lane, st);
                 begin = false;
             }
-            asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 1) : "memory");
-            __syncwarp();
-            uint8_t *kt = ring + stage + phase;
-            stage = stage == (Q4_STAGES - 1) * Q4<NB>::STAGE ? 0 : stage + Q4<NB>::STAGE;
-            int n = Q4_TILE;
+            if (!g.bulk) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(Q4_STAGES - 1) : "memory");
+                __syncwarp();
+            } else {
+                bool here = bar_try(bar + 8 * stage, parity >> stage & 1);
+                if (!here) here = bar_wait_long(bar + 8 * stage, parity >> stage & 1);
+                if (!__all_sync(0xffffffffu, here)) break;  // gave up: no result for this item (lmc_device_status)
+                parity ^= 1u << stage;
+            }
+            flying &= ~(1u << stage);
+            uint8_t *kt = ring + stage * Q4<NB>::STAGE + phase;
+            stage = stage + 1 == Q4_STAGES ? 0 : stage + 1;
+            int n = T;
             if (tile == nt - 1) {  // the item's last tile: fewer rows, the new row among them
-                n = ii->pos + 1 - tile * Q4_TILE;
+                n = ii->pos + 1 - tile * T;
                 if (a.append) {
                     for (int i = lane; i < RB / 4; i += 32) {
                         reinterpret_cast<uint32_t *>(kt + (n - 1) * RB)[i] = fresh[i];
                         reinterpret_cast<uint32_t *>(kt + Q4<NB>::SIDE + (n - 1) * RB)[i] = fresh[RB / 4 + i];
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next bulk copy
                     __syncwarp();
                 }
             }
@@ -682,13 +719,16 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? Q4_MB : 2) k_attn_q4(
                     d[4] = end;
                 }
                 part = 1;
-                next_item<RB>(g, ii);
+                next_item<NB>(g, ii);
                 tile = ii->tile;
                 end = ii->end;
                 nt = ii->nt;
                 begin = true;
             }
         }
+        // (after a wait that ran out) the copies still in flight, bounded again
+        for (int i = 0; g.bulk && i < Q4_STAGES; i++)
+            if (flying >> i & 1) bar_wait_long(bar + 8 * i, parity >> i & 1);
     }
     __syncthreads();
     // merge this CTA's parts of each item: neighbours in (warp, part) order
@@ -704,7 +744,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, NB <= 4 ? Q4_MB : 2) k_attn_q4(
             e = i;
         }
         const int b = d[1], j = d[2], h0 = (j % g.HG) * 8, heads = min(8, G - h0), kh = j / g.HG;
-        const int pos = seq_pos(g, b), nt = pos / Q4_TILE + 1;
+        const int pos = seq_pos(g, b), nt = pos / T + 1;
         const bool whole = d[3] == 0 && desc[e / 2][e % 2][4] == nt;
         // the CTAs that hold the item's first and last tile
         const int ca = (int)(((long long)(d[0] + Q4_ITEM + 1) * nC - 1) / total), cb = (int)(((long long)(d[0] + Q4_ITEM + nt) * nC - 1) / total);
@@ -814,8 +854,7 @@ template <int NB> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
     const int GH = g.a.H / g.a.Hkv < 8 ? g.a.H / g.a.Hkv : 8;
     const size_t smem = (size_t)Q4_WARPS * Q4<NB>::WARP_BYTES + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
     LMC_CUDA_TRY(cudaFuncSetAttribute(k_attn_q4<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int fit = (int)(227 * 1024 / (smem + 1536)), per_sm = fit < (NB <= 4 ? Q4_MB : 2) ? fit : (NB <= 4 ? Q4_MB : 2);
-    const int most = lmc_sm_count() * (per_sm > 0 ? per_sm : 1), want = max_units / g.rmin;
+    const int most = lmc_sm_count() * (smem + 2048 <= 114 * 1024 ? 2 : 1), want = max_units / g.rmin;
     LMC_LAUNCH("attention (4-bit rows)", k_attn_q4<NB>, want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);
     return LMC_OK;
 }
@@ -832,7 +871,7 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     const size_t slot = (size_t)batch * a.H * (a.Dh + 2) * sizeof(float);
     if ((size_t)a.nsplit * slot > ws_bytes) a.nsplit = (int)(ws_bytes / slot);
     if (a.nsplit < 2 || !a.ws) a.nsplit = 1;
-    const int G = a.H / a.Hkv, NT = (a.S + Q4_TILE - 1) / Q4_TILE;
+    const int G = a.H / a.Hkv, T = q4_tile(a.Dh / 32), NT = (a.S + T - 1) / T;
     g.HG = (G + 7) / 8;
     g.batch = batch;
     g.items_only = a.nsplit == 1;
@@ -841,6 +880,8 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     g.vec = (((uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.out) & 15) == 0 && a.ldq % 4 == 0 &&
             a.ldkv % 4 == 0 && a.ldo % 4 == 0;
     g.page_bytes = kv_q4_row_bytes(a.Dh) << a.page_shift;
+    g.bulk = a.pages || a.S % 4 == 0;
+    g.run = a.pages && (1 << a.page_shift) < T ? 1 << a.page_shift : T;
     const long long units = (long long)batch * a.Hkv * g.HG * (g.items_only ? 1 : NT + Q4_ITEM);
     if (units > 0x7fffffffLL) return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: batch %d x context %d is too large", batch, a.S);
     int (*const fn[8])(const Q4Args &, int, cudaStream_t) = {launch<1>, launch<2>, launch<3>, launch<4>, launch<5>, launch<6>, launch<7>, launch<8>};
@@ -852,11 +893,18 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     return LMC_OK;
 }
 
+extern "C" int lmc_attn_q4_set_wait_limit(long long ns) {
+    const long long v = ns > 0 ? ns : 1000000000ll;
+    LMC_CUDA_TRY(cudaMemcpyToSymbol(g_attn_q4_wait_ns, &v, sizeof v));
+    return LMC_OK;
+}
+
 extern "C" int lmc_attn_q4_status(void) {
     int v = 0;
     LMC_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_attn_q4_err, sizeof(int)));
     if (!v) return LMC_OK;
     const int zero = 0;
     LMC_CUDA_TRY(cudaMemcpyToSymbol(g_attn_q4_err, &zero, sizeof(int)));
+    if (v & 2) return lmc_set_error(LMC_ERR_TIMEOUT, "4-bit attention: a bounded wait ran out (bulk copy not completed)");
     return lmc_set_error(LMC_ERR_INVALID, "paged attention: a page id outside the pool (page 0 read instead)");
 }

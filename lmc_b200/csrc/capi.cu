@@ -40,6 +40,7 @@ extern "C" int lmc_set_wait_limit(long long ns) {
     if (!rc) rc = lmc_step_set_wait_limit(ns);
     if (!rc) rc = lmc_gemm_set_wait_limit(ns);
     if (!rc) rc = lmc_peer_set_wait_limit(ns);
+    if (!rc) rc = lmc_attn_q4_set_wait_limit(ns);
     return rc;
 }
 

@@ -134,6 +134,7 @@ int lmc_kv_append_launch(const float *k, const float *v, int ldk, int ldv, void 
 /* LMC_OK, or LMC_ERR_INVALID once after a kernel of that file met an index
  * outside its range (the flag is cleared). */
 int lmc_attn_q4_status(void);
+int lmc_attn_q4_set_wait_limit(long long ns);
 int lmc_kv_rows_status(void);
 int lmc_kv_pages_status(void);
 /* Generation bookkeeping after one step (see lmc_model_generate): the greedy
