@@ -452,7 +452,7 @@ def model_decode(args, rank, world, local_rank, dist):
         obj = [path]
         dist.broadcast_object_list(obj, src=0)
         path = obj[0]
-    kvd = {"f16": rt.KV_F16, "f32": rt.KV_F32, "q8": rt.KV_Q8}[args.kv]
+    kvd = {"f16": rt.KV_F16, "f32": rt.KV_F32, "q8": rt.KV_Q8, "q4": rt.KV_Q4}[args.kv]
     B = args.batch
     rows = args.prefill_rows or None
     # paged cache: just the pages prompt + gen positions of every sequence take
@@ -545,7 +545,7 @@ def main():
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--prompt", type=int, default=512)
     ap.add_argument("--gen", type=int, default=64)
-    ap.add_argument("--kv", choices=["f16", "f32", "q8"], default="f16")
+    ap.add_argument("--kv", choices=["f16", "f32", "q8", "q4"], default="f16")
     ap.add_argument("--prefill-rows", type=int, default=0)
     ap.add_argument("--kv-page", type=int, default=0,
                     help="paged KV cache of this many positions per page, the pool sized to prompt + gen")

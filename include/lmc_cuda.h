@@ -378,10 +378,18 @@ int lmc_model_load_ex(const char *gguf_path, int max_batch, int max_rows, int kv
  * too few free.  lmc_model_release_seq gives sequence seq's pages back (its
  * cached rows are gone: start it again at position 0).  The results are the
  * same as with the contiguous cache (such models always run the step
- * kernel by kernel, not as the persistent single-launch step). */
+ * kernel by kernel, not as the persistent single-launch step).
+ * lmc_model_fork_seq makes sequence dst a copy of sequence src (its cached
+ * rows so far; dst's own pages are given back first), sharing src's pages:
+ * samples of one prompt, a common system prompt, beams.  A page that several
+ * sequences hold is copied when one of them writes into it (forward, prefill,
+ * generate and replay count those pages among the ones they take); it
+ * returns to the pool when its last sequence gives it back.  Contiguous
+ * caches are refused with LMC_ERR_UNSUPPORTED. */
 int lmc_model_load_paged(const char *gguf_path, int max_batch, int max_rows, int kv_dtype, int page_size,
                          int n_pages, int tp_rank, int tp_size, const void *nccl_id_128, lmc_model **out);
 int lmc_model_release_seq(lmc_model *m, int seq);
+int lmc_model_fork_seq(lmc_model *m, int src, int dst);
 /* Page size (0: contiguous cache), pages in the pool and pages free. */
 int lmc_model_kv_pages(const lmc_model *m, int *page_size, int *n_pages, int *n_free);
 int lmc_model_shard(const lmc_model *m, int *tp_rank, int *tp_size, int *vocab_begin, int *vocab_rows);

@@ -59,9 +59,11 @@ struct lmc_model {
      * layer's pool).  The host hands pages out before the step that first
      * writes them: h_pages mirrors the table (-1: none), seq_np[s] = pages
      * sequence s holds (always its first seq_np[s] table entries), free_ids
-     * the n_free ids not held. */
-    int page_size, page_shift, max_pages, n_pages, n_free;
-    int *d_pages, *h_pages, *seq_np, *free_ids;
+     * the n_free ids not held.  Sequences may hold the same page
+     * (lmc_model_fork_seq): page_refs[p] = sequences that hold page p,
+     * n_extra = holders beyond the first over all pages (0: none shared). */
+    int page_size, page_shift, max_pages, n_pages, n_free, n_extra;
+    int *d_pages, *h_pages, *seq_np, *free_ids, *page_refs;
     int g_pos; /* next position of the last generation's step loop (lmc_model_replay) */
     float *x, *xn, *qkv, *att, *h, *h2, *logits;
     void *ws;
@@ -538,7 +540,8 @@ static int alloc_state(lmc_model *m) {
         m->h_pages = (int *)malloc(sizeof(int) * table);
         m->seq_np = (int *)calloc(NS, sizeof(int));
         m->free_ids = (int *)malloc(sizeof(int) * (size_t)m->n_pages);
-        if (!m->h_pages || !m->seq_np || !m->free_ids) return lmc_set_error(LMC_ERR_OOM, "KV page table");
+        m->page_refs = (int *)calloc((size_t)m->n_pages, sizeof(int));
+        if (!m->h_pages || !m->seq_np || !m->free_ids || !m->page_refs) return lmc_set_error(LMC_ERR_OOM, "KV page table");
         for (size_t i = 0; i < table; i++) m->h_pages[i] = -1;
         for (int k = 0; k < m->n_pages; k++) m->free_ids[k] = m->n_pages - 1 - k; /* handed out as 0, 1, 2, ... */
         m->n_free = m->n_pages;
@@ -659,41 +662,82 @@ int lmc_model_load_paged(const char *path, int max_batch, int max_rows, int kv_d
     return model_load(path, max_batch, max_rows, kv_dtype, page_size, n_pages, tp_rank, tp_size, nccl_id, out);
 }
 
-/* Pages for positions [0, npos[i]) of sequence seqs[i], i < n (distinct
- * sequences), taken from the free ids before the step that writes them; the
- * changed table entries are copied to the device on the model's stream, so
+static int pages_upload(lmc_model *m, int seq, int first, int n) {
+    const size_t at = (size_t)seq * m->max_pages + first;
+    /* pageable source: the copy has taken the entries when the call returns */
+    CUTRY(cudaMemcpyAsync(m->d_pages + at, m->h_pages + at, sizeof(int) * (size_t)n, cudaMemcpyHostToDevice, m->stream));
+    return LMC_OK;
+}
+
+/* Page src to page dst in every layer's K and V pool, on the model's stream. */
+static int page_copy(lmc_model *m, int src, int dst) {
+    const size_t bytes = (size_t)m->hkvl * (size_t)m->page_size * LMC_KV_ROW_BYTES(m->kv_dtype, m->cfg.head_dim);
+    for (int l = 0; l < m->cfg.n_layers; l++) {
+        char *kc = (char *)m->kc + m->kv_layer_bytes * l, *vc = (char *)m->vc + m->kv_layer_bytes * l;
+        CUTRY(cudaMemcpyAsync(kc + bytes * dst, kc + bytes * src, bytes, cudaMemcpyDeviceToDevice, m->stream));
+        CUTRY(cudaMemcpyAsync(vc + bytes * dst, vc + bytes * src, bytes, cudaMemcpyDeviceToDevice, m->stream));
+    }
+    return LMC_OK;
+}
+
+/* Makes positions [from[i], npos[i]) of sequence seqs[i], i < n (distinct
+ * sequences), writable before the step that writes them: pages up to npos[i]
+ * are taken from the free ids, and a page in that range that another
+ * sequence holds too is replaced by a copy (of several writers of one page
+ * the last keeps it).  Table entries and copies go onto the model's stream, so
  * they land after every step already queued.  All or nothing: with too few
  * free pages nothing changes and the call fails with LMC_ERR_OOM. */
-static int pages_reserve(lmc_model *m, int n, const int *seqs, const int *npos) {
+static int pages_reserve(lmc_model *m, int n, const int *seqs, const int *from, const int *npos) {
     if (!m->page_size) return LMC_OK;
     long long want = 0;
     for (int i = 0; i < n; i++) {
         const int need = (npos[i] + m->page_size - 1) >> m->page_shift;
         if (need > m->seq_np[seqs[i]]) want += need - m->seq_np[seqs[i]];
     }
+    /* pages to copy: counted on page_refs itself, put back below */
+    for (int pass = 0; m->n_extra && pass < 2; pass++)
+        for (int j = 0; j < n; j++) {
+            const int i = pass ? n - 1 - j : j, need = (npos[i] + m->page_size - 1) >> m->page_shift;
+            const int *row = m->h_pages + (size_t)seqs[i] * m->max_pages;
+            for (int k = from[i] >> m->page_shift; k < need && k < m->seq_np[seqs[i]]; k++) {
+                if (pass) m->page_refs[row[k]]++;
+                else if (--m->page_refs[row[k]] > 0) want++;
+            }
+        }
     if (want > m->n_free)
         return lmc_set_error(LMC_ERR_OOM, "KV pages: %lld more needed, %d of %d free", want, m->n_free, m->n_pages);
     for (int i = 0; i < n; i++) {
         const int sq = seqs[i], need = (npos[i] + m->page_size - 1) >> m->page_shift, first = m->seq_np[sq];
-        if (need <= first) continue;
         int *row = m->h_pages + (size_t)sq * m->max_pages;
-        for (int k = first; k < need; k++) row[k] = m->free_ids[--m->n_free];
+        for (int k = from[i] >> m->page_shift; m->n_extra && k < need && k < first; k++) {
+            const int was = row[k];
+            if (m->page_refs[was] < 2) continue;
+            row[k] = m->free_ids[--m->n_free];
+            m->page_refs[row[k]] = 1;
+            m->page_refs[was]--;
+            m->n_extra--;
+            TRY(page_copy(m, was, row[k]));
+            TRY(pages_upload(m, sq, k, 1));
+        }
+        if (need <= first) continue;
+        for (int k = first; k < need; k++) {
+            row[k] = m->free_ids[--m->n_free];
+            m->page_refs[row[k]] = 1;
+        }
         m->seq_np[sq] = need;
-        /* pageable source: the copy has taken the entries when the call returns */
-        CUTRY(cudaMemcpyAsync(m->d_pages + (size_t)sq * m->max_pages + first, row + first,
-                              sizeof(int) * (size_t)(need - first), cudaMemcpyHostToDevice, m->stream));
+        TRY(pages_upload(m, sq, first, need - first));
     }
     return LMC_OK;
 }
 
-/* The same pages for one position count shared by sequences 0 .. B-1. */
-static int pages_reserve_all(lmc_model *m, int B, int npos) {
+/* The same pages for one range of positions shared by sequences 0 .. B-1. */
+static int pages_reserve_all(lmc_model *m, int B, int from, int npos) {
     if (!m->page_size) return LMC_OK;
     int rc = LMC_OK;
-    int *seqs = (int *)malloc(sizeof(int) * 2 * (size_t)B);
+    int *seqs = (int *)malloc(sizeof(int) * 3 * (size_t)B);
     if (!seqs) return lmc_set_error(LMC_ERR_OOM, "KV pages: host");
-    for (int b = 0; b < B; b++) { seqs[b] = b; seqs[B + b] = npos; }
-    rc = pages_reserve(m, B, seqs, seqs + B);
+    for (int b = 0; b < B; b++) { seqs[b] = b; seqs[B + b] = from; seqs[2 * B + b] = npos; }
+    rc = pages_reserve(m, B, seqs, seqs + B, seqs + 2 * B);
     free(seqs);
     return rc;
 }
@@ -705,14 +749,30 @@ int lmc_model_release_seq(lmc_model *m, int seq) {
     const int np = m->seq_np[seq];
     int *row = m->h_pages + (size_t)seq * m->max_pages;
     for (int k = np - 1; k >= 0; k--) {
-        m->free_ids[m->n_free++] = row[k];
+        if (--m->page_refs[row[k]] == 0) m->free_ids[m->n_free++] = row[k];
+        else m->n_extra--; /* another sequence keeps it */
         row[k] = -1;
     }
     m->seq_np[seq] = 0;
-    if (np)
-        CUTRY(cudaMemcpyAsync(m->d_pages + (size_t)seq * m->max_pages, row, sizeof(int) * (size_t)np,
-                              cudaMemcpyHostToDevice, m->stream));
-    return LMC_OK;
+    return np ? pages_upload(m, seq, 0, np) : LMC_OK;
+}
+
+int lmc_model_fork_seq(lmc_model *m, int src, int dst) {
+    if (!m || src < 0 || src >= m->max_batch || dst < 0 || dst >= m->max_batch)
+        return lmc_set_error(LMC_ERR_INVALID, "model_fork_seq: sequence %d to %d (of %d)", src, dst, m ? m->max_batch : 0);
+    if (!m->page_size) return lmc_set_error(LMC_ERR_UNSUPPORTED, "model_fork_seq: the model's KV cache is not paged");
+    if (src == dst) return LMC_OK;
+    TRY(lmc_model_release_seq(m, dst));
+    const int np = m->seq_np[src];
+    if (!np) return LMC_OK;
+    int *from = m->h_pages + (size_t)src * m->max_pages, *to = m->h_pages + (size_t)dst * m->max_pages;
+    for (int k = 0; k < np; k++) {
+        to[k] = from[k];
+        m->page_refs[to[k]]++;
+    }
+    m->n_extra += np;
+    m->seq_np[dst] = np;
+    return pages_upload(m, dst, 0, np);
 }
 
 int lmc_model_kv_pages(const lmc_model *m, int *page_size, int *n_pages, int *n_free) {
@@ -772,6 +832,7 @@ int lmc_model_free(lmc_model *m) {
     free(m->h_pages);
     free(m->seq_np);
     free(m->free_ids);
+    free(m->page_refs);
     if (m->h_stage) cudaFreeHost(m->h_stage);
     if (m->h_next_map) cudaFreeHost(m->h_next_map);
     if (m->stream) cudaStreamDestroy(m->stream);
@@ -1219,7 +1280,7 @@ int lmc_model_forward(lmc_model *m, const int *h_tokens, const int *h_pos, int B
         int *sp = (int *)malloc(sizeof(int) * 2 * (size_t)B);
         if (!sp) return lmc_set_error(LMC_ERR_OOM, "model_forward: host");
         for (int b = 0; b < B; b++) { sp[b] = b; sp[B + b] = h_pos[b] + 1; }
-        const int rc = pages_reserve(m, B, sp, sp + B);
+        const int rc = pages_reserve(m, B, sp, h_pos, sp + B);
         free(sp);
         TRY(rc);
     }
@@ -1282,7 +1343,7 @@ int lmc_model_prefill(lmc_model *m, int seq, const int *h_tokens, int n, int sta
             return lmc_set_error(LMC_ERR_INVALID, "model_prefill: token %d outside [0, %d)", h_tokens[i], m->cfg.vocab_size);
     cudaStream_t s = m->stream;
     const int npos = start_pos + n;
-    TRY(pages_reserve(m, 1, &seq, &npos));
+    TRY(pages_reserve(m, 1, &seq, &start_pos, &npos));
     TRY(prefill_chunks(m, seq, h_tokens, n, start_pos, 1));
     TRY(lmc_keys_to_ids_launch(m->d_keys, m->d_next, 1, s));
     if (h_logits) CUTRY(cudaMemcpyAsync(h_logits, m->logits, sizeof(float) * m->vl, cudaMemcpyDeviceToHost, s));
@@ -1365,7 +1426,7 @@ static int generate(lmc_model *m, const int *h_prompt, int n_prompt, int B, int 
             return lmc_set_error(LMC_ERR_INVALID, "model_generate: token %d out of range", h_prompt[i]);
     TRY(ensure_gen_buffers(m, B, n_prompt, n_new));
     /* the loop writes positions 0 .. n_prompt + n_new - 2 of sequences 0 .. B-1 */
-    TRY(pages_reserve_all(m, B, n_prompt + n_new - 1));
+    TRY(pages_reserve_all(m, B, 0, n_prompt + n_new - 1));
     /* LMC_NO_GRAPH=1 launches the kernels directly (profilers that cannot
      * replay graph kernel nodes one by one); the kernels are the same. */
     const char *ng = getenv("LMC_NO_GRAPH");
@@ -1458,7 +1519,7 @@ int lmc_model_replay(lmc_model *m, int n, void *stream_out) {
         if (n < 0 || n > m->cfg.seq_len - m->g_pos)
             return lmc_set_error(LMC_ERR_INVALID, "model_replay: positions %d + %d exceed the context of %d", m->g_pos,
                                  n, m->cfg.seq_len);
-        TRY(pages_reserve_all(m, m->g_batch, m->g_pos + n));
+        TRY(pages_reserve_all(m, m->g_batch, m->g_pos, m->g_pos + n));
     }
     m->g_pos += n > 0 ? n : 0;
     m->smp = m->g_smp; /* the last generation's pick: greedy or its top-p draw */

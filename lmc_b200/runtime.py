@@ -57,6 +57,7 @@ SIGNATURES = {
     "lmc_model_load_ex": ([_c.c_char_p, _i, _i, _i, _i, _i, _vp, _c.POINTER(_vp)], _i),
     "lmc_model_load_paged": ([_c.c_char_p, _i, _i, _i, _i, _i, _i, _i, _vp, _c.POINTER(_vp)], _i),
     "lmc_model_release_seq": ([_vp, _i], _i),
+    "lmc_model_fork_seq": ([_vp, _i, _i], _i),
     "lmc_model_kv_pages": ([_vp, _ip, _ip, _ip], _i),
     "lmc_model_prefill": ([_vp, _i, _ip, _i, _i, _vp, _ip], _i),
     "lmc_model_shard": ([_vp, _ip, _ip, _ip, _ip], _i),
@@ -253,6 +254,11 @@ class Model:
     def release_seq(self, seq):
         """Give sequence `seq`'s KV pages back to the pool (lmc_model_release_seq)."""
         call("lmc_model_release_seq", self.h, seq)
+
+    def fork_seq(self, src, dst):
+        """Make sequence `dst` a copy of `src` that shares its KV pages
+        (lmc_model_fork_seq; paged caches)."""
+        call("lmc_model_fork_seq", self.h, src, dst)
 
     def kv_pages(self):
         """(page_size, n_pages, n_free); page_size 0 for a contiguous cache."""

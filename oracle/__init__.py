@@ -165,7 +165,8 @@ class OracleModel:
         self.arch, self.V, self.S, self.L, self.H, self.Hkv, self.D, self.F, self.Dh = (int(v) for v in c[:9])
 
     def set_kv(self, mode):
-        """Store K/V rows as a cache of mode 0 (fp32), 1 (fp16) or 2 (int8 rows)."""
+        """Store K/V rows as a cache of mode 0 (fp32), 1 (fp16), 2 (int8 rows)
+        or 3 (4-bit rows)."""
         self.lib.orc_model_set_kv(self.h, mode)
         return self
 

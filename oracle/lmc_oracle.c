@@ -101,6 +101,27 @@ void orc_kv_q8_row(const float *x, int n, int8_t *q, float *scale) {
     *scale = m / 127.0f;
 }
 
+/* One group of a 4-bit row replaced by the values it stores: m = fp16(min),
+ * d = fp16((max - m) / 15), saturated, and the code nearest to (x - m) / d,
+ * decided in double. */
+static void kv_q4_group(float *x, int n) {
+    float lo = x[0], hi = x[0];
+    for (int i = 0; i < n; i++) {
+        if (!isfinite(x[i])) {
+            for (int k = 0; k < n; k++) x[k] = NAN;
+            return;
+        }
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+    }
+    const float m = orc_f32_to_f16_to_f32(fminf(fmaxf(lo, -65504.0f), 65504.0f));
+    const float w = fmaxf(hi - m, 0.0f) / 15.0f, d = orc_f32_to_f16_to_f32(fminf(w, 65504.0f));
+    for (int i = 0; i < n; i++) {
+        const double c = d > 0.0f ? fmin(fmax(rint(((double)x[i] - (double)m) / (double)d), 0.0), 15.0) : 0.0;
+        x[i] = (float)((double)d * c + (double)m);
+    }
+}
+
 void orc_kv_round_row(float *row, int n, int mode) {
     if (mode == 1) {
         for (int i = 0; i < n; i++) row[i] = orc_f32_to_f16_to_f32(row[i]);
@@ -110,6 +131,8 @@ void orc_kv_round_row(float *row, int n, int mode) {
         if (n > 1024) return;
         orc_kv_q8_row(row, n, q, &sc);
         for (int i = 0; i < n; i++) row[i] = (float)q[i] * sc;
+    } else if (mode == 3) {
+        for (int i = 0; i < n; i += 64) kv_q4_group(row + i, n - i < 64 ? n - i : 64);
     }
 }
 

@@ -74,7 +74,9 @@ void  orc_attention(float *out, const float *q, const float *k_cache,
  * extension, restated here so the device path can be checked exactly):
  *   mode 0 fp32 (LMc), 1 fp16 (round to nearest even), 2 int8 codes with one
  *   fp32 scale per row: m = max|x|, q = clamp(rint(x * (127 / m)), +-127),
- *   scale = m / 127, value = q * scale (m = 0: all zero).
+ *   scale = m / 127, value = q * scale (m = 0: all zero), 3 4-bit codes with
+ *   fp16 d, m per group of 64: m = fp16(min), d = fp16((max - m) / 15), value =
+ *   d * code + m (NaN for a group with a value that is not finite).
  * orc_kv_q8_row quantizes one row; orc_kv_round_row replaces a row by the
  * values the cache returns for it. */
 void  orc_kv_q8_row(const float *x, int n, int8_t *q, float *scale);

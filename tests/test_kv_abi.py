@@ -112,3 +112,18 @@ def test_model_load_takes_4_bit_rows_and_refuses_unknown_ones():
     assert rc == -5 and b"cannot open" in msg
     rc, msg = status("lmc_model_load", b"/nonexistent.gguf", 1, 4, ctypes.byref(h))
     assert rc == INVALID and b"kv dtype" in msg
+
+
+def test_oracle_rounds_4_bit_rows_like_the_format(orc):
+    """The oracle's 4-bit rows (a C restatement) hold the values of the
+    format's definition in tests/kv_ref.py, special rows included."""
+    from tests.test_gpu_kv_q4 import rows_of, special_rows
+    rng = np.random.default_rng(5)
+    for Dh in (32, 64, 96, 128, 256):
+        x = np.concatenate([special_rows(Dh), rows_of(rng, (200, Dh), "outliers")])
+        want = kv_ref.q4_rows(x)[1]
+        got = orc.kv_round_rows(x, rt.KV_Q4).astype(np.float64)
+        # the oracle stores the value as fp32: half a step
+        assert (np.isnan(got) == np.isnan(want)).all()
+        ok = ~np.isnan(want)
+        assert (np.abs(got - want)[ok] <= 2.0 ** -24 * np.abs(want)[ok]).all()
