@@ -32,6 +32,8 @@
 // 16-byte boundaries) with a running softmax; parts of one item that lie in
 // one CTA are merged in shared memory, parts in several CTAs through the
 // workspace by k_q4_combine.
+#include <type_traits>
+
 #include "attention.cuh"
 #include "kv_q4.cuh"
 #include "lmc_common.cuh"
@@ -68,7 +70,7 @@ template <int NB> struct Q4 {
     static constexpr int META = T * NG * 2;               // floats: (d, m') of a tile's rows, one side
     static constexpr int FRESH = (2 * RB + 15) / 16 * 16; // the new K and V rows
     static constexpr int WARP_BYTES = Q4_STAGES * STAGE + 2 * META * 4 + FRESH;
-    static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, offset, sum)
+    static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, maximum, sum)
     static_assert(Q4_STAGES * STAGE >= 8 * SLOT * 4, "a partial result fits the ring that it is kept in");
 };
 
@@ -270,7 +272,7 @@ template <int NB> struct Q4State {
     float qsum[Q4<NB>::NG], qfac;     // head g: sum(q_j) and the factor of its products (q scaled to fp16's range)
     float2 o[2 * NB][2];              // dims x heads (see the output below)
     float2 om[Q4<NB>::NG], l;         // head g, this lane's positions (two sums each): p m', p
-    float off, mx;                    // offset and maximum of s
+    float mx;                         // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
     int vexp;                         // largest exponent field of the values' d so far
 };
 
@@ -296,7 +298,7 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
     // a power of two that brings the largest |q| into [2^12, 2^13)
-    const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+    const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
     const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
     const float scale = LOG2E / sqrtf((float)DH);
     st.qfac = scale * __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
@@ -306,10 +308,10 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
     for (int i = 0; i < NB; i++) {
         float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) s += x[i][e];
+        for (int e = 0; e < 8; e++) s = fmaf(x[i][e], up, s);
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        st.qsum[i / 2] += s * up;
+        st.qsum[i / 2] += s;
         // nibbles (0, 4) and (2, 6) of a word meet slice 2 i, (1, 5) and (3, 7), 16 times as large, slice 2 i + 1
         const float dn = up * 0.0625f;
         split2(x[i][0] * up, x[i][4] * up, st.qa[2 * i][0], st.qa[2 * i][1]);
@@ -322,7 +324,7 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
 #pragma unroll
     for (int i = 0; i < Q4<NB>::NG; i++) st.om[i] = make_float2(0.0f, 0.0f);
     st.l = make_float2(0.0f, 0.0f);
-    st.off = st.mx = -INFINITY;
+    st.mx = -INFINITY;
     st.vexp = 0;
 }
 
@@ -434,11 +436,10 @@ __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, 
     for (int h = 0; h < NH; h++) m = fmaxf(m, fmaxf(fmaxf(s[h][0].x, s[h][0].y), fmaxf(s[h][1].x, s[h][1].y)));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = fmaxf(m * st.qfac, st.mx);
+    m = fmaxf(m, st.mx);
     const int ve = max(vexp, st.vexp);
-    const float off = m - (float)(29 - ve), f = ex2(st.off - off);  // (2^-inf = 0 the first time)
+    const float up = (float)(29 - ve), f = ex2(fmaf(st.mx - m, st.qfac, (float)(st.vexp - ve)));  // (2^-inf = 0 the first time)
     st.mx = m;
-    st.off = off;
     st.vexp = ve;
     const float2 ff = make_float2(__shfl_sync(0xffffffffu, f, 8 * t), __shfl_sync(0xffffffffu, f, 8 * t + 4));
     st.l = mul2(st.l, make_float2(f, f));
@@ -446,7 +447,7 @@ __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, 
     for (int h = 0; h < NH; h++)
 #pragma unroll
         for (int par = 0; par < 2; par++) {
-            const float2 e = fma2(s[h][par], make_float2(st.qfac, st.qfac), make_float2(-off, -off));
+            const float2 e = fma2(add2(s[h][par], make_float2(-m, -m)), make_float2(st.qfac, st.qfac), make_float2(up, up));
             s[h][par] = make_float2(ex2(e.x), ex2(e.y));
             st.l = add2(st.l, s[h][par]);
         }
@@ -498,20 +499,21 @@ __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, 
 }
 
 // The item's result over its tiles so far, to dst + h * ld (heads h < heads
-// of the group of 8): with fin divided by the sum; else as it is, with the
-// offset of s and the sum behind it.  Lane (g, t) holds heads 2 t and 2 t + 1,
+// of the group of 8): with fin divided by the sum; else the sums themselves,
+// with the maximum of s and the sum of p behind them.  Lane (g, t) holds heads 2 t and 2 t + 1,
 // dims 8 g .. 8 g + 7 of each group of 64 (4 g .. 4 g + 3 of one of 32).
 template <int NB>
 __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
     const int gq = lane >> 2, t = lane & 3;
+    const float down = __uint_as_float((uint32_t)(127 - 29 + st.vexp) << 23);  // takes the probabilities' 2^(29 - vexp) back
     float l = st.l.x + st.l.y;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (!fin && t == 0 && gq < heads) {
-        dst[gq * ld + Q4<NB>::DH] = st.off;
-        dst[gq * ld + Q4<NB>::DH + 1] = l;
+        dst[gq * ld + Q4<NB>::DH] = st.mx * st.qfac;
+        dst[gq * ld + Q4<NB>::DH + 1] = l * down;
     }
-    const float inv = fin ? 1.0f / l : 1.0f;
+    const float inv = fin ? 1.0f / l : down;
 #pragma unroll
     for (int hd = 0; hd < 2; hd++) {
         const int from = 8 * t + 4 * hd, h = 2 * t + hd;
@@ -537,7 +539,262 @@ __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *d
     }
 }
 
+// ---------------------------------------------------------------------------
+// At most four query heads per kv head: the same tile with half the matrix
+// work and no idle columns.  The positions are the rows of both products, so
+// columns 2 t, 2 t + 1 of 8 can be two parts of one head t, and lane (g, t) has
+// head t's scores of rows 2 g and 2 g + 1 of each 16.
+//   scores  codes as bytes (nibbles of a word are two ANDs and a shift), q as
+//           23-bit whole numbers in three signed bytes (columns: top, middle |
+//           low, 0): integer products, exact, so codes need no centring here;
+//   output  p d as fp16 hi, lo in columns 2 t, 2 t + 1, turned to the operand's
+//           order with movmatrix.
+// On this chip a warp-level MMA keeps the integer and half pipes from issuing
+// (8 cycles each, measured in one loop with them), so their number counts: 32
+// for 32 rows of 128 dims against 64.  4 heads per kv head of 128 dims, the
+// other form against this one: one sequence of 131072 positions 56 -> 46 us
+// (3.3 TB/s), 128 ragged ones 118 -> 102 us; one head (GPT-2, 700 positions)
+// 10.5 -> 10.3 us.  Eight heads would take this form twice, at 0.8 of the
+// other's time each, so more than four heads take the other one.
+template <int NB> struct FewState {
+    uint32_t qt[NB][2], ql[NB][2];    // q as matrix operands: columns top / middle, low / 0
+    float qsum[Q4<NB>::NG], qfac;     // head t: sums of the whole numbers, the factor of their products
+    float2 o[2 * NB][2];              // dims x (hi, lo) of head t
+    float om[Q4<NB>::NG], l;          // head t, this lane's positions: sum p m', sum p
+    float mx;                         // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
+    int vexp;                         // largest exponent field of the values' d so far
+};
+
+__device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t x) {  // 8 x 8 halves of the warp, transposed
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 template <int NB>
+__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, FewState<NB> &st) {
+    const AttnArgs &a = g.a;
+    constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
+    // lane (n, t) makes column n's operand: head n / 2, n odd: the middle byte (and 0), even: the top (and low) one
+    const int G = a.H / a.Hkv, head = lane >> 3, t = lane & 3;
+    const bool odd = lane & 4;
+    float x[NB][8], big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+        if (head < G) {
+            load8(a.q + (size_t)p.b * a.ldq + ((size_t)p.kh * G + head) * DH + 32 * i + 8 * t, g.vec, x[i]);
+            rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[i][e]));
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // a power of two that brings the head's largest |q| into [2^21, 2^22): three signed bytes hold it
+    const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
+    const float up = __uint_as_float((uint32_t)(127 + 21 - ex) << 23);
+    float sum[NG];
+#pragma unroll
+    for (int j = 0; j < NG; j++) sum[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {  // dims 0, 2, 4, 6 of the word: its low nibbles; 1, 3, 5, 7: its high ones
+            const float y = rintf(x[i][e] * up);
+            s += y;  // (a value that is not finite makes the sum, and with it the score, NaN or infinite)
+            const uint32_t b = (uint32_t)__float2int_rn(y) + 0x808080u;  // the bytes, each 128 more
+            hi[e & 1] |= ((odd ? b >> 8 : b >> 16) & 0xffu) << (8 * (e >> 1));
+            lo[e & 1] |= (b & 0xffu) << (8 * (e >> 1));
+        }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        sum[i / 2] += s;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            st.qt[i][k] = hi[k] ^ 0x80808080u;
+            st.ql[i][k] = odd ? 0u : lo[k] ^ 0x80808080u;
+        }
+    }
+    // lane (g, t) goes on with head t, held by the lanes (2 t, ...)
+    st.qfac = __shfl_sync(0xffffffffu, LOG2E / sqrtf((float)DH) * __uint_as_float((uint32_t)(127 - 21 + ex) << 23), 8 * t);
+#pragma unroll
+    for (int j = 0; j < NG; j++) st.qsum[j] = __shfl_sync(0xffffffffu, sum[j], 8 * t);
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < NG; j++) st.om[j] = 0.0f;
+    st.l = 0.0f;
+    st.mx = -INFINITY;
+    st.vexp = 0;
+}
+
+// The (d, m) words of row r.
+template <int NB> __device__ __forceinline__ void row_factors(const uint8_t *rows, int r, uint32_t (&w)[Q4<NB>::NG]) {
+    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, DH = Q4<NB>::DH;
+    const uint8_t *at = rows + r * RB + DH / 2;
+    if constexpr (NG % 2 == 0 && RB % 8 == 0) {
+#pragma unroll
+        for (int j = 0; j < NG; j += 2) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(at + 4 * j);
+            w[j] = v.x;
+            w[j + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NG; j++) w[j] = *reinterpret_cast<const uint32_t *>(at + 4 * j);
+    }
+}
+
+template <int NB>
+__device__ __forceinline__ void attend_tile(FewState<NB> &st, const uint8_t *kt, const uint8_t *vt, float *, float *, int n, int lane) {
+    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, T = Q4<NB>::T, NH = T / 16;
+    const int gq = lane >> 2, t = lane & 3;
+    float s[NH][2];  // scores over qfac of rows 16 h + 2 g, + 1
+#pragma unroll
+    for (int h = 0; h < NH; h++) {
+        const uint32_t *const k0 = reinterpret_cast<const uint32_t *>(kt + (16 * h + 2 * gq) * RB) + t, *const k1 = k0 + RB / 4;
+        uint32_t f0[NG], f1[NG];
+        row_factors<NB>(kt, 16 * h + 2 * gq, f0);
+        row_factors<NB>(kt, 16 * h + 2 * gq + 1, f1);
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            int ct[4] = {0, 0, 0, 0}, cl[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
+                const uint32_t w0 = k0[4 * i], w1 = k1[4 * i];
+                const uint32_t a0 = w0 & 0x0f0f0f0fu, a1 = w1 & 0x0f0f0f0fu, a2 = w0 >> 4 & 0x0f0f0f0fu, a3 = w1 >> 4 & 0x0f0f0f0fu;
+                imma(ct, a0, a1, a2, a3, st.qt[i][0], st.qt[i][1]);
+                imma(cl, a0, a1, a2, a3, st.ql[i][0], st.ql[i][1]);
+            }
+            // 2^16 top + 2^8 middle + low: the first two together are below 2^24, exact in fp32
+            const float x0 = fmaf((float)(ct[0] * 256 + ct[1]), 256.0f, (float)cl[0]);
+            const float x1 = fmaf((float)(ct[2] * 256 + ct[3]), 256.0f, (float)cl[2]);
+            const float2 d0 = __half22float2(*reinterpret_cast<const __half2 *>(&f0[j])), d1 = __half22float2(*reinterpret_cast<const __half2 *>(&f1[j]));
+            s[h][0] = fmaf(d0.y, st.qsum[j], j ? fmaf(d0.x, x0, s[h][0]) : d0.x * x0);
+            s[h][1] = fmaf(d1.y, st.qsum[j], j ? fmaf(d1.x, x1, s[h][1]) : d1.x * x1);
+        }
+    }
+    uint32_t vf[NH][2][NG];  // (d, m) words of the values' rows
+    uint32_t dmax = 0;
+#pragma unroll
+    for (int h = 0; h < NH; h++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            row_factors<NB>(vt, 16 * h + 2 * gq + r, vf[h][r]);
+            if (16 * h + 2 * gq + r >= n) {  // past the end
+                s[h][r] = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NG; j++) vf[h][r][j] = 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < NG; j++) dmax = max(dmax, vf[h][r][j] & 0xffffu);
+        }
+    const int ve = max(min((int)(__reduce_max_sync(0xffffffffu, dmax) >> 10), 30), st.vexp);
+    float m = fmaxf(s[0][0], s[0][1]);
+#pragma unroll
+    for (int h = 1; h < NH; h++) m = fmaxf(m, fmaxf(s[h][0], s[h][1]));
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = fmaxf(m, st.mx);
+    const float up = (float)(29 - ve), f = ex2(fmaf(st.mx - m, st.qfac, (float)(st.vexp - ve)));  // (2^-inf = 0 the first time)
+    const float2 ff = make_float2(f, f);
+    st.mx = m;
+    st.vexp = ve;
+    st.l *= f;
+#pragma unroll
+    for (int h = 0; h < NH; h++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            s[h][r] = ex2(fmaf(s[h][r] - m, st.qfac, up));
+            st.l += s[h][r];
+        }
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        uint32_t b[NH][2];  // p d of the 16 rows of each set
+        st.om[j] *= f;
+#pragma unroll
+        for (int h = 0; h < NH; h++) {
+            const float2 d0 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][0][j])), d1 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][1][j]));
+            const float w0 = s[h][0] * d0.x, w1 = s[h][1] * d1.x;
+            st.om[j] = fmaf(s[h][0], fmaf(8.0f, d0.x, d0.y), fmaf(s[h][1], fmaf(8.0f, d1.x, d1.y), st.om[j]));
+            uint32_t hi, lo;
+            split2(w0, w1, hi, lo);
+            b[h][0] = turned(__byte_perm(hi, lo, 0x5410));  // row 2 g: (hi, lo)
+            b[h][1] = turned(__byte_perm(hi, lo, 0x7632));  // row 2 g + 1
+        }
+        // this lane's dims: word g of the group, or half a word of a group of 32
+        const bool half = NB % 2 && j == NG - 1;
+        const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
+#pragma unroll
+        for (int k = 0; k < (half ? 1 : 2); k++) {  // nibbles 0-3, 4-7 of the words (or the half word's four)
+            const uint32_t sel = half ? ((gq & 1) ? 0x7632u : 0x5410u) : (k ? 0x7632u : 0x5410u);
+            const int i = 4 * j + 2 * k;
+            float c[2][4];
+#pragma unroll
+            for (int h = 0; h < NH; h++) {
+                uint32_t cw[4], x[4], y[4];  // rows 4 t + (0, 2) and (1, 3)
+#pragma unroll
+                for (int r = 0; r < 4; r++) cw[r] = *reinterpret_cast<const uint32_t *>(vr + (16 * h + r) * RB);
+                codes8(__byte_perm(cw[0], cw[2], sel), x);
+                codes8(__byte_perm(cw[1], cw[3], sel), y);
+                if (h) {
+                    hmma(c[0], x[0], x[1], y[0], y[1], b[h][0], b[h][1]);
+                    hmma(c[1], x[2], x[3], y[2], y[3], b[h][0], b[h][1]);
+                } else {
+                    hmma0(c[0], x[0], x[1], y[0], y[1], b[h][0], b[h][1]);
+                    hmma0(c[1], x[2], x[3], y[2], y[3], b[h][0], b[h][1]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                st.o[i + e][0] = fma2(st.o[i + e][0], ff, make_float2(c[e][0], c[e][1]));
+                st.o[i + e][1] = fma2(st.o[i + e][1], ff, make_float2(c[e][2], c[e][3]));
+            }
+        }
+    }
+}
+
+template <int NB>
+__device__ __forceinline__ void result(const FewState<NB> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
+    const int gq = lane >> 2, t = lane & 3;
+    const float down = __uint_as_float((uint32_t)(127 - 29 + st.vexp) << 23);  // takes the probabilities' 2^(29 - vexp) back
+    float l = st.l;
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (!fin && gq == 0 && t < heads) {
+        dst[t * ld + Q4<NB>::DH] = st.mx * st.qfac;
+        dst[t * ld + Q4<NB>::DH + 1] = l * down;
+    }
+    const float iv = fin ? 1.0f / l : down;
+#pragma unroll
+    for (int j = 0; j < Q4<NB>::NG; j++) {
+        float m = st.om[j];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+        const bool half = NB % 2 && j == Q4<NB>::NG - 1;
+#pragma unroll
+        for (int k = 0; k < (half ? 1 : 2); k++) {
+            const float2 *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
+            const float4 v = make_float4((a[0].x + a[0].y + m) * iv, fmaf(a[1].x + a[1].y, 0.0625f, m) * iv, (b[0].x + b[0].y + m) * iv,
+                                         fmaf(b[1].x + b[1].y, 0.0625f, m) * iv);
+            float *o = dst + t * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
+            if (t >= heads) continue;
+            if (vec) *reinterpret_cast<float4 *>(o) = v;
+            else { o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w; }
+        }
+    }
+}
+
+template <int NB, bool FEW>
 __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_constant__ Q4Args g) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Item sh_item[Q4_WARPS][2];  // of the copies, of the computation
@@ -652,7 +909,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         int tile = p.tile, end = p.end, nt = p.nt, phase = 0, part = 0, stage = 0, fill = 0;
         uint32_t parity = 0, flying = 0;  // phase bits of the stages' barriers; stages whose copies are not waited for
         bool begin = true;
-        Q4State<NB> st;
+        std::conditional_t<FEW, FewState<NB>, Q4State<NB>> st;
 #pragma unroll 1
         for (int skip = Q4_STAGES - 1; tile < end; skip--) {  // the first turns only start copies
             if (a_tile < a_end) {
@@ -850,12 +1107,12 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
     }
 }
 
-template <int NB> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
+template <int NB, bool FEW> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
     const int GH = g.a.H / g.a.Hkv < 8 ? g.a.H / g.a.Hkv : 8;
     const size_t smem = (size_t)Q4_WARPS * Q4<NB>::WARP_BYTES + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
-    LMC_CUDA_TRY(cudaFuncSetAttribute(k_attn_q4<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    LMC_CUDA_TRY(cudaFuncSetAttribute((k_attn_q4<NB, FEW>), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int most = lmc_sm_count() * (smem + 2048 <= 114 * 1024 ? 2 : 1), want = max_units / g.rmin;
-    LMC_LAUNCH("attention (4-bit rows)", k_attn_q4<NB>, want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);
+    LMC_LAUNCH("attention (4-bit rows)", (k_attn_q4<NB, FEW>), want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);
     return LMC_OK;
 }
 
@@ -884,8 +1141,10 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     g.run = a.pages && (1 << a.page_shift) < T ? 1 << a.page_shift : T;
     const long long units = (long long)batch * a.Hkv * g.HG * (g.items_only ? 1 : NT + Q4_ITEM);
     if (units > 0x7fffffffLL) return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: batch %d x context %d is too large", batch, a.S);
-    int (*const fn[8])(const Q4Args &, int, cudaStream_t) = {launch<1>, launch<2>, launch<3>, launch<4>, launch<5>, launch<6>, launch<7>, launch<8>};
-    const int rc = fn[a.Dh / 32 - 1](g, (int)units, s);
+    int (*const fn[8][2])(const Q4Args &, int, cudaStream_t) = {
+        {launch<1, false>, launch<1, true>}, {launch<2, false>, launch<2, true>}, {launch<3, false>, launch<3, true>}, {launch<4, false>, launch<4, true>},
+        {launch<5, false>, launch<5, true>}, {launch<6, false>, launch<6, true>}, {launch<7, false>, launch<7, true>}, {launch<8, false>, launch<8, true>}};
+    const int rc = fn[a.Dh / 32 - 1][G <= 4](g, (int)units, s);
     if (rc != LMC_OK || a.nsplit == 1) return rc;
     const size_t heads = (size_t)batch * a.H;
     if (heads <= 1024) LMC_LAUNCH("attention combine (4-bit rows)", k_q4_combine<4>, heads, 128, 0, s, a, batch);

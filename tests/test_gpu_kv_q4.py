@@ -289,6 +289,52 @@ def test_attention_group_sizes(cuda, G, Dh, P):
     attend(cuda, G, [130, 64], 3 if G < 16 else 1, G, Dh, 160, P)
 
 
+@pytest.mark.parametrize("Dh", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("G,P", [(6, 0), (5, 32), (12, 16)])
+def test_attention_head_sizes_of_large_groups(cuda, Dh, G, P):
+    """More than four query heads per kv head take another form of the kernel."""
+    attend(cuda, Dh + G, [150, 63, 0], 2, G, Dh, 160, P)
+
+
+@pytest.mark.parametrize("G", [1, 3, 4, 5, 8])
+def test_attention_largest_queries(cuda, G):
+    """Queries near the end of fp32: one position takes all the weight (its
+    lead is far over the scores' rounding), so the output is its values."""
+    rng = np.random.default_rng(40 + G)
+    Dh, n = 64, 70
+    c = Cache(cuda, rng, [n], 1, Dh, 128, 0, "normal")
+    q = (rows_of(rng, (1, G * Dh)) * np.float32(3e37)).astype(np.float32)
+    kn, vn = rows_of(rng, (1, Dh)), rows_of(rng, (1, Dh))
+    out = cuda.full((1, G * Dh), 5.0, device="cuda")
+    c.decode(cuda, out, *(dev(cuda, a) for a in (q, kn, vn, np.array([n], np.int32))), G)
+    k = np.concatenate([c.k[0], kv_ref.q4_rows(kn.reshape(1, 1, Dh))[1]], 1)
+    v = np.concatenate([c.v[0], kv_ref.q4_rows(vn.reshape(1, 1, Dh))[1]], 1)
+    s = np.sort(q.reshape(G, Dh).astype(np.float64) @ k[0].T / 8)
+    assert np.isfinite(q).all() and (s[:, -1] - s[:, -2] > 64 + 2.0 ** -19 * np.abs(s).max(-1)).all()
+    want, _ = kv_ref.attention(q.reshape(G, Dh), k, v)
+    assert np.abs(out.cpu().numpy().reshape(G, Dh) - want).max() <= 2.0 ** -20 * np.abs(v).max()
+
+
+@pytest.mark.parametrize("G", [3, 4, 6, 9])
+def test_attention_queries_that_are_not_finite(cuda, G):
+    """An infinity or a NaN in a query makes its own head NaN and no other."""
+    rng = np.random.default_rng(50 + G)
+    Dh, n = 128, 90
+    c = Cache(cuda, rng, [n], 2, Dh, 128, 0, "normal")
+    q = rows_of(rng, (1, 2 * G * Dh))
+    q[0, 1 * Dh + 5], q[0, (G + 2) * Dh + 77] = np.inf, np.nan
+    kn, vn = rows_of(rng, (1, 2 * Dh)), rows_of(rng, (1, 2 * Dh))
+    out = cuda.full((1, 2 * G * Dh), 5.0, device="cuda")
+    c.decode(cuda, out, *(dev(cuda, a) for a in (q, kn, vn, np.array([n], np.int32))), G)
+    got = out.cpu().numpy().reshape(2 * G, Dh)
+    bad = np.zeros(2 * G, bool)
+    bad[[1, G + 2]] = True
+    assert np.isnan(got[bad]).all()
+    k, v = (np.concatenate([x[0], kv_ref.q4_rows(y.reshape(2, 1, Dh))[1]], 1) for x, y in ((c.k, kn), (c.v, vn)))
+    want, _ = kv_ref.attention(np.where(bad[:, None], 0, q.reshape(2 * G, Dh)), k, v)
+    assert rel_err(got[~bad], want[~bad]) < 1e-5
+
+
 @pytest.mark.parametrize("pos", list(range(0, 70)) + [127, 128, 129, 255, 256, 257, 511, 512, 1023])
 def test_attention_every_length(cuda, pos):
     """Each length up to two tiles and the borders of longer ones."""
