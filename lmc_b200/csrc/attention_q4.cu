@@ -54,7 +54,7 @@ constexpr int q4_tile(int NB) { return NB <= 4 ? 64 : 32; }  // positions per ti
 
 struct Q4Args {
     AttnArgs a;
-    int HG;         // groups of 8 query heads per kv head
+    int G, HG;      // query heads per kv head, groups of 8 of them
     int rmin;       // tiles per CTA at least (workspace slots per head: a.nsplit)
     int items_only; // 1: an item is never divided (a.nsplit is 1)
     int batch, vec; // vec: q, new rows and out can be moved 16 bytes at a time
@@ -176,6 +176,9 @@ struct Item {
     long long off;   // contiguous: byte offset of the item's row 0 in a cache
     const int *row;  // paged: the sequence's table row
 };
+struct Part {  // of an item, left in shared memory by a warp: its first unit, sequence, heads, tiles [first, end) of nt
+    int unit, b, head, heads, first, end, nt;
+};
 __device__ __forceinline__ int seq_pos(const Q4Args &g, int b) {  // position, or -1 when the row has nothing to do
     const int p = __ldg(g.a.pos + b);
     return p < 0 || p >= g.a.S ? -1 : p;
@@ -183,7 +186,7 @@ __device__ __forceinline__ int seq_pos(const Q4Args &g, int b) {  // position, o
 __device__ __forceinline__ int item_units(const Q4Args &g, int nt) { return g.items_only ? 1 : nt + Q4_ITEM; }
 // The item at (p.b, p.j), p.nt and p.pos known; its tiles up to the share's end.
 template <int NB> __device__ __forceinline__ void set_item(const Q4Args &g, Item &p) {
-    p.kh = p.j / g.HG;
+    p.kh = g.HG == 1 ? p.j : p.j / g.HG;
     p.end = g.items_only ? (p.left > 0 ? p.nt : 0) : min(p.nt, p.left - Q4_ITEM);
     const long long cs = g.a.seq ? __ldg(g.a.seq + p.b) : p.b;
     p.row = g.a.pages + cs * g.a.max_pages;
@@ -276,22 +279,28 @@ template <int NB> struct Q4State {
     int vexp;                         // largest exponent field of the values' d so far
 };
 
+// This lane's values of query `head` of the item's kv head (0 for heads past the last one).
+template <int NB> __device__ __forceinline__ void fetch_q(const Q4Args &g, const Item &p, int lane, int head, float (&x)[NB][8]) {
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+        if (head < g.G) load8(g.a.q + (size_t)p.b * g.a.ldq + ((size_t)p.kh * g.G + head) * Q4<NB>::DH + 32 * i + 8 * (lane & 3), g.vec, x[i]);
+    }
+}
+template <int NB> __device__ __forceinline__ int q_head(const Q4Args &g, const Item &p, int lane, const Q4State<NB> &) {
+    return (p.j - p.kh * g.HG) * 8 + (lane >> 2);
+}
+
 template <int NB>
-__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, Q4State<NB> &st) {
+__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], Q4State<NB> &st) {
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH;
-    const int G = a.H / a.Hkv, head = (p.j - p.kh * g.HG) * 8 + (lane >> 2), t = lane & 3;
-    float x[NB][8];
+    const int t = lane & 3;
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-        if (head < G) {
-            load8(a.q + (size_t)p.b * a.ldq + ((size_t)p.kh * G + head) * DH + 32 * i + 8 * t, g.vec, x[i]);
-            rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-        }
+        rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
 #pragma unroll
         for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[i][e]));
     }
@@ -333,32 +342,29 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
 template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const Item &p, uint32_t *fresh, int lane) {
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH, NW = DH / 8, RB = Q4<NB>::RB;
-    float x[2][8];
-#pragma unroll
-    for (int side = 0; side < 2; side++) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[side][e] = 0.0f;
-        if (lane < NW) load8((side ? a.v_new : a.k_new) + (size_t)p.b * a.ldkv + (size_t)p.kh * DH + 8 * lane, g.vec, x[side]);
-    }
-    if (lane < NW) rope8(a, p.pos, DH, 8 * lane, x[0]);
+    constexpr int SIDES = NW <= 16 ? 2 : 1;  // K in lanes 0-15, V in lanes 16-31 when they fit
     bool ok = true;
     const long long off = row_offset<NB>(g, p, p.pos, &ok);
     ok &= p.j == p.kh * g.HG;
 #pragma unroll 1
-    for (int side = 0; side < 2; side++) {
+    for (int side0 = 0; side0 < 2; side0 += SIDES) {
+        const int side = SIDES == 2 ? lane >> 4 : side0, w = SIDES == 2 ? lane & 15 : lane;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (w < NW) {
+            load8((side ? a.v_new : a.k_new) + (size_t)p.b * a.ldkv + (size_t)p.kh * DH + 8 * w, g.vec, x);
+            if (!side) rope8(a, p.pos, DH, 8 * w, x);
+        }
         uint32_t codes, dm;
-        kv_q4_quantize<32>(x[0], lane < NW, codes, dm);
+        kv_q4_quantize<32 / SIDES>(x, w < NW, codes, dm);
         uint32_t *dst = reinterpret_cast<uint32_t *>((uint8_t *)(side ? a.v_cache : a.k_cache) + off);
-        if (lane < NW) {
-            fresh[side * (RB / 4) + lane] = codes;
-            if (ok) dst[lane] = codes;
-            if (lane % 8 == 0) {
-                fresh[side * (RB / 4) + NW + lane / 8] = dm;
-                if (ok) dst[NW + lane / 8] = dm;
+        if (w < NW) {
+            fresh[side * (RB / 4) + w] = codes;
+            if (ok) dst[w] = codes;
+            if (w % 8 == 0) {
+                fresh[side * (RB / 4) + NW + w / 8] = dm;
+                if (ok) dst[NW + w / 8] = dm;
             }
         }
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[0][e] = x[1][e];
     }
 }
 
@@ -576,22 +582,18 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {  // 8 x 8 halves of the
     return y;
 }
 
+// Lane (n, t) makes column n's operand: head n / 2, n odd: the middle byte (and 0), even: the top (and low) one.
+template <int NB> __device__ __forceinline__ int q_head(const Q4Args &, const Item &, int lane, const FewState<NB> &) { return lane >> 3; }
 template <int NB>
-__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, FewState<NB> &st) {
+__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], FewState<NB> &st) {
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
-    // lane (n, t) makes column n's operand: head n / 2, n odd: the middle byte (and 0), even: the top (and low) one
-    const int G = a.H / a.Hkv, head = lane >> 3, t = lane & 3;
+    const int t = lane & 3;
     const bool odd = lane & 4;
-    float x[NB][8], big = 0.0f;
+    float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-        if (head < G) {
-            load8(a.q + (size_t)p.b * a.ldq + ((size_t)p.kh * G + head) * DH + 32 * i + 8 * t, g.vec, x[i]);
-            rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
-        }
+        rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
 #pragma unroll
         for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[i][e]));
     }
@@ -799,11 +801,12 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Item sh_item[Q4_WARPS][2];  // of the copies, of the computation
     __shared__ __align__(8) uint64_t sh_bar[Q4_WARPS][Q4_STAGES];
-    __shared__ int sh_total[Q4_WARPS], desc[Q4_WARPS][2][5];  // a warp's parts: first unit of the item, b, j, first tile, end
+    __shared__ int sh_total[Q4_WARPS];
+    __shared__ Part desc[Q4_WARPS][2];
     constexpr int DH = Q4<NB>::DH, SLOT = Q4<NB>::SLOT, RB = Q4<NB>::RB, T = Q4<NB>::T;
     const AttnArgs &a = g.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int G = a.H / a.Hkv, items = a.Hkv * g.HG, GH = min(G, 8);
+    const int G = g.G, items = a.Hkv * g.HG, GH = min(G, 8);
     pdl_wait();
     pdl_launch_dependents();
     // units (tiles) of the whole batch, and this CTA's and this warp's share
@@ -811,22 +814,43 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         const int p = seq_pos(g, b);
         return p < 0 ? 0 : item_units(g, p / T + 1) * items;
     };
-    int sum = 0;
-    for (int b = threadIdx.x; b < g.batch; b += 32 * Q4_WARPS) sum += units_of(b);
-    sum = __reduce_add_sync(0xffffffffu, sum);
+    // up to 32 sequences: each warp sums them by itself
+    auto scan = [&](int mine) {  // inclusive sum over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, mine, o);
+            if (lane >= o) mine += y;
+        }
+        return mine;
+    };
+    const bool small = g.batch <= 32;
+    int mine = 0, inc = 0, total;
     if (lane == 0) {
-        sh_total[warp] = sum;
-        desc[warp][0][0] = desc[warp][1][0] = -1;
+        desc[warp][0].unit = desc[warp][1].unit = -1;
         for (int i = 0; i < Q4_STAGES; i++)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&sh_bar[warp][i])));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
-    const int total = sh_total[0] + sh_total[1] + sh_total[2] + sh_total[3];
+    if (small) {
+        mine = lane < g.batch ? units_of(lane) : 0;
+        inc = scan(mine);
+        total = __shfl_sync(0xffffffffu, inc, 31);
+        __syncwarp();
+    } else {
+        int sum = 0;
+        for (int b = threadIdx.x; b < g.batch; b += 32 * Q4_WARPS) sum += units_of(b);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) sh_total[warp] = sum;
+        __syncthreads();
+        total = sh_total[0] + sh_total[1] + sh_total[2] + sh_total[3];
+    }
     const int nC = min((int)gridDim.x, max(1, total / g.rmin));
     if ((int)blockIdx.x >= nC || total == 0) return;
-    const int c0 = (int)((long long)blockIdx.x * total / nC), c1 = (int)((long long)(blockIdx.x + 1) * total / nC);
-    const int u0 = c0 + (int)((long long)(c1 - c0) * warp / Q4_WARPS), u1 = c0 + (int)((long long)(c1 - c0) * (warp + 1) / Q4_WARPS);
+    // CTA i has per or (the first `more`) per + 1 units, a warp the like of them
+    const int per = total / nC, more = total - per * nC;
+    auto cta_of = [&](int unit) { return unit < more * (per + 1) ? unit / (per + 1) : more + (unit - more * (per + 1)) / per; };
+    const int cta = blockIdx.x, c0 = cta * per + min(cta, more), cn = per + (cta < more);
+    const int wn = cn / Q4_WARPS, wm = cn % Q4_WARPS, u0 = c0 + warp * wn + min(warp, wm), u1 = u0 + wn + (warp < wm);
     uint8_t *const ring = smem + warp * Q4<NB>::WARP_BYTES;
     float *const kdm = reinterpret_cast<float *>(ring + Q4_STAGES * Q4<NB>::STAGE), *const vdm = kdm + Q4<NB>::META;
     uint32_t *const fresh = reinterpret_cast<uint32_t *>(vdm + Q4<NB>::META);
@@ -839,12 +863,9 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         p.b = 0;
         int before = 0;
         for (int b0 = 0; b0 < g.batch; b0 += 32) {
-            const int mine = b0 + lane < g.batch ? units_of(b0 + lane) : 0;
-            int inc = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
+            if (!small) {
+                mine = b0 + lane < g.batch ? units_of(b0 + lane) : 0;
+                inc = scan(mine);
             }
             const unsigned hit = __ballot_sync(0xffffffffu, before + inc > u0);
             if (hit) {
@@ -856,11 +877,12 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             before += __shfl_sync(0xffffffffu, inc, 31);
         }
         set_seq<NB>(g, p);
-        const int at = u0 - before, per = item_units(g, p.nt);
-        p.j = at / per;
-        p.unit = u0 - at % per;
+        const int at = u0 - before, units = item_units(g, p.nt);
+        p.j = at / units;
+        const int within = at - p.j * units;
+        p.unit = u0 - within;
         p.left = u1 - p.unit;
-        p.tile = g.items_only ? 0 : max(0, at % per - Q4_ITEM);
+        p.tile = g.items_only ? 0 : max(0, within - Q4_ITEM);
         set_item<NB>(g, p);
         Item *const ia = &sh_item[warp][0], *const ii = &sh_item[warp][1];
         *ia = p;
@@ -927,8 +949,10 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             if (skip > 0) continue;
             if (begin) {
                 phase = g.bulk ? 0 : (int)(ii->off & 15);  // rows lie in the ring at the phase that they have in the cache
-                if (a.append && end == nt) append<NB>(g, *ii, fresh, lane);
-                load_q<NB>(g, *ii, lane, st);
+                float x[NB][8];
+                fetch_q<NB>(g, *ii, lane, q_head<NB>(g, *ii, lane, st), x);
+                if (a.append && end == nt) append<NB>(g, *ii, fresh, lane);  // (while q is on its way)
+                load_q<NB>(g, *ii, lane, x, st);
                 begin = false;
             }
             if (!g.bulk) {
@@ -958,22 +982,16 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             attend_tile<NB>(st, kt, kt + Q4<NB>::SIDE, kdm, vdm, n, lane);
             __syncwarp();  // the stage and (d, m') are read; they may be written again
             if (++tile == end) {  // the item, or this warp's part of it, ends
-                const int b = ii->b, j = ii->j, kh = ii->kh, first = ii->tile;
-                const int h0 = (j - kh * g.HG) * 8, heads = min(8, G - h0);
-                const size_t head = (size_t)kh * G + h0;
+                const int b = ii->b, kh = ii->kh, first = ii->tile;
+                const int h0 = (ii->j - kh * g.HG) * 8, heads = min(8, G - h0), head = kh * G + h0;
                 const bool whole = first == 0 && end == nt;
                 float *slot = part ? reinterpret_cast<float *>(ring) : slots + warp * GH * SLOT;
-                result<NB>(st, lane, whole ? a.out + (size_t)b * a.ldo + head * DH : slot, whole ? DH : SLOT, heads, whole, !whole || g.vec);
+                result<NB>(st, lane, whole ? a.out + (size_t)b * a.ldo + (size_t)head * DH : slot, whole ? DH : SLOT, heads, whole, !whole || g.vec);
                 if (whole) {
                     if (lane < heads && a.nsplit > 1)  // nothing for the combine kernel to do
                         a.ws[((size_t)b * a.H + head + lane) * hstride + DH + 1] = 0.0f;
                 } else if (lane == 0) {
-                    int *d = desc[warp][part];
-                    d[0] = ii->unit;
-                    d[1] = b;
-                    d[2] = j;
-                    d[3] = first;
-                    d[4] = end;
+                    desc[warp][part] = Part{ii->unit, b, head, heads, first, end, nt};
                 }
                 part = 1;
                 next_item<NB>(g, ii);
@@ -989,52 +1007,62 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
     }
     __syncthreads();
     // merge this CTA's parts of each item: neighbours in (warp, part) order
-    const int nw = Q4_WARPS;
-    int k = 0;
-    while (k < 2 * nw) {
-        const int *d = desc[k / 2][k % 2];
-        if (d[0] < 0) { k++; continue; }
-        int e = k;  // last part of the same item
-        for (int i = k + 1; i < 2 * nw; i++) {
-            if (desc[i / 2][i % 2][0] < 0) continue;
-            if (desc[i / 2][i % 2][0] != d[0]) break;
-            e = i;
-        }
-        const int b = d[1], j = d[2], h0 = (j % g.HG) * 8, heads = min(8, G - h0), kh = j / g.HG;
-        const int pos = seq_pos(g, b), nt = pos / T + 1;
-        const bool whole = d[3] == 0 && desc[e / 2][e % 2][4] == nt;
-        // the CTAs that hold the item's first and last tile
-        const int ca = (int)(((long long)(d[0] + Q4_ITEM + 1) * nC - 1) / total), cb = (int)(((long long)(d[0] + Q4_ITEM + nt) * nC - 1) / total);
-        for (int i = threadIdx.x; i < heads * DH; i += 32 * Q4_WARPS) {
-            const int h = i / DH, x = i % DH;
-            float M = -INFINITY, L = 0.0f, acc = 0.0f;
-            for (int q = k; q <= e; q++) {
-                if (desc[q / 2][q % 2][0] < 0) continue;
+    constexpr int PARTS = 2 * Q4_WARPS;
+    const int id = lane < PARTS ? desc[lane >> 1][lane & 1].unit : -1;
+    unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
+    while (todo) {
+        const int k = __ffs(todo) - 1, unit = __shfl_sync(0xffffffffu, id, k);
+        const unsigned parts = __ballot_sync(0xffffffffu, id == unit);
+        todo &= ~parts;
+        const int e = 31 - __clz(parts);
+        const Part d = desc[k >> 1][k & 1];
+        const bool whole = d.first == 0 && desc[e >> 1][e & 1].end == d.nt;
+        // the slot is this CTA's place among those that hold the item's tiles
+        const int slot = whole ? 0 : cta - cta_of(unit + Q4_ITEM);
+        const bool last = !whole && cta_of(unit + Q4_ITEM + d.nt - 1) == cta;
+        for (int i = threadIdx.x; i < d.heads * (DH / 4); i += 32 * Q4_WARPS) {
+            const int h = i / (DH / 4), x = 4 * (i % (DH / 4));
+            float M = -INFINITY, L = 0.0f, m[PARTS], l[PARTS];
+            float4 v[PARTS], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < PARTS; q++) {
                 const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::WARP_BYTES) : slots + (q / 2) * GH * SLOT) + h * SLOT;
-                M = fmaxf(M, s[DH]);
+                m[q] = -INFINITY;
+                if (parts >> q & 1) {
+                    m[q] = s[DH];
+                    l[q] = s[DH + 1];
+                    v[q] = *reinterpret_cast<const float4 *>(s + x);
+                }
+                M = fmaxf(M, m[q]);
             }
-            for (int q = k; q <= e; q++) {
-                if (desc[q / 2][q % 2][0] < 0) continue;
-                const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::WARP_BYTES) : slots + (q / 2) * GH * SLOT) + h * SLOT;
-                const float f = ex2(s[DH] - M);
-                L = fmaf(s[DH + 1], f, L);
-                acc = fmaf(s[x], f, acc);
-            }
-            const size_t head = (size_t)kh * G + h0 + h;
+#pragma unroll
+            for (int q = 0; q < PARTS; q++)
+                if (parts >> q & 1) {
+                    const float f = ex2(m[q] - M);
+                    L = fmaf(l[q], f, L);
+                    acc.x = fmaf(v[q].x, f, acc.x);
+                    acc.y = fmaf(v[q].y, f, acc.y);
+                    acc.z = fmaf(v[q].z, f, acc.z);
+                    acc.w = fmaf(v[q].w, f, acc.w);
+                }
+            float *w = a.ws + ((size_t)d.b * a.H + d.head + h) * hstride;
             if (whole) {
-                a.out[(size_t)b * a.ldo + head * DH + x] = acc / L;
-                if (x == 0 && a.nsplit > 1) a.ws[((size_t)b * a.H + head) * hstride + DH + 1] = 0.0f;
+                const float iv = 1.0f / L;
+                acc = make_float4(acc.x * iv, acc.y * iv, acc.z * iv, acc.w * iv);
+                float *o = a.out + (size_t)d.b * a.ldo + (size_t)(d.head + h) * DH + x;
+                if (g.vec) *reinterpret_cast<float4 *>(o) = acc;
+                else { o[0] = acc.x; o[1] = acc.y; o[2] = acc.z; o[3] = acc.w; }
+                if (x == 0 && a.nsplit > 1) w[DH + 1] = 0.0f;
             } else {
-                float *w = a.ws + ((size_t)b * a.H + head) * hstride + (size_t)((int)blockIdx.x - ca) * (DH + 2);
-                w[x] = acc;
+                w += (size_t)slot * (DH + 2);
+                w[x] = acc.x; w[x + 1] = acc.y; w[x + 2] = acc.z; w[x + 3] = acc.w;
                 if (x == 0) {
                     w[DH] = M;
                     // the sum; its sign bit marks the item's last part
-                    w[DH + 1] = __uint_as_float((__float_as_uint(L) & 0x7fffffffu) | ((int)blockIdx.x == cb ? 0x80000000u : 0u));
+                    w[DH + 1] = __uint_as_float((__float_as_uint(L) & 0x7fffffffu) | (last ? 0x80000000u : 0u));
                 }
             }
         }
-        k = e + 1;
     }
 }
 
@@ -1129,6 +1157,7 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     if ((size_t)a.nsplit * slot > ws_bytes) a.nsplit = (int)(ws_bytes / slot);
     if (a.nsplit < 2 || !a.ws) a.nsplit = 1;
     const int G = a.H / a.Hkv, T = q4_tile(a.Dh / 32), NT = (a.S + T - 1) / T;
+    g.G = G;
     g.HG = (G + 7) / 8;
     g.batch = batch;
     g.items_only = a.nsplit == 1;
