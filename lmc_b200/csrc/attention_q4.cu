@@ -45,7 +45,9 @@ __device__ int g_attn_q4_err;  // bit 0: a page id outside the pool, bit 1: a wa
 
 constexpr int Q4_WARPS = 4;
 constexpr int Q4_STAGES = 2;  // tiles in a warp's ring
-constexpr int Q4_ITEM = 1;    // what beginning and ending an item costs, in tiles
+// What beginning and ending an item costs, in tiles (q, the new row, the
+// result): 128 ragged sequences of 8 kv heads 85, 79, 80 us with 1, 2, 3.
+constexpr int Q4_ITEM = 2;
 constexpr float LOG2E = 1.4426950408889634f;
 // Limit of a wait for bulk copies (nanoseconds of %globaltimer).
 __device__ long long g_attn_q4_wait_ns = 1000000000ll;
@@ -558,9 +560,9 @@ __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *d
 // On this chip a warp-level MMA keeps the integer and half pipes from issuing
 // (8 cycles each, measured in one loop with them), so their number counts: 32
 // for 32 rows of 128 dims against 64.  4 heads per kv head of 128 dims, the
-// other form against this one: one sequence of 131072 positions 56 -> 46 us
-// (3.3 TB/s), 128 ragged ones 118 -> 102 us; one head (GPT-2, 700 positions)
-// 10.5 -> 10.3 us.  Eight heads would take this form twice, at 0.8 of the
+// other form against this one: one sequence of 131072 positions 52 -> 42 us
+// (3.6 TB/s), 128 ragged ones 102 -> 79 us (3.9 TB/s); one head (GPT-2, 700
+// positions) 9.6 -> 9.3 us.  Eight heads would take this form twice, at 0.8 of the
 // other's time each, so more than four heads take the other one.
 template <int NB> struct FewState {
     uint32_t qt[NB][2], ql[NB][2];    // q as matrix operands: columns top / middle, low / 0
