@@ -69,18 +69,35 @@ template <int LPR, int U> __global__ void __launch_bounds__(128) k_append_q4(Row
     const unsigned first = blockIdx.x * (U * 128u / LPR) + threadIdx.x / LPR;
     float x[U][2][8];
     long long off[U];
+    unsigned row[U], head[U];
+    bool in[U];
+    // the values first, for every item: they do not wait for the place they go to
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const unsigned item = first + u * (128 / LPR), r = item / a.Hkv, kh = item - r * a.Hkv;
-        off[u] = r < (unsigned)a.rows && w < a.Dh / 8 ? row_offset(a, r, kh) : -1;
-        const size_t at = (size_t)kh * a.Dh + 8 * w;
+        const unsigned item = first + u * (128 / LPR);
+        row[u] = item / a.Hkv;
+        head[u] = item - row[u] * a.Hkv;
+        in[u] = row[u] < (unsigned)a.rows && w < a.Dh / 8;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
 #pragma unroll
         for (int i = 0; i < 8; i++) x[u][0][i] = x[u][1][i] = 0.0f;
-        if (off[u] < 0) continue;
-        if (a.k) load8(a.k + (size_t)r * a.ldk + at, a.vec, x[u][0]);
-        if (a.v) load8(a.v + (size_t)r * a.ldv + at, a.vec, x[u][1]);
-        if (a.k && a.rope_cos) {  // pairs (2 d, 2 d + 1) (src/ops_llama.c:39-48)
-            const size_t t = (size_t)a.pos[r] * (a.Dh / 2) + 4 * w;
+    if (a.k)
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (in[u]) load8(a.k + (size_t)row[u] * a.ldk + (size_t)head[u] * a.Dh + 8 * w, a.vec, x[u][0]);
+    if (a.v)
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (in[u]) load8(a.v + (size_t)row[u] * a.ldv + (size_t)head[u] * a.Dh + 8 * w, a.vec, x[u][1]);
+#pragma unroll
+    for (int u = 0; u < U; u++) off[u] = in[u] ? row_offset(a, row[u], head[u]) : -1;
+    if (a.k && a.rope_cos)  // pairs (2 d, 2 d + 1) (src/ops_llama.c:39-48)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (off[u] < 0) continue;
+            const size_t t = (size_t)a.pos[row[u]] * (a.Dh / 2) + 4 * w;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float c = a.rope_cos[t + i], s = a.rope_sin[t + i], x0 = x[u][0][2 * i], x1 = x[u][0][2 * i + 1];
@@ -88,7 +105,6 @@ template <int LPR, int U> __global__ void __launch_bounds__(128) k_append_q4(Row
                 x[u][0][2 * i + 1] = x0 * s + x1 * c;
             }
         }
-    }
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
