@@ -3,12 +3,17 @@
 //
 // Both stream: append reads 4 Dh bytes per row and side and writes the row's
 // form, read the reverse, so HBM bounds them, and close behind it the
-// instructions per value; a thread therefore has the K and the V side of its
-// rows, whose place in the cache it works out once, and starts all loads
-// before it uses the first.  4-bit rows: LPR = 4 .. 32 lanes per row, eight
-// dims a lane; append takes neighbouring dims (a word of codes, three shuffles
-// for a group's minimum and maximum), read two runs of four (stores without
-// gaps).  The other forms take a warp per row and side.
+// instructions per value (4-bit append issues in 69 of 100 cycles); a thread
+// therefore has the K and the V side of its rows, whose place in the cache it
+// works out once, and starts all loads before it uses the first.  LPR = 4 ..
+// 32 lanes per row, eight dims a lane: append takes neighbouring dims (a word
+// of codes, three shuffles for a group's minimum and maximum; 16 bytes of
+// fp16), read two runs of four (stores without gaps).
+// 32000 rows of 8 x 128, append / read: 4-bit 63 / 51 us (4.7 / 5.9 TB/s),
+// int8 60 / 54 us, fp16 59 / 61 us (6.7 / 6.4 TB/s); 509 rows of 4 x 64 take
+// 2.9 / 1.8 us in 4 bits, most of it latency.
+#include <type_traits>
+
 #include "attention.cuh"
 #include "kv_q4.cuh"
 #include "lmc_common.cuh"
@@ -60,9 +65,43 @@ __device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
     }
 }
 
+struct KvQ4 {};  // the form's tag
+
+// Dims 8 w .. 8 w + 7 of a row into the cache (`active`: this lane has them);
+// the LPR lanes of a row call this together.
+template <typename KV, int LPR> __device__ __forceinline__ void store8(uint8_t *row, bool active, int w, int Dh, const float (&x)[8]) {
+    if constexpr (std::is_same_v<KV, KvQ4>) {
+        uint32_t codes, dm;
+        kv_q4_quantize<LPR>(x, active, codes, dm);
+        if (!active) return;
+        reinterpret_cast<uint32_t *>(row)[w] = codes;
+        if (w % 8 == 0) reinterpret_cast<uint32_t *>(row)[Dh / 8 + w / 8] = dm;
+    } else if constexpr (KvT<KV>::Q8) {  // (as kv_q8_store_row)
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));  // (0 in lanes without dims)
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!active) return;
+        const float inv = m > 0.0f ? 127.0f / m : 0.0f;
+        uint32_t c[2] = {0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            c[i / 4] |= (uint32_t)(max(-127, min(127, __float2int_rn(__fmul_rn(x[i], inv)))) & 0xff) << (8 * (i % 4));
+        reinterpret_cast<uint2 *>(row)[w] = make_uint2(c[0], c[1]);
+        if (w == 0) *reinterpret_cast<float *>(row + Dh) = m / 127.0f;
+    } else if (active) {
+        KV y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = kv_cvt<KV>(x[i]);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof y / 16; i++) reinterpret_cast<uint4 *>(row)[w * (sizeof y / 16) + i] = reinterpret_cast<const uint4 *>(y)[i];
+    }
+}
+
 // Item = (row, kv head), heads innermost; a CTA has U x 128 / LPR neighbouring
 // items, a thread items 128 / LPR apart.
-template <int LPR, int U> __global__ void __launch_bounds__(128) k_append_q4(RowArgs a) {
+template <typename KV, int LPR, int U> __global__ void __launch_bounds__(128) k_append(RowArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     const int w = threadIdx.x % LPR;
@@ -110,119 +149,87 @@ template <int LPR, int U> __global__ void __launch_bounds__(128) k_append_q4(Row
 #pragma unroll
         for (int side = 0; side < 2; side++) {
             if (!(side ? a.v : a.k)) continue;
-            uint32_t codes, dm;
-            kv_q4_quantize<LPR>(x[u][side], off[u] >= 0, codes, dm);
-            if (off[u] < 0) continue;
-            uint32_t *to = reinterpret_cast<uint32_t *>((side ? a.vc : a.kc) + off[u]);
-            to[w] = codes;
-            if (w % 8 == 0) to[a.Dh / 8 + w / 8] = dm;
+            store8<KV, LPR>((side ? a.vc : a.kc) + off[u], off[u] >= 0, w, a.Dh, x[u][side]);
         }
 }
 
-template <int LPR, int U> __global__ void __launch_bounds__(128) k_read_q4(RowArgs a) {
+// Two runs of four dims a lane, so a warp's stores leave no gaps.
+template <typename KV, int LPR> __global__ void __launch_bounds__(128) k_read(RowArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     const int w = threadIdx.x % LPR, half = a.Dh / 8;  // quads w and w + half
     if (w >= half) return;
-    const unsigned first = blockIdx.x * (U * 128u / LPR) + threadIdx.x / LPR;
-    uint32_t codes[U][2][2], dm[U][2][2];
-    long long off[U];
-    unsigned row[U], head[U];
+    const unsigned item = blockIdx.x * (128u / LPR) + threadIdx.x / LPR, r = item / a.Hkv, kh = item - r * a.Hkv;
+    const long long off = r < (unsigned)a.rows ? row_offset(a, r, kh) : -1;
+    if (off < 0) return;
+    using Raw = std::conditional_t<std::is_same_v<KV, float>, uint4, uint2>;
+    Raw raw[2][2];  // every load before the first use
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const unsigned item = first + u * (128 / LPR), r = item / a.Hkv, kh = item - r * a.Hkv;
-        off[u] = r < (unsigned)a.rows ? row_offset(a, r, kh) : -1;
-        row[u] = r;
-        head[u] = kh;
+    for (int side = 0; side < 2; side++) {
+        if (!(side ? a.v : a.k)) continue;
+        const uint8_t *p = (side ? a.vc : a.kc) + off;
 #pragma unroll
-        for (int side = 0; side < 2; side++) {
-            if (off[u] < 0 || !(side ? a.v : a.k)) continue;
-            const uint8_t *p = (side ? a.vc : a.kc) + off[u];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                codes[u][side][i] = reinterpret_cast<const uint16_t *>(p)[w + i * half];
-                dm[u][side][i] = reinterpret_cast<const uint32_t *>(p)[half + (w + i * half) / 16];
-            }
+        for (int i = 0; i < 2; i++) {
+            const int quad = w + i * half;
+            if constexpr (std::is_same_v<KV, KvQ4>)
+                raw[side][i] = make_uint2(reinterpret_cast<const uint16_t *>(p)[quad], reinterpret_cast<const uint32_t *>(p)[half + quad / 16]);
+            else if constexpr (KvT<KV>::Q8)
+                raw[side][i] = make_uint2(reinterpret_cast<const uint32_t *>(p)[quad], *reinterpret_cast<const uint32_t *>(p + a.Dh));
+            else
+                raw[side][i] = reinterpret_cast<const Raw *>(p)[quad];
         }
     }
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int side = 0; side < 2; side++) {
+        if (!(side ? a.v : a.k)) continue;
+        float *to = (side ? a.v + (size_t)r * a.ldv : a.k + (size_t)r * a.ldk) + (size_t)kh * a.Dh + 4 * w;
 #pragma unroll
-        for (int side = 0; side < 2; side++) {
-            if (off[u] < 0 || !(side ? a.v : a.k)) continue;
-            float *to = (side ? a.v + (size_t)row[u] * a.ldv : a.k + (size_t)row[u] * a.ldk) + (size_t)head[u] * a.Dh + 4 * w;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float d = __half2float(__ushort_as_half((unsigned short)(dm[u][side][i] & 0xffff)));
-                const float m = __half2float(__ushort_as_half((unsigned short)(dm[u][side][i] >> 16)));
-                float x[4];
+        for (int i = 0; i < 2; i++) {
+            const Raw u = raw[side][i];
+            float y[4];
+            if constexpr (std::is_same_v<KV, KvQ4>) {
+                const float2 dm = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
 #pragma unroll
                 for (int e = 0; e < 4; e++)  // 2^23 | code is the number 2^23 + code
-                    x[e] = fmaf(d, __uint_as_float(0x4b000000u | ((codes[u][side][i] >> (4 * e)) & 15u)) - 8388608.0f, m);
-                float *p = to + 4 * half * i;
-                if (a.vec) *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-                else
+                    y[e] = fmaf(dm.x, __uint_as_float(0x4b000000u | ((u.x >> (4 * e)) & 15u)) - 8388608.0f, dm.y);
+            } else if constexpr (KvT<KV>::Q8) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) p[e] = x[e];
+                for (int e = 0; e < 4; e++) y[e] = (float)(int8_t)(u.x >> (8 * e)) * __uint_as_float(u.y);
+            } else if constexpr (std::is_same_v<KV, float>) {
+                y[0] = __uint_as_float(u.x); y[1] = __uint_as_float(u.y); y[2] = __uint_as_float(u.z); y[3] = __uint_as_float(u.w);
+            } else {
+                const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+                y[0] = lo.x; y[1] = lo.y; y[2] = hi.x; y[3] = hi.y;
             }
-        }
-}
-
-template <int LPR, int U> int launch_q4(const char *name, const RowArgs &a, bool read, cudaStream_t s) {
-    LMC_LAUNCH(name, (read ? k_read_q4<LPR, U> : k_append_q4<LPR, U>), lmc_cdiv((size_t)a.rows * a.Hkv, U * 128 / LPR), 128, 0, s, a);
-    return LMC_OK;
-}
-// Two items a thread when that still gives every SM eight CTAs, else one.
-template <int LPR> int launch_q4(const char *name, const RowArgs &a, bool read, cudaStream_t s) {
-    const bool many = (long long)a.rows * a.Hkv * LPR >= 2ll * 128 * 8 * lmc_sm_count();
-    return many ? launch_q4<LPR, 2>(name, a, read, s) : launch_q4<LPR, 1>(name, a, read, s);
-}
-
-// One warp per (row, kv head, side) for the other row forms.
-template <typename KV, bool READ>
-__global__ void __launch_bounds__(128) k_rows(RowArgs a) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const bool is_v = blockIdx.y;
-    float *f = is_v ? a.v : a.k;
-    if (!f) return;
-    const unsigned item = blockIdx.x * 4u + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31, r = (int)((unsigned)item / a.Hkv), kh = (int)((unsigned)item % a.Hkv);
-    if (r >= a.rows) return;
-    const long long off = row_offset(a, r, kh);
-    if (off < 0) return;
-    f += (size_t)r * (is_v ? a.ldv : a.ldk) + (size_t)kh * a.Dh;
-    KV *row = reinterpret_cast<KV *>((is_v ? a.vc : a.kc) + off);
-    if constexpr (KvT<KV>::Q8) {
-        if constexpr (READ) {
-            const float sc = kv_q8_scale(row, a.Dh);
-            for (int d = lane; d < a.Dh; d += 32) f[d] = kv_ld<KV>(row + d) * sc;
-        } else {
-            kv_q8_store_row(row, f, nullptr, nullptr, a.Dh, lane);
-        }
-    } else {
-        for (int d = lane; d < a.Dh; d += 32) {
-            if constexpr (READ) f[d] = kv_ld<KV>(row + d);
-            else row[d] = kv_cvt<KV>(f[d]);
+            float *p = to + 4 * half * i;
+            if (a.vec) *reinterpret_cast<float4 *>(p) = make_float4(y[0], y[1], y[2], y[3]);
+            else { p[0] = y[0]; p[1] = y[1]; p[2] = y[2]; p[3] = y[3]; }
         }
     }
 }
 
+// Appending, two items a thread from 32 CTAs (of one item) per SM on: 32000
+// rows of 8 x 128 66 us with one, 63 with two; 2048 rows 6.4 and 6.8.  Reading
+// gains nothing from a second (50 and 52 us).
+template <typename KV, int LPR> int launch(const char *name, const RowArgs &a, bool read, cudaStream_t s) {
+    const size_t items = (size_t)a.rows * a.Hkv;
+    if (read) LMC_LAUNCH(name, (k_read<KV, LPR>), lmc_cdiv(items, 128 / LPR), 128, 0, s, a);
+    else if (items * LPR >= 128ull * 32 * lmc_sm_count()) LMC_LAUNCH(name, (k_append<KV, LPR, 2>), lmc_cdiv(items, 2 * 128 / LPR), 128, 0, s, a);
+    else LMC_LAUNCH(name, (k_append<KV, LPR, 1>), lmc_cdiv(items, 128 / LPR), 128, 0, s, a);
+    return LMC_OK;
+}
+template <typename KV> int launch_form(const char *name, const RowArgs &a, bool read, cudaStream_t s) {
+    const int lanes = a.Dh / 8;
+    return lanes <= 4    ? launch<KV, 4>(name, a, read, s)
+           : lanes <= 8  ? launch<KV, 8>(name, a, read, s)
+           : lanes <= 16 ? launch<KV, 16>(name, a, read, s)
+                         : launch<KV, 32>(name, a, read, s);
+}
 int rows_launch(const char *name, const RowArgs &a, int kv_dtype, bool read, cudaStream_t s) {
-    const long long items = (long long)a.rows * a.Hkv;
-    if (kv_dtype == LMC_KV_Q4) {
-        const int words = a.Dh / 8;
-        return words <= 4    ? launch_q4<4>(name, a, read, s)
-               : words <= 8  ? launch_q4<8>(name, a, read, s)
-               : words <= 16 ? launch_q4<16>(name, a, read, s)
-                             : launch_q4<32>(name, a, read, s);
-    }
-    const dim3 grid(lmc_cdiv(items, 4), 2);
-    void (*fn)(RowArgs) = kv_dtype == LMC_KV_F32   ? (read ? k_rows<float, true> : k_rows<float, false>)
-                          : kv_dtype == LMC_KV_F16 ? (read ? k_rows<__half, true> : k_rows<__half, false>)
-                                                   : (read ? k_rows<KvQ8, true> : k_rows<KvQ8, false>);
-    LMC_LAUNCH(name, fn, grid, 128, 0, s, a);
-    return LMC_OK;
+    return kv_dtype == LMC_KV_Q4    ? launch_form<KvQ4>(name, a, read, s)
+           : kv_dtype == LMC_KV_Q8  ? launch_form<KvQ8>(name, a, read, s)
+           : kv_dtype == LMC_KV_F16 ? launch_form<__half>(name, a, read, s)
+                                    : launch_form<float>(name, a, read, s);
 }
 
 // The checks that lmc_kv_append and lmc_kv_read share; fills `a`.
