@@ -300,7 +300,8 @@ int lmc_kv_read(float *d_k, float *d_v, int ld, const void *d_k_cache, const voi
  * fork: sequence b becomes a copy of sequence d_parent[b] (all rows as they
  * were before the call), sharing its pages; d_parent[b] == b leaves it as it
  * is, -1 gives its pages back (entries -1).  So one call forks samples,
- * reorders beams and frees finished sequences.  No page is copied here.
+ * reorders beams and frees finished sequences.  No page is copied here.  At
+ * most 16384 sequences.
  *
  * reserve: makes position d_pos[b] of every sequence b writable (negative:
  * nothing to do for b): an entry that is -1 gets a free page, and a page that
@@ -320,7 +321,8 @@ int lmc_kv_read(float *d_k, float *d_v, int ld, const void *d_k_cache, const voi
  * and V pool; 16-byte aligned), read during the call; page_bytes = Hkv *
  * page_size * LMC_KV_ROW_BYTES (a multiple of 16).  d_workspace holds
  * lmc_kv_pages_workspace_bytes(n_seqs, n_pages) bytes, used until the call's
- * work is done: calls that may overlap on the GPU need one each. */
+ * work is done: calls that may overlap on the GPU need one each.  reserve and
+ * compact take pools of up to 2^30 pages. */
 size_t lmc_kv_pages_workspace_bytes(int n_seqs, int n_pages);
 int lmc_kv_pages_fork(int *d_pages, int n_seqs, int max_pages, int *d_refs, int n_pages, const int *d_parent,
                       void *stream);

@@ -258,3 +258,41 @@ def test_samples_and_beams_share_a_prompt(cuda, kvd):
     fork([-1] * B)
     assert int(refs.abs().sum()) == 0 and int(table.max()) == -1
     assert rt.lib().lmc_device_status() == 0
+
+
+@pytest.mark.parametrize("n_seqs,width,n_pages,pinned", [(700, 80, 40000, 0), (60, 40, 50021, 33000), (60, 40, 16384, 16000),
+                                                         (3, 5, 16385, 16384), (900, 60, 32769, 400)])
+def test_pools_of_many_pages(cuda, n_seqs, width, n_pages, pinned):
+    """Pools that the plans go through in several rounds; the first `pinned`
+    pages have a count of their own that no table names."""
+    rng = np.random.default_rng(n_pages + pinned)
+    table, refs = state(rng, n_seqs, width, n_pages, 0.9, 0.4)
+    if pinned:  # the tables' pages lie anywhere behind them
+        free = pinned + rng.permutation(n_pages - pinned)
+        names = np.unique(table[table >= 0])
+        names = names[:len(free)]
+        to = np.full(n_pages, -1, np.int32)
+        to[names] = free[:len(names)]
+        table = np.where(table >= 0, to[table], -1).astype(np.int32)
+        refs = np.bincount(table[table >= 0], minlength=n_pages).astype(np.int32)
+        refs[:pinned] = 1
+    pool = Pool(cuda, rng, 1, n_pages, 16)
+    dt, dr = dev(cuda, table), dev(cuda, refs)
+    held = (table >= 0).sum(1)
+    for step in range(2):
+        pos = np.minimum(held + step, width - 1) * 16 + step
+        missing, pairs = kv_ref.reserve(table, refs, pos, 16)
+        assert reserve(cuda, pool, dt, dr, pos, 16, n_pages) == missing
+        pool.copied(pairs)
+        assert np.array_equal(dt.cpu().numpy(), table) and np.array_equal(dr.cpu().numpy(), refs)
+    pool.check()
+    ws, n = workspace(cuda, n_seqs, n_pages)
+    live = cuda.full((1,), -7, dtype=cuda.int32, device="cuda")
+    rt.call("lmc_kv_pages_compact", pool.list, 1, 16, dt.data_ptr(), n_seqs, width, dr.data_ptr(), n_pages, live.data_ptr(),
+            ws.data_ptr(), n, None)
+    n_live, pairs = kv_ref.compact(table, refs)
+    pool.copied(pairs)
+    assert int(live.cpu()) == n_live and (ws[n:] == 0xff).all()
+    assert np.array_equal(dt.cpu().numpy(), table) and np.array_equal(dr.cpu().numpy(), refs)
+    pool.check()
+    assert rt.lib().lmc_device_status() == 0

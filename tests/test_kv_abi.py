@@ -106,6 +106,16 @@ def test_page_operator_refusals():
         assert rc == INVALID and word in msg, (args, rc, msg)
 
 
+def test_page_pools_too_large_are_refused():
+    one, n = (ctypes.c_void_p * 1)(4096), (1 << 30) + 1
+    ws = rt.lib().lmc_kv_pages_workspace_bytes(4, n)
+    assert ws > 16 << 30
+    for args in (("lmc_kv_pages_reserve", one, 1, 4096, P, 4, 8, 16, P, n, P, P, P, ws, None),
+                 ("lmc_kv_pages_compact", one, 1, 4096, P, 4, 8, P, n, P, P, ws, None)):
+        rc, msg = status(*args)
+        assert rc == INVALID and b"1073741825 pages" in msg, (rc, msg)
+
+
 def test_model_load_takes_4_bit_rows_and_refuses_unknown_ones():
     h = ctypes.c_void_p()
     rc, msg = status("lmc_model_load", b"/nonexistent.gguf", 1, rt.KV_Q4, ctypes.byref(h))
