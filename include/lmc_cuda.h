@@ -58,7 +58,8 @@ const char *lmc_last_error(void);
 int lmc_device_status(void);
 
 /* Limit of every bounded wait inside the kernels - the bulk-copy rings of
- * the GEMV and GEMM, the grid barriers of the persistent decode step - in
+ * the GEMV, GEMM and 4-bit attention, the grid barriers of the persistent
+ * decode step - in
  * nanoseconds; 0 restores the default of one second.  A wait that runs out
  * records a timeout that lmc_device_status reports; the kernel drains its
  * own copies and returns, and the context stays usable.  No counterpart in
@@ -66,7 +67,8 @@ int lmc_device_status(void);
 int lmc_set_wait_limit(long long ns);
 /* Self-test of that failure path: runs a device wait that nothing can
  * complete - which = 0: a GEMV ring's mbarrier wait, 1: a persistent-step
- * grid barrier (two CTAs) - under the current limit.  Returns LMC_ERR_TIMEOUT
+ * grid barrier (two CTAs), 2: the 4-bit attention's copy ring - under the
+ * current limit.  Returns LMC_ERR_TIMEOUT
  * when the wait ran out as designed (and clears the recorded timeout). */
 int lmc_wait_selftest(int which);
 

@@ -1189,6 +1189,22 @@ extern "C" int lmc_attn_q4_set_wait_limit(long long ns) {
     return LMC_OK;
 }
 
+// Failure-path self-test: a wait for bulk copies that nobody issued runs out,
+// is recorded, and the kernel returns.
+__global__ void k_attn_q4_wait_selftest(int *gave_up) {
+    __shared__ __align__(8) uint64_t sh_bar;
+    if (threadIdx.x) return;
+    const uint32_t bar = (uint32_t)__cvta_generic_to_shared(&sh_bar);
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *gave_up = bar_wait_long(bar, 0u) ? 0 : 1;
+}
+extern "C" int lmc_attn_q4_wait_selftest(int *d_flag, cudaStream_t s) {
+    k_attn_q4_wait_selftest<<<1, 32, 0, s>>>(d_flag);
+    LMC_LAUNCH_CHECK("wait self-test");
+    return LMC_OK;
+}
+
 extern "C" int lmc_attn_q4_status(void) {
     int v = 0;
     LMC_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_attn_q4_err, sizeof(int)));

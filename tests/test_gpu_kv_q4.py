@@ -19,7 +19,7 @@ from tests.conftest import rel_err
 
 pytestmark = pytest.mark.gpu
 
-INVALID = -1
+INVALID, TIMEOUT = -1, -6
 GUARD = 64  # bytes behind every cache that must stay as they were
 
 
@@ -451,6 +451,18 @@ def test_attention_page_outside_the_pool(cuda):
     for now, was in zip((c.dk, c.dv), before):  # only sequence 0's new row changed
         was[c.table[0, 2], :, 8] = now[c.table[0, 2], :, 8]
         assert cuda.equal(now, was)
+
+
+def test_attention_wait_that_runs_out(cuda):
+    """A wait for copies that never come ends within the limit, is reported
+    once, and the next call's result is right."""
+    rt.call("lmc_set_wait_limit", 2_000_000)  # 2 ms
+    try:
+        assert rt.lib().lmc_wait_selftest(2) == TIMEOUT and b"4-bit attention" in rt.lib().lmc_last_error()
+        assert rt.lib().lmc_device_status() == 0
+    finally:
+        rt.call("lmc_set_wait_limit", 0)
+    attend(cuda, 60, [100, 20], 2, 4, 64, 128, 16)
 
 
 def test_attention_captured_and_replayed(cuda):
