@@ -275,10 +275,11 @@ int lmc_attention_decode_paged(float *d_out, const float *d_q, const float *d_k_
  * lmc_kv_append stores the rows in the cache's row form (the same bytes
  * lmc_attention_decode writes); rows must name distinct positions.
  * lmc_kv_read writes the values the cached rows stand for.  A row whose
- * position is negative is padding: nothing is read or written for it.  A
+ * position is negative is padding: nothing is written for it (d_k and d_v
+ * hold `rows` rows all the same, padding among them).  A
  * position >= S, a sequence outside [0, n_seqs) or a page outside
- * [0, n_pages) is left out the same way, and lmc_device_status() then
- * reports LMC_ERR_INVALID. */
+ * [0, n_pages) leaves its row out (nothing is written for it), and
+ * lmc_device_status() then reports LMC_ERR_INVALID. */
 int lmc_kv_append(const float *d_k, const float *d_v, int ld, void *d_k_cache, void *d_v_cache, int kv_dtype,
                   const int *d_seq, const int *d_pos, int rows, int n_seqs, int Hkv, int Dh, int S,
                   const int *d_pages, int page_size, int n_pages, void *stream);

@@ -1140,7 +1140,9 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
 template <int NB, bool FEW> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
     const int GH = g.a.H / g.a.Hkv < 8 ? g.a.H / g.a.Hkv : 8;
     const size_t smem = (size_t)Q4_WARPS * Q4<NB>::WARP_BYTES + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
-    LMC_CUDA_TRY(cudaFuncSetAttribute((k_attn_q4<NB, FEW>), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // the most that any G takes: threads that call with different ones set the same value
+    constexpr int MOST = Q4_WARPS * Q4<NB>::WARP_BYTES + Q4_WARPS * (FEW ? 4 : 8) * Q4<NB>::SLOT * (int)sizeof(float);
+    LMC_CUDA_TRY(cudaFuncSetAttribute((k_attn_q4<NB, FEW>), cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
     const int most = lmc_sm_count() * (smem + 2048 <= 114 * 1024 ? 2 : 1), want = max_units / g.rmin;
     LMC_LAUNCH("attention (4-bit rows)", (k_attn_q4<NB, FEW>), want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);
     return LMC_OK;

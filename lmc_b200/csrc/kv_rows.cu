@@ -110,7 +110,8 @@ template <typename KV, int LPR, int U> __global__ void __launch_bounds__(128) k_
     long long off[U];
     unsigned row[U], head[U];
     bool in[U];
-    // the values first, for every item: they do not wait for the place they go to
+    // the values first, padding's too: they do not wait for the place they go to
+    // (after the position 32000 rows take 68 us, 509 rows of 4 x 64 3.9)
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const unsigned item = first + u * (128 / LPR);

@@ -465,6 +465,41 @@ def test_attention_wait_that_runs_out(cuda):
     attend(cuda, 60, [100, 20], 2, 4, 64, 128, 16)
 
 
+def test_attention_from_several_threads(cuda):
+    """Calls of different group sizes (shared memory of different sizes, one
+    kernel) from three threads at once, each on its own stream."""
+    import threading
+    todo, errors = [], []
+    for i, G in enumerate((1, 4, 2)):
+        rng = np.random.default_rng(70 + G)
+        c = Cache(cuda, rng, [90, 33], 2, 64, 128, 0)
+        q, kn, vn = (rows_of(rng, (2, n * 64)) for n in (2 * G, 2, 2))
+        out = cuda.full((2, 2 * G * 64), 5.0, device="cuda")
+        d = [dev(cuda, a) for a in (q, kn, vn, np.array([90, 33], np.int32))]
+        todo.append((c, q, kn, vn, out, d, G, cuda.cuda.Stream()))
+    wsb = rt.lib().lmc_attention_workspace_bytes(2, 8, 64, 128)
+    spaces = [cuda.full((wsb + GUARD,), 0xff, dtype=cuda.uint8, device="cuda") for _ in todo]
+    cuda.cuda.synchronize()
+
+    def run(job, ws):
+        c, _, _, _, out, d, G, stream = job
+        try:
+            for _ in range(300):
+                c.decode(cuda, out, d[0], d[1], d[2], d[3], G, stream=stream.cuda_stream, ws=ws)
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(todo, spaces)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    cuda.cuda.synchronize()
+    assert not errors, errors
+    for c, q, kn, vn, out, _, G, _ in todo:
+        c.check(out.cpu().numpy(), q, kn, vn, [90, 33], G)
+
+
 def test_attention_captured_and_replayed(cuda):
     """The call in a CUDA graph, replayed while positions move on: each
     replay attends one row more and appends at the new position; a second
