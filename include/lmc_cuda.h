@@ -313,7 +313,8 @@ int lmc_kv_read(float *d_k, float *d_v, int ld, const void *d_k_cache, const voi
  * keeps it when no other entry names it).  Free pages are handed out lowest
  * id first, in order of b.  When fewer are free than needed nothing changes
  * and *d_short receives how many are missing (else 0).  Call it before the
- * step that writes those positions.
+ * step that writes those positions, and do not run that step when *d_short
+ * is not 0: it would write into pages that other sequences share.
  *
  * compact: moves the pages in use to the ids 0 .. *d_n_live - 1 (the i-th
  * page in use above that range, in ascending order, to the i-th free id in
