@@ -167,6 +167,35 @@ def test_append_and_read(cuda, kvd, rows, Hkv, Dh, S, P, extra, shift):
     assert rt.lib().lmc_device_status() == 0
 
 
+@pytest.mark.parametrize("kvd", [rt.KV_F32, rt.KV_F16, rt.KV_Q8, rt.KV_Q4])
+def test_append_and_read_many_rows(cuda, kvd):
+    """Enough rows for two a thread, the last ones alone; one in seven is
+    padding."""
+    rows, Hkv, Dh, S = 5001, 8, 128, 2600
+    rng = np.random.default_rng(9)
+    x = rows_of(rng, (2, rows, Hkv * Dh), "outliers")
+    where = rng.permutation(2 * S)[:rows]
+    seq, pos = (where // S).astype(np.int32), (where % S).astype(np.int32)
+    skip = np.arange(rows) % 7 == 6
+    RB = rt.kv_row_bytes(kvd, Dh)
+    c = [cuda.full((2, Hkv, S, RB), 0x5A, dtype=cuda.uint8, device="cuda") for _ in range(2)]
+    dx, out = dev(cuda, x), cuda.full((2, rows, Hkv * Dh), 7.0, device="cuda")
+    dpos, dseq = dev(cuda, np.where(skip, -1, pos).astype(np.int32)), dev(cuda, seq)
+    tail = (Hkv * Dh, c[0].data_ptr(), c[1].data_ptr(), kvd, dseq.data_ptr(), dpos.data_ptr(), rows, 2, Hkv, Dh, S, None, 0, 0,
+            None)
+    rt.call("lmc_kv_append", dx[0].data_ptr(), dx[1].data_ptr(), *tail)
+    rt.call("lmc_kv_read", out[0].data_ptr(), out[1].data_ptr(), *tail)
+    for side in range(2):
+        w, val = stored(x[side].reshape(rows, Hkv, Dh), kvd)
+        ref = np.full(c[side].shape, 0x5A, np.uint8)
+        ref[seq[~skip], :, pos[~skip]] = w[~skip]
+        sized = slice(0, RB if kvd != rt.KV_Q8 else Dh + 4)
+        assert np.array_equal(c[side].cpu().numpy()[..., sized], ref[..., sized])
+        o, want = out[side].cpu().numpy(), val.reshape(rows, -1)
+        assert (o[skip] == 7).all() and (np.abs(o - want)[~skip] <= 2.0 ** -24 * np.abs(want)[~skip]).all()
+    assert rt.lib().lmc_device_status() == 0
+
+
 @pytest.mark.parametrize("kvd", [rt.KV_F16, rt.KV_Q4])
 def test_rows_outside_the_cache_are_left_out(cuda, kvd):
     """A position at the context's end, a sequence that does not exist, a page
@@ -294,6 +323,26 @@ def test_attention_group_sizes(cuda, G, Dh, P):
 def test_attention_head_sizes_of_large_groups(cuda, Dh, G, P):
     """More than four query heads per kv head take another form of the kernel."""
     attend(cuda, Dh + G, [150, 63, 0], 2, G, Dh, 160, P)
+
+
+@pytest.mark.parametrize("Hkv,G,Dh,S,P,pos", [(2, 4, 64, 2048, 16, [1500, 3]), (2, 8, 128, 512, 0, [400, 64, -1]),
+                                              (1, 3, 96, 160, 32, [100]), (3, 5, 224, 64, 0, [40, 63])])
+def test_attention_of_rows_off_the_16_byte_boundary(cuda, Hkv, G, Dh, S, P, pos):
+    """q, the new rows and the output at any 4-byte address."""
+    rng = np.random.default_rng(S + G)
+    B = len(pos)
+    c = Cache(cuda, rng, [max(p, 0) for p in pos], Hkv, Dh, S, P)
+    host = [rows_of(rng, (B, Hkv * n * Dh)) for n in (G, 1, 1)]
+    flat = []
+    for i, a in enumerate(host):
+        t = cuda.zeros(a.size + 8, device="cuda")
+        t[i + 1:i + 1 + a.size] = dev(cuda, a).flatten()
+        flat.append(t[i + 1:i + 1 + a.size].view(a.shape))
+    o = cuda.full((B * Hkv * G * Dh + 8,), 5.0, device="cuda")
+    out = o[3:3 + B * Hkv * G * Dh].view(B, -1)
+    c.decode(cuda, out, *flat, dev(cuda, np.array(pos, np.int32)), G)
+    c.check(out.cpu().numpy(), *host, pos, G)
+    assert (o[:3] == 5).all() and (o[-5:] == 5).all()
 
 
 @pytest.mark.parametrize("G", [1, 3, 4, 5, 8])
