@@ -199,24 +199,24 @@ template <int NB> __device__ __forceinline__ void set_seq(const Q4Args &g, Item 
     while (p.b < g.batch && (p.pos = seq_pos(g, p.b)) < 0) p.b++;
     p.nt = p.pos / Q4<NB>::T + 1;
 }
-// The share's next item, in place (tile == end: there is none).  The items of
-// the copies and of the computation lie in shared memory: only what each tile
-// needs is kept in registers.
+// The share goes on behind the item.
+__device__ __forceinline__ bool more_items(const Q4Args &g, const Item *at) { return at->left > item_units(g, at->nt); }
+// The share's next item, in place (tile == end: of it there are no tiles).  The
+// items of the copies and of the computation lie in shared memory: only what
+// each tile needs is kept in registers.
 template <int NB> __device__ __noinline__ void next_item(const Q4Args &g, Item *at) {
     Item p = *at;
     const int units = item_units(g, p.nt);
     p.unit += units;
     p.left -= units;
-    p.tile = p.end = 0;
-    if (p.left > 0) {
-        if (++p.j == g.a.Hkv * g.HG) {
-            p.j = 0;
-            p.b++;
-            set_seq<NB>(g, p);
-        }
-        set_item<NB>(g, p);
-        p.end = max(p.end, 0);
+    p.tile = 0;
+    if (++p.j == g.a.Hkv * g.HG) {
+        p.j = 0;
+        p.b++;
+        set_seq<NB>(g, p);
     }
+    set_item<NB>(g, p);
+    p.end = max(p.end, 0);
     __syncwarp();
     *at = p;  // (every lane the same)
     __syncwarp();
@@ -809,13 +809,17 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
     const AttnArgs &a = g.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = g.G, items = a.Hkv * g.HG, GH = min(G, 8);
+    if (lane == 0) {
+        desc[warp][0].unit = desc[warp][1].unit = -1;
+        for (int i = 0; i < Q4_STAGES; i++)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&sh_bar[warp][i])));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     pdl_wait();
     pdl_launch_dependents();
     // units (tiles) of the whole batch, and this CTA's and this warp's share
-    auto units_of = [&](int b) -> int {
-        const int p = seq_pos(g, b);
-        return p < 0 ? 0 : item_units(g, p / T + 1) * items;
-    };
+    auto units_at = [&](int pos) -> int { return pos < 0 ? 0 : item_units(g, pos / T + 1) * items; };
     // up to 32 sequences: each warp sums them by itself
     auto scan = [&](int mine) {  // inclusive sum over the lanes
 #pragma unroll
@@ -826,21 +830,15 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         return mine;
     };
     const bool small = g.batch <= 32;
-    int mine = 0, inc = 0, total;
-    if (lane == 0) {
-        desc[warp][0].unit = desc[warp][1].unit = -1;
-        for (int i = 0; i < Q4_STAGES; i++)
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&sh_bar[warp][i])));
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
+    int pos = -1, mine = 0, inc = 0, total;  // lane's sequence
     if (small) {
-        mine = lane < g.batch ? units_of(lane) : 0;
+        if (lane < g.batch) pos = seq_pos(g, lane);
+        mine = units_at(pos);
         inc = scan(mine);
         total = __shfl_sync(0xffffffffu, inc, 31);
-        __syncwarp();
     } else {
         int sum = 0;
-        for (int b = threadIdx.x; b < g.batch; b += 32 * Q4_WARPS) sum += units_of(b);
+        for (int b = threadIdx.x; b < g.batch; b += 32 * Q4_WARPS) sum += units_at(seq_pos(g, b));
         sum = __reduce_add_sync(0xffffffffu, sum);
         if (lane == 0) sh_total[warp] = sum;
         __syncthreads();
@@ -862,23 +860,25 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
     if (u0 < u1) {
         // where unit u0 lies
         Item p;
-        p.b = 0;
+        p.b = p.pos = 0;
         int before = 0;
         for (int b0 = 0; b0 < g.batch; b0 += 32) {
             if (!small) {
-                mine = b0 + lane < g.batch ? units_of(b0 + lane) : 0;
+                pos = b0 + lane < g.batch ? seq_pos(g, b0 + lane) : -1;
+                mine = units_at(pos);
                 inc = scan(mine);
             }
             const unsigned hit = __ballot_sync(0xffffffffu, before + inc > u0);
             if (hit) {
                 const int w = __ffs(hit) - 1;
                 p.b = b0 + w;
+                p.pos = __shfl_sync(0xffffffffu, pos, w);
                 before += __shfl_sync(0xffffffffu, inc - mine, w);
                 break;
             }
             before += __shfl_sync(0xffffffffu, inc, 31);
         }
-        set_seq<NB>(g, p);
+        p.nt = p.pos / T + 1;
         const int at = u0 - before, units = item_units(g, p.nt);
         p.j = at / units;
         const int within = at - p.j * units;
@@ -940,8 +940,12 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                 fetch(fill);
                 flying |= 1u << fill;
                 if (++a_tile == a_end) {
-                    next_item<NB>(g, ia);
-                    item_ahead();
+                    if (more_items(g, ia)) {
+                        next_item<NB>(g, ia);
+                        item_ahead();
+                    } else {
+                        a_tile = a_end = 0;
+                    }
                 } else {
                     look_up();
                 }
@@ -996,6 +1000,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                     desc[warp][part] = Part{ii->unit, b, head, heads, first, end, nt};
                 }
                 part = 1;
+                if (!more_items(g, ii)) break;
                 next_item<NB>(g, ii);
                 tile = ii->tile;
                 end = ii->end;

@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t kv_q4_codes(const float (&x)[8], float d, fl
         codes += __float_as_uint(k) << (4 * i);
     }
     codes -= (uint32_t)(0x4b400000ull * 0x11111111ull);  // the eight sums' 1.5 * 2^23
-    if (far > 0.49998f) {
+    if (__builtin_expect(far > 0.49998f, 0)) {
         codes = 0u;
 #pragma unroll 1
         for (int i = 0; i < 8; i++) {
