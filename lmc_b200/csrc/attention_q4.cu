@@ -32,6 +32,13 @@
 // 16-byte boundaries) with a running softmax; parts of one item that lie in
 // one CTA are merged in shared memory, parts in several CTAs through the
 // workspace by k_q4_combine.
+//
+// Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 41 us, 128 ragged
+// sequences of them 79 us (3.6 and 3.9 TB/s), 64 ragged ones of 4 heads of 64
+// dims 18.7 us, one of 12 heads with 700 positions 8.3 us.  Instructions bound
+// the first two (matrix, integer and half instructions share the issue), the
+// latency of a warp's chain (its share, the copies, q, a tile, the merge) the
+// others.
 #include <algorithm>
 #include <type_traits>
 
@@ -47,7 +54,8 @@ __device__ int g_attn_q4_err;  // bit 0: a page id outside the pool, bit 1: a wa
 constexpr int Q4_WARPS = 4;
 constexpr int Q4_STAGES = 2;  // tiles in a warp's ring
 // What beginning and ending an item costs, in tiles (q, the new row, the
-// result): 128 ragged sequences of 8 kv heads 85, 79, 80 us with 1, 2, 3.
+// result): 128 ragged sequences of 8 kv heads 85, 79, 80 us with 1, 2, 3; 64 of
+// 4 kv heads, eight query heads each, 18.9, 18.7, 19.1.
 constexpr int Q4_ITEM = 2;
 constexpr float LOG2E = 1.4426950408889634f;
 // Limit of a wait for bulk copies (nanoseconds of %globaltimer).
@@ -561,9 +569,9 @@ __device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *d
 // On this chip a warp-level MMA keeps the integer and half pipes from issuing
 // (8 cycles each, measured in one loop with them), so their number counts: 32
 // for 32 rows of 128 dims against 64.  4 heads per kv head of 128 dims, the
-// other form against this one: one sequence of 131072 positions 52 -> 42 us
-// (3.6 TB/s), 128 ragged ones 102 -> 79 us (3.9 TB/s); one head (GPT-2, 700
-// positions) 9.6 -> 9.3 us.  Eight heads would take this form twice, at 0.8 of the
+// other form against this one: one sequence of 131072 positions 52 -> 41 us
+// (3.6 TB/s), 128 ragged ones 101 -> 79 us (3.9 TB/s); one head (GPT-2, 700
+// positions) 8.4 -> 8.3 us.  Eight heads would take this form twice, at 0.8 of the
 // other's time each, so more than four heads take the other one.
 template <int NB> struct FewState {
     uint32_t qt[NB][2], ql[NB][2];    // q as matrix operands: columns top / middle, low / 0
@@ -1077,7 +1085,8 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
 // Merges the parts of each (row, query head) that several CTAs left in the
 // workspace; nothing to do when slot 0's sum is zero.  W warps (1 or 4) share
 // a head's parts: four when there are few heads, whose parts are then many
-// (131072 positions of one sequence: 56 for each of 32 heads).
+// (131072 positions of one sequence, 56 parts for each of 32 heads, the whole
+// call: 45.9 us with one, 41.5 with four; 128 sequences of 32 heads 79 and 82).
 template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a, int batch) {
     pdl_wait();
     pdl_launch_dependents();
