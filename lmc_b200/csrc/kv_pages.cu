@@ -6,6 +6,8 @@
 // bound by latency; what costs bandwidth is copying pages, 2 x page_bytes x
 // pools for each, done by one kernel for all pools of a call from the list of
 // page pairs that the plan left in the workspace.
+#include <algorithm>
+
 #include "lmc_common.cuh"
 #include "lmc_internal.h"
 
@@ -312,9 +314,11 @@ int check_pools(const char *name, void *const *h_pools, int n_pools, size_t page
     return LMC_OK;
 }
 
-int copy_launch(const char *name, void *const *h_pools, int n_pools, size_t page_bytes, const int *ws, int *pages,
+// At most `most` pages are copied and `entries` table entries renamed: no more CTAs than that has work for.
+int copy_launch(const char *name, void *const *h_pools, int n_pools, size_t page_bytes, int most, const int *ws, int *pages,
                 long long entries, const int *d_n_live, int n_pages, cudaStream_t s) {
-    const int grid = lmc_sm_count() * 8;
+    const long long pieces = (long long)(page_bytes / 16 + COPY_VECS - 1) / COPY_VECS * std::min(n_pools, MAX_POOLS) * most;
+    const int grid = (int)std::min<long long>(lmc_sm_count() * 8, std::max(pieces, (entries + 255) / 256));
     for (int p0 = 0; p0 < n_pools; p0 += MAX_POOLS) {
         Pools pools;
         const int n = n_pools - p0 < MAX_POOLS ? n_pools - p0 : MAX_POOLS;
@@ -369,7 +373,7 @@ extern "C" int lmc_kv_pages_reserve(void *const *h_pools, int n_pools, size_t pa
     cudaStream_t s = lmc_stream(stream);
     LMC_LAUNCH("kv pages reserve", (n_pages <= SMALL_POOL ? k_reserve_plan<1> : k_reserve_plan<16>), 1, PLAN_THREADS, 0, s, d_pages, n_seqs, max_pages, shift, d_refs, n_pages,
                d_pos, d_short, (int *)d_ws);
-    return copy_launch("kv pages copy", h_pools, n_pools, page_bytes, (const int *)d_ws, nullptr, 0, nullptr, n_pages, s);
+    return copy_launch("kv pages copy", h_pools, n_pools, page_bytes, n_seqs, (const int *)d_ws, nullptr, 0, nullptr, n_pages, s);
 }
 
 extern "C" int lmc_kv_pages_compact(void *const *h_pools, int n_pools, size_t page_bytes, int *d_pages, int n_seqs,
@@ -387,7 +391,7 @@ extern "C" int lmc_kv_pages_compact(void *const *h_pools, int n_pools, size_t pa
                              lmc_kv_pages_workspace_bytes(n_seqs, n_pages));
     cudaStream_t s = lmc_stream(stream);
     LMC_LAUNCH("kv pages compact", (n_pages <= SMALL_POOL ? k_compact_plan<1> : k_compact_plan<16>), 1, PLAN_THREADS, 0, s, d_refs, n_pages, d_n_live, (int *)d_ws);
-    return copy_launch("kv pages copy", h_pools, n_pools, page_bytes, (const int *)d_ws, d_pages,
+    return copy_launch("kv pages copy", h_pools, n_pools, page_bytes, n_pages / 2, (const int *)d_ws, d_pages,
                        (long long)n_seqs * max_pages, d_n_live, n_pages, s);
 }
 
