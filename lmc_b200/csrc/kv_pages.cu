@@ -96,7 +96,7 @@ template <int M, class F> __device__ __forceinline__ int number_pages(const unsi
 // in the counts of row r's old entries is the same in every column: one more
 // for each other row that copies r, one less when r itself is replaced; so one
 // atomic addition per entry of a row where that is not 0 (and none per copy;
-// 256 rows of 2048 entries 24 -> 7.8 us).  5 rows of 128: 3.1 us, latency.
+// 256 rows of 2048 entries 24 -> 7.5 us).  5 rows of 128: 3.0 us, latency.
 __global__ void __launch_bounds__(256) k_pages_fork(int *pages, int n_seqs, int max_pages, int *refs, int n_pages,
                                                     const int *parent, int cs) {
     extern __shared__ int tile[];  // [n_seqs][2^cs], then parent[n_seqs], change[n_seqs]
@@ -104,8 +104,12 @@ __global__ void __launch_bounds__(256) k_pages_fork(int *pages, int n_seqs, int 
     pdl_wait();
     pdl_launch_dependents();
     const int c0 = blockIdx.x << cs, nc = min(1 << cs, max_pages - c0), mask = (1 << cs) - 1;
+    const int p0 = threadIdx.x < n_seqs ? parent[threadIdx.x] : 0;  // (on its way beside the table)
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n_seqs << cs; i += 256)
+        if ((i & mask) < nc) tile[i] = pages[(size_t)(i >> cs) * max_pages + c0 + (i & mask)];
     for (int b = threadIdx.x; b < n_seqs; b += 256) {
-        int p = parent[b];
+        int p = b < 256 ? p0 : parent[b];
         if (p >= n_seqs) {
             atomicExch(&g_kv_pages_err, 1);
             p = b;
@@ -113,9 +117,6 @@ __global__ void __launch_bounds__(256) k_pages_fork(int *pages, int n_seqs, int 
         par[b] = p;
         change[b] = p == b ? 0 : -1;
     }
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n_seqs << cs; i += 256)
-        if ((i & mask) < nc) tile[i] = pages[(size_t)(i >> cs) * max_pages + c0 + (i & mask)];
     __syncthreads();
     for (int b = threadIdx.x; b < n_seqs; b += 256)
         if (par[b] >= 0 && par[b] != b) atomicAdd(change + par[b], 1);
