@@ -3,7 +3,7 @@
 //
 // Both stream: append reads 4 Dh bytes per row and side and writes the row's
 // form, read the reverse, so HBM bounds them, and close behind it the
-// instructions per value (4-bit append issues in 69 of 100 cycles); a thread
+// instructions per value (4-bit append issues in 75 of 100 cycles); a thread
 // therefore has the K and the V side of its rows, whose place in the cache it
 // works out once, and starts all loads before it uses the first.  LPR = 4 ..
 // 32 lanes per row, eight dims a lane: append takes neighbouring dims (a word
