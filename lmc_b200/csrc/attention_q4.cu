@@ -1092,12 +1092,24 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
     pdl_launch_dependents();
     __shared__ float sh[W == 1 ? 1 : 4][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long id = W == 1 ? (long long)blockIdx.x * 4 + warp : blockIdx.x;
-    const int b = (int)(id / a.H), h = (int)(id % a.H), Dh = a.Dh;
+    const unsigned id = W == 1 ? blockIdx.x * 4 + warp : blockIdx.x;  // (batch x H is an int)
+    const int b = (int)(id / (unsigned)a.H), h = (int)(id - (unsigned)b * a.H), Dh = a.Dh;
     if (b >= batch) return;
-    const int pos = a.pos[b];
-    if (pos < 0 || pos >= a.S) return;
+    const int pos = a.pos[b], first = W == 1 ? 0 : warp;
     const float *w = a.ws + ((size_t)b * a.H + h) * a.nsplit * (Dh + 2);
+    float v[4][8];
+    auto load = [&](int k0, int n) {  // four parts' accumulators, one in W from k0 on
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int k = k0 + u * W;
+                v[u][e] = k < n && lane + 32 * e < Dh ? w[(size_t)k * (Dh + 2) + lane + 32 * e] : 0.0f;
+            }
+    };
+    // Few heads: beside the slots' maxima and sums, before those tell what is in them
+    // (700 positions of 12 heads 8.3 -> 7.8 us); for many heads that reads too much.
+    if (W > 1) load(first, a.nsplit);
     // offsets and sums of all slots (at most 64); slots past the last part hold anything
     float m[2], l[2];
     int n = a.nsplit;
@@ -1107,7 +1119,7 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
         m[i] = k < a.nsplit ? w[(size_t)k * (Dh + 2) + Dh] : 0.0f;
         l[i] = k < a.nsplit ? w[(size_t)k * (Dh + 2) + Dh + 1] : 0.0f;
     }
-    if (__shfl_sync(0xffffffffu, l[0], 0) == 0.0f) return;
+    if (pos < 0 || pos >= a.S || __shfl_sync(0xffffffffu, l[0], 0) == 0.0f) return;
 #pragma unroll
     for (int i = 1; i >= 0; i--) {
         const unsigned last = __ballot_sync(0xffffffffu, __float_as_uint(l[i]) >> 31);
@@ -1120,15 +1132,8 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
     for (int i = 0; i < 2; i++) f[i] = lane + 32 * i < n ? ex2(m[i] - M) : 0.0f;
     const float L = warp_sum((lane < n ? fabsf(l[0]) * f[0] : 0.0f) + (lane + 32 < n ? fabsf(l[1]) * f[1] : 0.0f));
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int k0 = W == 1 ? 0 : warp; k0 < n; k0 += 4 * W) {  // four parts' loads at a time
-        float v[4][8];
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int k = k0 + u * W;
-                v[u][e] = k < n && lane + 32 * e < Dh ? w[(size_t)k * (Dh + 2) + lane + 32 * e] : 0.0f;
-            }
+    for (int k0 = first; k0 < n; k0 += 4 * W) {
+        if (W == 1 || k0 > first) load(k0, n);
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int k = k0 + u * W;
