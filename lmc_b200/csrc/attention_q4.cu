@@ -34,8 +34,8 @@
 // workspace by k_q4_combine.
 //
 // Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 41 us, 128 ragged
-// sequences of them 79 us (3.6 and 3.9 TB/s), 64 ragged ones of 4 heads of 64
-// dims 18.7 us, one of 12 heads with 700 positions 8.3 us.  Instructions bound
+// sequences of them 78 us (3.7 and 3.9 TB/s), 64 ragged ones of 4 heads of 64
+// dims 18.2 us, one of 12 heads with 700 positions 7.8 us.  Instructions bound
 // the first two (matrix, integer and half instructions share the issue), the
 // latency of a warp's chain (its share, the copies, q, a tile, the merge) the
 // others.
