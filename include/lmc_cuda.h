@@ -200,7 +200,7 @@ unsigned long long lmc_rng_seed(unsigned long long seed);
  * saturate at +-65504) and the code in 0..15 nearest to (x - m) / d, ties to
  * even (decided exactly; all 0 when d is 0).  A group with an infinity or a
  * NaN gets d = NaN: its values read back as NaN.  Such caches start on a
- * 16-byte boundary.  For `batch` sequences
+ * 16-byte boundary and hold at most 2^30 positions a sequence.  For `batch` sequences
  * the caches are batch consecutive [Hkv][S][Dh] slabs and q/k_new/v_new/out
  * are batch rows of H*Dh (q, out) and Hkv*Dh (k_new, v_new) floats.
  * d_pos[b] is the position written this step; positions 0..d_pos[b] are

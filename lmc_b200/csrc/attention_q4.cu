@@ -19,8 +19,8 @@
 // accumulator.  The probabilities are scaled so that p d stays just below
 // 2^15 (the largest exponent of d so far is tracked like the running
 // maximum), so small values keep their relative accuracy.  The matrix unit
-// truncates its sums, so a tile's products go to fresh accumulators that are
-// added to the running ones in rounded fp32.
+// truncates its sums, so a tile's products (and its sums of p and p m') go to
+// fresh accumulators that are added to the running ones in rounded fp32.
 //
 // Work: tiles of 64 positions (32 from head size 160 on) of one (sequence, kv
 // head, 8 query heads).  All tiles of the batch, in order, are divided evenly
@@ -71,7 +71,7 @@ struct Q4Args {
     int batch, vec; // vec: q, new rows and out can be moved 16 bytes at a time
     int bulk;       // every run of rows starts on a 16-byte boundary, four rows are whole 16-byte pieces
     int run;        // rows that lie together: a page's, at most a tile's
-    int page_bytes; // of one kv head's rows of a page
+    long long page_bytes; // of one kv head's rows of a page
 };
 
 template <int NB> struct Q4 {
@@ -242,7 +242,7 @@ template <int NB> __device__ __forceinline__ long long row_offset(const Q4Args &
     const AttnArgs &a = g.a;
     if (!a.pages) return it.off + (long long)t * Q4<NB>::RB;
     const int pg = checked_page(a, __ldg(it.row + (t >> a.page_shift)), ok);
-    return ((long long)pg * a.Hkv + it.kh) * g.page_bytes + (t & ((1 << a.page_shift) - 1)) * Q4<NB>::RB;
+    return ((long long)pg * a.Hkv + it.kh) * g.page_bytes + (long long)(t & ((1 << a.page_shift) - 1)) * Q4<NB>::RB;
 }
 // Starts the copies of a tile's rows, from any 4-byte phase: from the 16-byte
 // boundary at or before the first row; the last copy reads no byte past the run.
@@ -459,28 +459,30 @@ __device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, 
     st.mx = m;
     st.vexp = ve;
     const float2 ff = make_float2(__shfl_sync(0xffffffffu, f, 8 * t), __shfl_sync(0xffffffffu, f, 8 * t + 4));
-    st.l = mul2(st.l, make_float2(f, f));
+    float2 l = make_float2(0.0f, 0.0f);  // (a tile's sums by themselves: small terms would be lost one by one beside a large one)
 #pragma unroll
     for (int h = 0; h < NH; h++)
 #pragma unroll
         for (int par = 0; par < 2; par++) {
             const float2 e = fma2(add2(s[h][par], make_float2(-m, -m)), make_float2(st.qfac, st.qfac), make_float2(up, up));
             s[h][par] = make_float2(ex2(e.x), ex2(e.y));
-            st.l = add2(st.l, s[h][par]);
+            l = add2(l, s[h][par]);
         }
+    st.l = fma2(st.l, make_float2(f, f), l);
 #pragma unroll
     for (int j = 0; j < NG; j++) {
         uint32_t bh[NH][2], bl[NH][2];  // p d of the 16 rows of each set: hi, lo
-        st.om[j] = mul2(st.om[j], make_float2(f, f));
+        float2 om = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int h = 0; h < NH; h++)
 #pragma unroll
             for (int par = 0; par < 2; par++) {
                 const float4 dm = *reinterpret_cast<const float4 *>(vdm + 4 * (2 * (4 * h + t) + par) + 2 * T * j);
                 const float2 w = mul2(s[h][par], make_float2(dm.x, dm.y));
-                st.om[j] = fma2(s[h][par], make_float2(dm.z, dm.w), st.om[j]);
+                om = fma2(s[h][par], make_float2(dm.z, dm.w), om);
                 split2(w.x, w.y, bh[h][par], bl[h][par]);
             }
+        st.om[j] = fma2(st.om[j], make_float2(f, f), om);
         // this lane's dims: word g of the group, or half a word of a group of 32
         const bool half = NB % 2 && j == NG - 1;
         const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
@@ -722,28 +724,30 @@ __device__ __forceinline__ void attend_tile(FewState<NB> &st, const uint8_t *kt,
     const float2 ff = make_float2(f, f);
     st.mx = m;
     st.vexp = ve;
-    st.l *= f;
+    float l = 0.0f;
 #pragma unroll
     for (int h = 0; h < NH; h++)
 #pragma unroll
         for (int r = 0; r < 2; r++) {
             s[h][r] = ex2(fmaf(s[h][r] - m, st.qfac, up));
-            st.l += s[h][r];
+            l += s[h][r];
         }
+    st.l = fmaf(st.l, f, l);
 #pragma unroll
     for (int j = 0; j < NG; j++) {
         uint32_t b[NH][2];  // p d of the 16 rows of each set
-        st.om[j] *= f;
+        float om = 0.0f;
 #pragma unroll
         for (int h = 0; h < NH; h++) {
             const float2 d0 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][0][j])), d1 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][1][j]));
             const float w0 = s[h][0] * d0.x, w1 = s[h][1] * d1.x;
-            st.om[j] = fmaf(s[h][0], fmaf(8.0f, d0.x, d0.y), fmaf(s[h][1], fmaf(8.0f, d1.x, d1.y), st.om[j]));
+            om = fmaf(s[h][0], fmaf(8.0f, d0.x, d0.y), fmaf(s[h][1], fmaf(8.0f, d1.x, d1.y), om));
             uint32_t hi, lo;
             split2(w0, w1, hi, lo);
             b[h][0] = turned(__byte_perm(hi, lo, 0x5410));  // row 2 g: (hi, lo)
             b[h][1] = turned(__byte_perm(hi, lo, 0x7632));  // row 2 g + 1
         }
+        st.om[j] = fmaf(st.om[j], f, om);
         // this lane's dims: word g of the group, or half a word of a group of 32
         const bool half = NB % 2 && j == NG - 1;
         const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
@@ -931,7 +935,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                 if (a.pages) {
                     bool ok;
                     off = ((long long)checked_page(a, a_pg, &ok) * a.Hkv + ia->kh) * g.page_bytes +
-                          ((a_tile * T + r0) & ((1 << a.page_shift) - 1)) * RB;
+                          (long long)((a_tile * T + r0) & ((1 << a.page_shift) - 1)) * RB;
                 } else {
                     off = ia->off + (long long)a_tile * (T * RB);
                 }
@@ -1174,13 +1178,14 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     Q4Args g;
     g.a = *args;
     AttnArgs &a = g.a;
+    if (a.S > 1 << 30) return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: 4-bit rows take contexts of at most 2^30 positions (%d)", a.S);
     // one part per head and workspace slot: the most slots that fit, up to the plan's
     int CH;
     lmc_attn_plan(a.S, batch * a.H, 1, &CH, &a.nsplit);
     const size_t slot = (size_t)batch * a.H * (a.Dh + 2) * sizeof(float);
     if ((size_t)a.nsplit * slot > ws_bytes) a.nsplit = (int)(ws_bytes / slot);
     if (a.nsplit < 2 || !a.ws) a.nsplit = 1;
-    const int G = a.H / a.Hkv, T = q4_tile(a.Dh / 32), NT = (a.S + T - 1) / T;
+    const int G = a.H / a.Hkv, T = q4_tile(a.Dh / 32), NT = (a.S - 1) / T + 1;
     g.G = G;
     g.HG = (G + 7) / 8;
     g.batch = batch;
@@ -1191,7 +1196,7 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     g.rmin = g.items_only ? 1 : NT < 2 ? Q4_ITEM + 1 : std::max((NT - 2) / (a.nsplit - 1) + 1, Q4_ITEM + 1);
     g.vec = (((uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.out) & 15) == 0 && a.ldq % 4 == 0 &&
             a.ldkv % 4 == 0 && a.ldo % 4 == 0;
-    g.page_bytes = kv_q4_row_bytes(a.Dh) << a.page_shift;
+    g.page_bytes = (long long)kv_q4_row_bytes(a.Dh) << a.page_shift;
     g.bulk = a.pages || a.S % 4 == 0;
     g.run = a.pages && (1 << a.page_shift) < T ? 1 << a.page_shift : T;
     const long long units = (long long)batch * a.Hkv * g.HG * (g.items_only ? 1 : NT + Q4_ITEM);

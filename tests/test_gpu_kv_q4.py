@@ -604,6 +604,50 @@ def test_attention_same_result_each_time(cuda):
     assert all(cuda.equal(o, outs[0]) for o in outs)
 
 
+def test_attention_one_page_past_2_gib(cuda):
+    """One page of 2^24 positions, whose rows end past 2^31 bytes.  All rows
+    are zeros (score 0, value 0) but three: one at each end and the new one,
+    their scores around 17 (e^17 is the number of the others), so the output
+    is sum p v over the three, p = e^s / (sum of the three + 2^24 - 3).
+
+    Tolerance: at most 64 workspace slots share an item, so 63 CTAs of four
+    warps have its 2^19 tiles of 32 rows, 2081 a warp.  Each tile's sum of p is
+    added to the warp's with a rounding of at most half a step, 2^-24 of the
+    sum, 2081 * 2^-24 = 1.3e-4 in all (nothing is lost of sum p v, whose other
+    terms are zeros); the rest is below 1e-5 as everywhere."""
+    Dh, P = 256, 1 << 24
+    RB = kv_ref.row_bytes(Dh)
+    rng = np.random.default_rng(14)
+    q = rng.normal(size=(1, Dh)).astype(np.float32)
+    kx = (q * (17.0 * 16 / (q * q).sum()) + 0.05 * rng.normal(size=(3, Dh))).astype(np.float32)
+    vx = rows_of(rng, (3, Dh))
+    (kr, k), (vr, v) = kv_ref.q4_rows(kx), kv_ref.q4_rows(vx)
+    pools = [cuda.zeros((1, 1, P, RB), dtype=cuda.uint8, device="cuda") for _ in range(2)]
+    at = [3, P - 7, P - 1]
+    for pool, r in zip(pools, (kr, vr)):
+        for i in range(2):
+            pool[0, 0, at[i]] = dev(cuda, r[i])
+    out = cuda.full((1, Dh), 5.0, device="cuda")
+    wsb = rt.lib().lmc_attention_workspace_bytes(1, 1, Dh, P)
+    ws = cuda.full((wsb + GUARD,), 0xff, dtype=cuda.uint8, device="cuda")
+    dq, dk, dv = dev(cuda, q), dev(cuda, kx[2:]), dev(cuda, vx[2:])
+    pos, tab, seq = (dev(cuda, np.array([i], np.int32)) for i in (P - 1, 0, 0))
+    rt.call("lmc_attention_decode_paged", out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), pools[0].data_ptr(),
+            pools[1].data_ptr(), rt.KV_Q4, 1, tab.data_ptr(), 1, P, pos.data_ptr(), 1, 1, 1, Dh, ws.data_ptr(), wsb, None)
+    for pool, r in zip(pools, (kr, vr)):
+        assert np.array_equal(pool[0, 0, P - 1].cpu().numpy(), r[2]) and not pool[0, 0, P - 6:P - 1].any()
+        assert not pool[0, 0, 4:1000].any()
+    s = k @ q[0].astype(np.float64) / 16
+    p = np.exp(s)
+    want = p @ v / (p.sum() + P - 3)
+    assert 10 < s.min() and s.max() < 25 and rel_err(out.cpu().numpy()[0], want) < 2081 * 2.0 ** -24 + 1e-5
+    vals = cuda.zeros((1, Dh), device="cuda")
+    rt.call("lmc_kv_read", vals.data_ptr(), None, Dh, pools[0].data_ptr(), None, rt.KV_Q4, seq.data_ptr(), pos.data_ptr(), 1, 1, 1,
+            Dh, P, tab.data_ptr(), P, 1, None)
+    assert rel_err(vals.cpu().numpy(), k[2:]) < 1e-7
+    assert (ws[wsb:] == 0xff).all() and rt.lib().lmc_device_status() == 0
+
+
 def test_attention_offsets_past_32_bits(cuda):
     """A pool of more than 4 GiB: pages near its end hold the sequence."""
     Hkv, Dh, P = 8, 256, 64

@@ -83,6 +83,12 @@ def test_attention_refusals_of_4_bit_caches():
     assert rc == INVALID and b"attention_paged" in msg
 
 
+def test_attention_refuses_contexts_too_long_for_4_bit_rows():
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        rc, msg = status("lmc_attention_decode", P, P, P, P, P, P, rt.KV_Q4, P, 1, 1, 1, 32, n, P, 1 << 40, None)
+        assert rc == UNSUPPORTED and b"2^30" in msg, (rc, msg)
+
+
 def test_page_operator_refusals():
     one = (ctypes.c_void_p * 1)(4096)
     null, odd = (ctypes.c_void_p * 2)(4096, None), (ctypes.c_void_p * 2)(4096, 4104)
