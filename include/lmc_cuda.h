@@ -59,8 +59,7 @@ int lmc_device_status(void);
 
 /* Limit of every bounded wait inside the kernels - the bulk-copy rings of
  * the GEMV, GEMM and 4-bit attention, the grid barriers of the persistent
- * decode step - in
- * nanoseconds; 0 restores the default of one second.  A wait that runs out
+ * decode step - in nanoseconds; 0 restores the default of one second.  A wait that runs out
  * records a timeout that lmc_device_status reports; the kernel drains its
  * own copies and returns, and the context stays usable.  No counterpart in
  * LMc (a CPU program has no device waits). */
@@ -276,10 +275,10 @@ int lmc_attention_decode_paged(float *d_out, const float *d_q, const float *d_k_
  * lmc_attention_decode writes); rows must name distinct positions.
  * lmc_kv_read writes the values the cached rows stand for.  A row whose
  * position is negative is padding: nothing is written for it (d_k and d_v
- * hold `rows` rows all the same, padding among them).  A
- * position >= S, a sequence outside [0, n_seqs) or a page outside
- * [0, n_pages) leaves its row out (nothing is written for it), and
- * lmc_device_status() then reports LMC_ERR_INVALID. */
+ * hold `rows` rows all the same, padding among them).  A position >= S, a
+ * sequence outside [0, n_seqs) or a page outside [0, n_pages) leaves its row
+ * out (nothing is written for it), and lmc_device_status() then reports
+ * LMC_ERR_INVALID. */
 int lmc_kv_append(const float *d_k, const float *d_v, int ld, void *d_k_cache, void *d_v_cache, int kv_dtype,
                   const int *d_seq, const int *d_pos, int rows, int n_seqs, int Hkv, int Dh, int S,
                   const int *d_pages, int page_size, int n_pages, void *stream);
@@ -314,7 +313,8 @@ int lmc_kv_read(float *d_k, float *d_v, int ld, const void *d_k_cache, const voi
  * id first, in order of b.  When fewer are free than needed nothing changes
  * and *d_short receives how many are missing (else 0).  Call it before the
  * step that writes those positions, and do not run that step when *d_short
- * is not 0: it would write into pages that other sequences share.
+ * is not 0: it would write into pages that other sequences share.  At most
+ * 65536 sequences.
  *
  * compact: moves the pages in use to the ids 0 .. *d_n_live - 1 (the i-th
  * page in use above that range, in ascending order, to the i-th free id in

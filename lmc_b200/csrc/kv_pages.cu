@@ -363,7 +363,8 @@ extern "C" int lmc_kv_pages_reserve(void *const *h_pools, int n_pools, size_t pa
     if (rc != LMC_OK) return rc;
     if (!d_pages || !d_refs || !d_pos || !d_short || !d_ws)
         return lmc_set_error(LMC_ERR_INVALID, "kv_pages_reserve: null pointer");
-    if (n_seqs <= 0 || max_pages <= 0 || n_pages <= 0 || n_pages > MAX_PAGES || page_size < 16 || (page_size & (page_size - 1)))
+    // (the plan compares each writer of a shared page with those before it)
+    if (n_seqs <= 0 || n_seqs > 65536 || max_pages <= 0 || n_pages <= 0 || n_pages > MAX_PAGES || page_size < 16 || (page_size & (page_size - 1)))
         return lmc_set_error(LMC_ERR_INVALID, "kv_pages_reserve: %d sequences x %d entries, %d pages of %d positions",
                              n_seqs, max_pages, n_pages, page_size);
     if (ws_bytes < lmc_kv_pages_workspace_bytes(n_seqs, n_pages))

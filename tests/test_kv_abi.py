@@ -112,6 +112,12 @@ def test_page_operator_refusals():
         assert rc == INVALID and word in msg, (args, rc, msg)
 
 
+def test_reserve_of_too_many_sequences_is_refused():
+    one, ws = (ctypes.c_void_p * 1)(4096), rt.lib().lmc_kv_pages_workspace_bytes(65537, 9)
+    rc, msg = status("lmc_kv_pages_reserve", one, 1, 4096, P, 65537, 8, 16, P, 9, P, P, P, ws, None)
+    assert rc == INVALID and b"65537 sequences" in msg, (rc, msg)
+
+
 def test_page_pools_too_large_are_refused():
     one, n = (ctypes.c_void_p * 1)(4096), (1 << 30) + 1
     ws = rt.lib().lmc_kv_pages_workspace_bytes(4, n)
