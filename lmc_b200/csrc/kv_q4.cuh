@@ -20,13 +20,23 @@ __device__ __forceinline__ float kv_min_nan(float a, float b) {
     return r;
 }
 
+// x / 15 rounded to nearest, x in [0, 2^127): the product with the rounded
+// reciprocal is off by at most one step, the FMA's remainder is exact, and
+// adding its share rounds correctly (Markstein's theorem; 15's reciprocal is
+// rounded correctly).  Below 2^-80, where the remainder would underflow, the
+// quotient may be off by a step; as fp16 it is 0 there.
+__device__ __forceinline__ float kv_div15(float x) {
+    const float r = 1.0f / 15.0f, q = x * r;
+    return fmaf(fmaf(-15.0f, q, x), r, q);
+}
+
 // A group's (d, m) word from its minimum (NaN when the group has one) and
 // maximum; d = m = 0 and `bad` when a value is not finite.
 __device__ __forceinline__ uint32_t kv_q4_scale(float lo, float hi, float &d, float &m, bool &bad) {
     bad = !(fabsf(lo) < INFINITY && fabsf(hi) < INFINITY);
     const __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
     m = __half2float(mh);
-    const __half dh = __float2half_rn(fminf(__fdiv_rn(fmaxf(hi - m, 0.0f), 15.0f), 65504.0f));
+    const __half dh = __float2half_rn(fminf(kv_div15(fmaxf(hi - m, 0.0f)), 65504.0f));
     d = __half2float(dh);
     return bad ? 0x7e00u : (uint32_t)__half_as_ushort(dh) | (uint32_t)__half_as_ushort(mh) << 16;
 }

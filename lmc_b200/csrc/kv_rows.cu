@@ -9,7 +9,7 @@
 // 32 lanes per row, eight dims a lane: append takes neighbouring dims (a word
 // of codes, three shuffles for a group's minimum and maximum; 16 bytes of
 // fp16), read two runs of four (stores without gaps).
-// 32000 rows of 8 x 128, append / read: 4-bit 63 / 51 us (4.7 / 5.9 TB/s),
+// 32000 rows of 8 x 128, append / read: 4-bit 61 / 50 us (4.9 / 5.9 TB/s),
 // int8 60 / 54 us, fp16 59 / 61 us (6.7 / 6.4 TB/s); 509 rows of 4 x 64 take
 // 2.9 / 1.8 us in 4 bits, most of it latency.
 #include <type_traits>
