@@ -1,25 +1,22 @@
 // attention_q4.cu - decode attention over 4-bit K/V rows (LMC_KV_Q4).
 //
 // With codes c and (d, m) of group j (64 dims) of row t, and m' = m + 8 d:
-//   s_t = sum_j [ d_tj (q_j . (c_tj - 8)) + m'_tj sum(q_j) ] / sqrt(Dh)
+//   s_t = sum_j [ d_tj (q_j . c_tj) + m_tj sum(q_j) ] / sqrt(Dh)
 //   o_j = sum_t p_t d_tj (c_tj - 8) + sum_t p_t m'_tj,   p_t = 2^(s_t log2 e - max)
-// so the tensor cores only ever see whole numbers and fp32 factors; the
-// scales are applied per group outside (keys) or folded into the
-// probabilities (values).  Codes are centred because a sum of p d c over
-// positive codes would be large against the result of a long, flat softmax
-// and take its rounding with it.
+// so the matrix units only ever see whole numbers and fp32 factors; the scales
+// are applied per group outside (keys) or folded into the probabilities
+// (values).  Keys: integer products, q as whole numbers of 23 bits in three
+// signed bytes.  Values: codes centred, because a sum of p d c over positive
+// codes would be large against the result of a long, flat softmax and take its
+// rounding with it.
 //
-// A code as fp16: a nibble ORed into the low bits of 1024.0 is 1024 + c,
-// exactly, and 1032 less is c - 8 (two instructions for two operands); the
-// nibble above it gives 16 (c - 8), and the 16 goes into q (keys) or the
-// final factor (values).  fp32 factors become an fp16 pair hi + lo (22
-// bits): q, scaled by a power of two into fp16's range, with hi in rows 0-7
-// of the 16 x 16 operand (8 query heads) and lo in rows 8-15, so the padding
-// that 8 heads leave carries the low part; p d as two products into one
-// accumulator.  The probabilities are scaled so that p d stays just below
-// 2^15 (the largest exponent of d so far is tracked like the running
-// maximum), so small values keep their relative accuracy.  The matrix unit
-// truncates its sums, so a tile's products (and its sums of p and p m') go to
+// A value's code as fp16: a nibble ORed into the low bits of 1024.0 is 1024 +
+// c, exactly, and 1032 less is c - 8 (two instructions for two operands); the
+// nibble above it gives 16 (c - 8), and the 16 goes into the final factor.
+// p d becomes an fp16 pair hi + lo (22 bits).  The probabilities are scaled so
+// that p d stays just below 2^15 (the largest exponent of d so far is tracked
+// like the running maximum), so small values keep their relative accuracy.
+// The matrix unit truncates its sums, so a tile's products (and its sums of p and p m') go to
 // fresh accumulators that are added to the running ones in rounded fp32.
 //
 // Work: tiles of 64 positions (32 from head size 160 on) of one (sequence, kv
@@ -34,8 +31,8 @@
 // workspace by k_q4_combine.
 //
 // Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 41 us, 128 ragged
-// sequences of them 78 us (3.7 and 3.9 TB/s), 64 ragged ones of 4 heads of 64
-// dims 18.2 us, one of 12 heads with 700 positions 7.8 us.  Instructions bound
+// sequences of them 77 us (3.7 and 4.0 TB/s), 64 ragged ones of 4 heads of 64
+// dims 17.9 us, one of 12 heads with 700 positions 7.5 us.  Instructions bound
 // the first two (matrix, integer and half instructions share the issue), the
 // latency of a warp's chain (its share, the copies, q, a tile, the merge) the
 // others.
@@ -78,9 +75,8 @@ template <int NB> struct Q4 {
     static constexpr int T = q4_tile(NB), DH = 32 * NB, NG = kv_q4_groups(DH), RB = kv_q4_row_bytes(DH);
     static constexpr int SIDE = T * RB + 16;              // a tile's K or V rows, from any 4-byte phase
     static constexpr int STAGE = 2 * SIDE;
-    static constexpr int META = T * NG * 2;               // floats: (d, m') of a tile's rows, one side
     static constexpr int FRESH = (2 * RB + 15) / 16 * 16; // the new K and V rows
-    static constexpr int WARP_BYTES = Q4_STAGES * STAGE + 2 * META * 4 + FRESH;
+    static constexpr int WARP_BYTES = Q4_STAGES * STAGE + FRESH;
     static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, maximum, sum)
     static_assert(Q4_STAGES * STAGE >= 8 * SLOT * 4, "a partial result fits the ring that it is kept in");
 };
@@ -106,18 +102,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long &>(r))
         : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
           "l"(reinterpret_cast<unsigned long long &>(c)));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(r))
-        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(r))
-        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
     return r;
 }
 // x, y as fp16 pairs hi + lo
@@ -280,15 +264,45 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
     }
 }
 
-// What a warp carries through the tiles of one item.
-template <int NB> struct Q4State {
-    uint32_t qa[2 * NB][4];           // q as matrix operands: head g hi, lo, hi, lo
-    float qsum[Q4<NB>::NG], qfac;     // head g: sum(q_j) and the factor of its products (q scaled to fp16's range)
-    float2 o[2 * NB][2];              // dims x heads (see the output below)
-    float2 om[Q4<NB>::NG], l;         // head g, this lane's positions (two sums each): p m', p
-    float mx;                         // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
-    int vexp;                         // largest exponent field of the values' d so far
+// ---------------------------------------------------------------------------
+// A tile.  The positions are the rows of both products: of each 16 rows lane
+// (g, t) holds the scores of rows 2 g and 2 g + 1, and the eight columns are
+//   FEW    (at most four query heads per kv head) two parts of each head, so
+//          columns 2 t, 2 t + 1 belong to head t and none is idle;
+//   else   eight heads, columns 2 t, 2 t + 1 being heads 2 t, 2 t + 1.
+// Scores: codes as bytes (nibbles of a word are two ANDs and a shift), q as
+// 23-bit whole numbers in three signed bytes: integer products, exact, so codes
+// need no centring here.  FEW: two products, columns (top, middle) and (low, 0);
+// else three, one for each byte.
+// Output: p d as fp16 hi, lo, turned to the operand's order with movmatrix.
+// FEW: hi and lo are a head's two columns; else two products.
+// On this chip a warp-level MMA keeps the integer and half pipes from issuing
+// (8 cycles each, measured in one loop with them), so their number counts: FEW
+// has 32 for 32 rows of 128 dims, the other form 56.  4 heads per kv head of
+// 128 dims, the other form against FEW: one sequence of 131072 positions 48.8
+// -> 40.6 us, 128 ragged ones 95.6 -> 77.4; one head (GPT-2, 700 positions) 7.8
+// -> 7.5.  Eight heads would take FEW twice, at 0.83 of the other's time each.
+template <int NB, bool FEW> struct State {
+    static constexpr int HL = FEW ? 1 : 2;  // heads of a lane
+    static constexpr int LP = FEW ? 2 : 3;  // products of q's bytes
+    uint32_t q[LP][NB][2];                  // q as matrix operands
+    float qsum[Q4<NB>::NG][HL], qfac[HL];   // sums of the whole numbers, the factor of their products
+    float2 o[2 * NB][2];                    // dims x this lane's two columns
+    float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p m', sum p
+    float mx[HL];                           // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
+    int vexp;                               // largest exponent field of the values' d so far
 };
+
+__device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t x) {  // 8 x 8 halves of the warp, transposed
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
 // This lane's values of query `head` of the item's kv head (0 for heads past the last one).
 template <int NB> __device__ __forceinline__ void fetch_q(const Q4Args &g, const Item &p, int lane, int head, float (&x)[NB][8]) {
@@ -299,15 +313,17 @@ template <int NB> __device__ __forceinline__ void fetch_q(const Q4Args &g, const
         if (head < g.G) load8(g.a.q + (size_t)p.b * g.a.ldq + ((size_t)p.kh * g.G + head) * Q4<NB>::DH + 32 * i + 8 * (lane & 3), g.vec, x[i]);
     }
 }
-template <int NB> __device__ __forceinline__ int q_head(const Q4Args &g, const Item &p, int lane, const Q4State<NB> &) {
-    return (p.j - p.kh * g.HG) * 8 + (lane >> 2);
+// Lane (n, t) makes column n's operand: FEW: head n / 2, n odd: the middle byte (and 0), even: the top (and low) one.
+template <int NB, bool FEW> __device__ __forceinline__ int q_head(const Q4Args &g, const Item &p, int lane) {
+    return FEW ? lane >> 3 : (p.j - p.kh * g.HG) * 8 + (lane >> 2);
 }
-
-template <int NB>
-__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], Q4State<NB> &st) {
+template <int NB, bool FEW>
+__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], State<NB, FEW> &st) {
+    using S = State<NB, FEW>;
     const AttnArgs &a = g.a;
-    constexpr int DH = Q4<NB>::DH;
+    constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
     const int t = lane & 3;
+    const bool odd = lane & 4;
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
@@ -317,34 +333,53 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
     }
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // a power of two that brings the largest |q| into [2^12, 2^13)
+    // a power of two that brings the head's largest |q| into [2^21, 2^22): three signed bytes hold it
     const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
-    const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
-    const float scale = LOG2E / sqrtf((float)DH);
-    st.qfac = scale * __uint_as_float((uint32_t)(127 - 12 + ex) << 23);
+    const float up = __uint_as_float((uint32_t)(127 + 21 - ex) << 23);
+    float sum[NG];
 #pragma unroll
-    for (int i = 0; i < Q4<NB>::NG; i++) st.qsum[i] = 0.0f;
+    for (int j = 0; j < NG; j++) sum[j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
+        uint32_t byte[3][2] = {};  // top, middle, low; each 128 more
         float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) s = fmaf(x[i][e], up, s);
+        for (int e = 0; e < 8; e++) {  // dims 0, 2, 4, 6 of the word: its low nibbles; 1, 3, 5, 7: its high ones
+            const float y = rintf(x[i][e] * up);
+            s += y;  // (a value that is not finite makes the sum, and with it the score, NaN or infinite)
+            const uint32_t b = (uint32_t)__float2int_rn(y) + 0x808080u;
+#pragma unroll
+            for (int k = 0; k < 3; k++) byte[k][e & 1] |= (b >> (16 - 8 * k) & 0xffu) << (8 * (e >> 1));
+        }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        st.qsum[i / 2] += s;
-        // nibbles (0, 4) and (2, 6) of a word meet slice 2 i, (1, 5) and (3, 7), 16 times as large, slice 2 i + 1
-        const float dn = up * 0.0625f;
-        split2(x[i][0] * up, x[i][4] * up, st.qa[2 * i][0], st.qa[2 * i][1]);
-        split2(x[i][2] * up, x[i][6] * up, st.qa[2 * i][2], st.qa[2 * i][3]);
-        split2(x[i][1] * dn, x[i][5] * dn, st.qa[2 * i + 1][0], st.qa[2 * i + 1][1]);
-        split2(x[i][3] * dn, x[i][7] * dn, st.qa[2 * i + 1][2], st.qa[2 * i + 1][3]);
+        sum[i / 2] += s;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (FEW) {
+                st.q[0][i][k] = (odd ? byte[1][k] : byte[0][k]) ^ 0x80808080u;
+                st.q[1][i][k] = odd ? 0u : byte[2][k] ^ 0x80808080u;
+            } else {
+#pragma unroll
+                for (int b = 0; b < S::LP; b++) st.q[b][i][k] = byte[b][k] ^ 0x80808080u;
+            }
+        }
+    }
+    // lane (g, t) goes on with the heads of columns 2 t (and 2 t + 1)
+    const float fac = LOG2E / sqrtf((float)DH) * __uint_as_float((uint32_t)(127 - 21 + ex) << 23);
+#pragma unroll
+    for (int hl = 0; hl < S::HL; hl++) {
+        st.qfac[hl] = __shfl_sync(0xffffffffu, fac, 8 * t + 4 * hl);
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            st.qsum[j][hl] = __shfl_sync(0xffffffffu, sum[j], 8 * t + 4 * hl);
+            st.om[j][hl] = 0.0f;
+        }
+        st.l[hl] = 0.0f;
+        st.mx[hl] = -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < Q4<NB>::NG; i++) st.om[i] = make_float2(0.0f, 0.0f);
-    st.l = make_float2(0.0f, 0.0f);
-    st.mx = -INFINITY;
     st.vexp = 0;
 }
 
@@ -379,279 +414,6 @@ template <int NB> __device__ __forceinline__ void append(const Q4Args &g, const 
     }
 }
 
-// One tile: n valid rows at kt / vt (row r at r * RB); kdm, vdm: this warp's
-// (d, m') floats.  Of each 16 rows (h) lane (g, t) holds the scores of head g
-// at rows 4 t + 2 e + par, as pairs over e: matrix columns then are rows 2 g
-// + par (QK) and 4 t + (0, 2 | 1, 3) (PV), which lie in different banks.  The
-// factors of a pair of rows are one 16-byte word: d, d, m', m'.
-template <int NB>
-__device__ __forceinline__ void attend_tile(Q4State<NB> &st, const uint8_t *kt, const uint8_t *vt, float *kdm, float *vdm, int n, int lane) {
-    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, DH = Q4<NB>::DH, T = Q4<NB>::T, NH = T / 16;
-    const int gq = lane >> 2, t = lane & 3;
-    // factors of rows `lane`, lane + 32; rows past the end: d = m' = 0
-    uint32_t dmax = 0;
-#pragma unroll
-    for (int r = 0; r < T; r += 32) {
-        const int to = 4 * ((lane >> 1 & 14) | (lane & 1)) + (lane >> 1 & 1) + 2 * r;
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            uint32_t kw = *reinterpret_cast<const uint32_t *>(kt + (r + lane) * RB + DH / 2 + 4 * j);
-            uint32_t vw = *reinterpret_cast<const uint32_t *>(vt + (r + lane) * RB + DH / 2 + 4 * j);
-            if (r + lane >= n) kw = vw = 0u;
-            const float2 kf = __half22float2(*reinterpret_cast<const __half2 *>(&kw));
-            const float2 vf = __half22float2(*reinterpret_cast<const __half2 *>(&vw));
-            kdm[to + 2 * T * j] = kf.x;
-            kdm[to + 2 * T * j + 2] = fmaf(8.0f, kf.x, kf.y);
-            vdm[to + 2 * T * j] = vf.x;
-            vdm[to + 2 * T * j + 2] = fmaf(8.0f, vf.x, vf.y);
-            dmax = max(dmax, vw & 0xffffu);
-        }
-    }
-    const int vexp = min((int)(__reduce_max_sync(0xffffffffu, dmax) >> 10), 30);
-    __syncwarp();
-    // scores over qfac, group by group; four column sets at a time are independent chains of products
-    float2 s[NH][2];  // [16 rows][par]
-    const uint32_t *const kr = reinterpret_cast<const uint32_t *>(kt + 2 * gq * RB) + t;
-#pragma unroll
-    for (int h0 = 0; h0 < NH; h0 += 2) {
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            float c[4][4];
-#pragma unroll
-            for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
-#pragma unroll
-                for (int hp = 0; hp < 4; hp++) {
-                    uint32_t w[4];
-                    codes8(kr[(16 * (h0 + (hp >> 1)) + (hp & 1)) * (RB / 4) + 4 * i], w);
-                    if (i % 2) hmma(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
-                    else hmma0(c[hp], st.qa[2 * i][0], st.qa[2 * i][1], st.qa[2 * i][2], st.qa[2 * i][3], w[0], w[2]);
-                    hmma(c[hp], st.qa[2 * i + 1][0], st.qa[2 * i + 1][1], st.qa[2 * i + 1][2], st.qa[2 * i + 1][3], w[1], w[3]);
-                }
-            }
-#pragma unroll
-            for (int hp = 0; hp < 4; hp++) {  // columns 2 t, 2 t + 1: rows 4 t + par, 4 t + 2 + par
-                const int h = h0 + (hp >> 1), par = hp & 1;
-                const float4 dm = *reinterpret_cast<const float4 *>(kdm + 4 * (2 * (4 * h + t) + par) + 2 * T * j);
-                const float2 d = make_float2(dm.x, dm.y), m = make_float2(dm.z, dm.w);
-                const float2 x = add2(make_float2(c[hp][0], c[hp][1]), make_float2(c[hp][2], c[hp][3]));
-                s[h][par] = j ? fma2(d, x, s[h][par]) : mul2(d, x);
-                s[h][par] = fma2(m, make_float2(st.qsum[j], st.qsum[j]), s[h][par]);
-            }
-        }
-    }
-    if (n < T)
-#pragma unroll
-        for (int h = 0; h < NH; h++)
-#pragma unroll
-            for (int par = 0; par < 2; par++) {
-                if (16 * h + 4 * t + par >= n) s[h][par].x = -INFINITY;
-                if (16 * h + 4 * t + 2 + par >= n) s[h][par].y = -INFINITY;
-            }
-    // running maximum of head g and exponent of the values' scales
-    float m = -INFINITY;
-#pragma unroll
-    for (int h = 0; h < NH; h++) m = fmaxf(m, fmaxf(fmaxf(s[h][0].x, s[h][0].y), fmaxf(s[h][1].x, s[h][1].y)));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = fmaxf(m, st.mx);
-    const int ve = max(vexp, st.vexp);
-    const float up = (float)(29 - ve), f = ex2(fmaf(st.mx - m, st.qfac, (float)(st.vexp - ve)));  // (2^-inf = 0 the first time)
-    st.mx = m;
-    st.vexp = ve;
-    const float2 ff = make_float2(__shfl_sync(0xffffffffu, f, 8 * t), __shfl_sync(0xffffffffu, f, 8 * t + 4));
-    float2 l = make_float2(0.0f, 0.0f);  // (a tile's sums by themselves: small terms would be lost one by one beside a large one)
-#pragma unroll
-    for (int h = 0; h < NH; h++)
-#pragma unroll
-        for (int par = 0; par < 2; par++) {
-            const float2 e = fma2(add2(s[h][par], make_float2(-m, -m)), make_float2(st.qfac, st.qfac), make_float2(up, up));
-            s[h][par] = make_float2(ex2(e.x), ex2(e.y));
-            l = add2(l, s[h][par]);
-        }
-    st.l = fma2(st.l, make_float2(f, f), l);
-#pragma unroll
-    for (int j = 0; j < NG; j++) {
-        uint32_t bh[NH][2], bl[NH][2];  // p d of the 16 rows of each set: hi, lo
-        float2 om = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int h = 0; h < NH; h++)
-#pragma unroll
-            for (int par = 0; par < 2; par++) {
-                const float4 dm = *reinterpret_cast<const float4 *>(vdm + 4 * (2 * (4 * h + t) + par) + 2 * T * j);
-                const float2 w = mul2(s[h][par], make_float2(dm.x, dm.y));
-                om = fma2(s[h][par], make_float2(dm.z, dm.w), om);
-                split2(w.x, w.y, bh[h][par], bl[h][par]);
-            }
-        st.om[j] = fma2(st.om[j], make_float2(f, f), om);
-        // this lane's dims: word g of the group, or half a word of a group of 32
-        const bool half = NB % 2 && j == NG - 1;
-        const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
-#pragma unroll
-        for (int k = 0; k < (half ? 1 : 2); k++) {  // nibbles 0-3, 4-7 of the words (or the half word's four)
-            const uint32_t sel = half ? ((gq & 1) ? 0x7632u : 0x5410u) : (k ? 0x7632u : 0x5410u);
-            const int i = 4 * j + 2 * k;
-            float c[2][4];
-#pragma unroll
-            for (int h = 0; h < NH; h++) {
-                uint32_t cw[4], x[4], y[4];  // rows 4 t + (0, 2) and (1, 3)
-#pragma unroll
-                for (int r = 0; r < 4; r++) cw[r] = *reinterpret_cast<const uint32_t *>(vr + (16 * h + r) * RB);
-                codes8(__byte_perm(cw[0], cw[2], sel), x);
-                codes8(__byte_perm(cw[1], cw[3], sel), y);
-                if (h) {
-                    hmma(c[0], x[0], x[1], y[0], y[1], bh[h][0], bh[h][1]);
-                    hmma(c[1], x[2], x[3], y[2], y[3], bh[h][0], bh[h][1]);
-                } else {
-                    hmma0(c[0], x[0], x[1], y[0], y[1], bh[h][0], bh[h][1]);
-                    hmma0(c[1], x[2], x[3], y[2], y[3], bh[h][0], bh[h][1]);
-                }
-                hmma(c[0], x[0], x[1], y[0], y[1], bl[h][0], bl[h][1]);
-                hmma(c[1], x[2], x[3], y[2], y[3], bl[h][0], bl[h][1]);
-            }
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                st.o[i + e][0] = fma2(st.o[i + e][0], ff, make_float2(c[e][0], c[e][1]));
-                st.o[i + e][1] = fma2(st.o[i + e][1], ff, make_float2(c[e][2], c[e][3]));
-            }
-        }
-    }
-}
-
-// The item's result over its tiles so far, to dst + h * ld (heads h < heads
-// of the group of 8): with fin divided by the sum; else the sums themselves,
-// with the maximum of s and the sum of p behind them.  Lane (g, t) holds heads 2 t and 2 t + 1,
-// dims 8 g .. 8 g + 7 of each group of 64 (4 g .. 4 g + 3 of one of 32).
-template <int NB>
-__device__ __forceinline__ void result(const Q4State<NB> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
-    const int gq = lane >> 2, t = lane & 3;
-    const float down = __uint_as_float((uint32_t)(127 - 29 + st.vexp) << 23);  // takes the probabilities' 2^(29 - vexp) back
-    float l = st.l.x + st.l.y;
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (!fin && t == 0 && gq < heads) {
-        dst[gq * ld + Q4<NB>::DH] = st.mx * st.qfac;
-        dst[gq * ld + Q4<NB>::DH + 1] = l * down;
-    }
-    const float inv = fin ? 1.0f / l : down;
-#pragma unroll
-    for (int hd = 0; hd < 2; hd++) {
-        const int from = 8 * t + 4 * hd, h = 2 * t + hd;
-        const float iv = __shfl_sync(0xffffffffu, inv, from);
-#pragma unroll
-        for (int j = 0; j < Q4<NB>::NG; j++) {
-            float m = st.om[j].x + st.om[j].y;
-            m += __shfl_xor_sync(0xffffffffu, m, 1);
-            m += __shfl_xor_sync(0xffffffffu, m, 2);
-            m = __shfl_sync(0xffffffffu, m, from);
-            const bool half = NB % 2 && j == Q4<NB>::NG - 1;
-#pragma unroll
-            for (int k = 0; k < (half ? 1 : 2); k++) {
-                const float2 *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];  // (pairs over the heads)
-                const float4 v = make_float4(((hd ? a[0].y : a[0].x) + m) * iv, fmaf(hd ? a[1].y : a[1].x, 0.0625f, m) * iv,
-                                             ((hd ? b[0].y : b[0].x) + m) * iv, fmaf(hd ? b[1].y : b[1].x, 0.0625f, m) * iv);
-                float *o = dst + h * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
-                if (h >= heads) continue;
-                if (vec) *reinterpret_cast<float4 *>(o) = v;
-                else { o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w; }
-            }
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------
-// At most four query heads per kv head: the same tile with half the matrix
-// work and no idle columns.  The positions are the rows of both products, so
-// columns 2 t, 2 t + 1 of 8 can be two parts of one head t, and lane (g, t) has
-// head t's scores of rows 2 g and 2 g + 1 of each 16.
-//   scores  codes as bytes (nibbles of a word are two ANDs and a shift), q as
-//           23-bit whole numbers in three signed bytes (columns: top, middle |
-//           low, 0): integer products, exact, so codes need no centring here;
-//   output  p d as fp16 hi, lo in columns 2 t, 2 t + 1, turned to the operand's
-//           order with movmatrix.
-// On this chip a warp-level MMA keeps the integer and half pipes from issuing
-// (8 cycles each, measured in one loop with them), so their number counts: 32
-// for 32 rows of 128 dims against 64.  4 heads per kv head of 128 dims, the
-// other form against this one: one sequence of 131072 positions 52 -> 41 us
-// (3.6 TB/s), 128 ragged ones 101 -> 79 us (3.9 TB/s); one head (GPT-2, 700
-// positions) 8.4 -> 8.3 us.  Eight heads would take this form twice, at 0.8 of the
-// other's time each, so more than four heads take the other one.
-template <int NB> struct FewState {
-    uint32_t qt[NB][2], ql[NB][2];    // q as matrix operands: columns top / middle, low / 0
-    float qsum[Q4<NB>::NG], qfac;     // head t: sums of the whole numbers, the factor of their products
-    float2 o[2 * NB][2];              // dims x (hi, lo) of head t
-    float om[Q4<NB>::NG], l;          // head t, this lane's positions: sum p m', sum p
-    float mx;                         // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
-    int vexp;                         // largest exponent field of the values' d so far
-};
-
-__device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t turned(uint32_t x) {  // 8 x 8 halves of the warp, transposed
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
-// Lane (n, t) makes column n's operand: head n / 2, n odd: the middle byte (and 0), even: the top (and low) one.
-template <int NB> __device__ __forceinline__ int q_head(const Q4Args &, const Item &, int lane, const FewState<NB> &) { return lane >> 3; }
-template <int NB>
-__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], FewState<NB> &st) {
-    const AttnArgs &a = g.a;
-    constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
-    const int t = lane & 3;
-    const bool odd = lane & 4;
-    float big = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
-#pragma unroll
-        for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[i][e]));
-    }
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // a power of two that brings the head's largest |q| into [2^21, 2^22): three signed bytes hold it
-    const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
-    const float up = __uint_as_float((uint32_t)(127 + 21 - ex) << 23);
-    float sum[NG];
-#pragma unroll
-    for (int j = 0; j < NG; j++) sum[j] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {  // dims 0, 2, 4, 6 of the word: its low nibbles; 1, 3, 5, 7: its high ones
-            const float y = rintf(x[i][e] * up);
-            s += y;  // (a value that is not finite makes the sum, and with it the score, NaN or infinite)
-            const uint32_t b = (uint32_t)__float2int_rn(y) + 0x808080u;  // the bytes, each 128 more
-            hi[e & 1] |= ((odd ? b >> 8 : b >> 16) & 0xffu) << (8 * (e >> 1));
-            lo[e & 1] |= (b & 0xffu) << (8 * (e >> 1));
-        }
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        sum[i / 2] += s;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            st.qt[i][k] = hi[k] ^ 0x80808080u;
-            st.ql[i][k] = odd ? 0u : lo[k] ^ 0x80808080u;
-        }
-    }
-    // lane (g, t) goes on with head t, held by the lanes (2 t, ...)
-    st.qfac = __shfl_sync(0xffffffffu, LOG2E / sqrtf((float)DH) * __uint_as_float((uint32_t)(127 - 21 + ex) << 23), 8 * t);
-#pragma unroll
-    for (int j = 0; j < NG; j++) st.qsum[j] = __shfl_sync(0xffffffffu, sum[j], 8 * t);
-#pragma unroll
-    for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int j = 0; j < NG; j++) st.om[j] = 0.0f;
-    st.l = 0.0f;
-    st.mx = -INFINITY;
-    st.vexp = 0;
-}
-
 // The (d, m) words of row r.
 template <int NB> __device__ __forceinline__ void row_factors(const uint8_t *rows, int r, uint32_t (&w)[Q4<NB>::NG]) {
     constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, DH = Q4<NB>::DH;
@@ -669,33 +431,40 @@ template <int NB> __device__ __forceinline__ void row_factors(const uint8_t *row
     }
 }
 
-template <int NB>
-__device__ __forceinline__ void attend_tile(FewState<NB> &st, const uint8_t *kt, const uint8_t *vt, float *, float *, int n, int lane) {
-    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, T = Q4<NB>::T, NH = T / 16;
+// One tile: n valid rows at kt / vt (row r at r * RB).
+template <int NB, bool FEW>
+__device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *kt, const uint8_t *vt, int n, int lane) {
+    using S = State<NB, FEW>;
+    constexpr int RB = Q4<NB>::RB, NG = Q4<NB>::NG, T = Q4<NB>::T, NH = T / 16, HL = S::HL;
     const int gq = lane >> 2, t = lane & 3;
-    float s[NH][2];  // scores over qfac of rows 16 h + 2 g, + 1
+    float s[NH][2][HL];  // scores over qfac of rows 16 h + 2 g, + 1
 #pragma unroll
     for (int h = 0; h < NH; h++) {
         const uint32_t *const k0 = reinterpret_cast<const uint32_t *>(kt + (16 * h + 2 * gq) * RB) + t, *const k1 = k0 + RB / 4;
-        uint32_t f0[NG], f1[NG];
-        row_factors<NB>(kt, 16 * h + 2 * gq, f0);
-        row_factors<NB>(kt, 16 * h + 2 * gq + 1, f1);
+        uint32_t f[2][NG];
+        row_factors<NB>(kt, 16 * h + 2 * gq, f[0]);
+        row_factors<NB>(kt, 16 * h + 2 * gq + 1, f[1]);
 #pragma unroll
         for (int j = 0; j < NG; j++) {
-            int ct[4] = {0, 0, 0, 0}, cl[4] = {0, 0, 0, 0};
+            int c[S::LP][4] = {};
 #pragma unroll
             for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
                 const uint32_t w0 = k0[4 * i], w1 = k1[4 * i];
                 const uint32_t a0 = w0 & 0x0f0f0f0fu, a1 = w1 & 0x0f0f0f0fu, a2 = w0 >> 4 & 0x0f0f0f0fu, a3 = w1 >> 4 & 0x0f0f0f0fu;
-                imma(ct, a0, a1, a2, a3, st.qt[i][0], st.qt[i][1]);
-                imma(cl, a0, a1, a2, a3, st.ql[i][0], st.ql[i][1]);
+#pragma unroll
+                for (int b = 0; b < S::LP; b++) imma(c[b], a0, a1, a2, a3, st.q[b][i][0], st.q[b][i][1]);
             }
-            // 2^16 top + 2^8 middle + low: the first two together are below 2^24, exact in fp32
-            const float x0 = fmaf((float)(ct[0] * 256 + ct[1]), 256.0f, (float)cl[0]);
-            const float x1 = fmaf((float)(ct[2] * 256 + ct[3]), 256.0f, (float)cl[2]);
-            const float2 d0 = __half22float2(*reinterpret_cast<const __half2 *>(&f0[j])), d1 = __half22float2(*reinterpret_cast<const __half2 *>(&f1[j]));
-            s[h][0] = fmaf(d0.y, st.qsum[j], j ? fmaf(d0.x, x0, s[h][0]) : d0.x * x0);
-            s[h][1] = fmaf(d1.y, st.qsum[j], j ? fmaf(d1.x, x1, s[h][1]) : d1.x * x1);
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const float2 d = __half22float2(*reinterpret_cast<const __half2 *>(&f[r][j]));
+#pragma unroll
+                for (int hl = 0; hl < HL; hl++) {
+                    // 2^16 top + 2^8 middle + low: the first two together are below 2^24, exact in fp32
+                    const int top = c[0][2 * r + hl], mid = FEW ? c[0][2 * r + 1] : c[1][2 * r + hl], low = c[S::LP - 1][2 * r + hl];
+                    const float x = fmaf((float)(top * 256 + mid), 256.0f, (float)low);
+                    s[h][r][hl] = fmaf(d.y, st.qsum[j][hl], j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
+                }
+            }
         }
     }
     uint32_t vf[NH][2][NG];  // (d, m) words of the values' rows
@@ -706,48 +475,67 @@ __device__ __forceinline__ void attend_tile(FewState<NB> &st, const uint8_t *kt,
         for (int r = 0; r < 2; r++) {
             row_factors<NB>(vt, 16 * h + 2 * gq + r, vf[h][r]);
             if (16 * h + 2 * gq + r >= n) {  // past the end
-                s[h][r] = -INFINITY;
+#pragma unroll
+                for (int hl = 0; hl < HL; hl++) s[h][r][hl] = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < NG; j++) vf[h][r][j] = 0u;
             }
 #pragma unroll
             for (int j = 0; j < NG; j++) dmax = max(dmax, vf[h][r][j] & 0xffffu);
         }
+    // running maximum and exponent of the values' scales
     const int ve = max(min((int)(__reduce_max_sync(0xffffffffu, dmax) >> 10), 30), st.vexp);
-    float m = fmaxf(s[0][0], s[0][1]);
+    const float up = (float)(29 - ve);
+    float f[HL];
 #pragma unroll
-    for (int h = 1; h < NH; h++) m = fmaxf(m, fmaxf(s[h][0], s[h][1]));
+    for (int hl = 0; hl < HL; hl++) {
+        float m = fmaxf(s[0][0][hl], s[0][1][hl]);
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    m = fmaxf(m, st.mx);
-    const float up = (float)(29 - ve), f = ex2(fmaf(st.mx - m, st.qfac, (float)(st.vexp - ve)));  // (2^-inf = 0 the first time)
-    const float2 ff = make_float2(f, f);
-    st.mx = m;
+        for (int h = 1; h < NH; h++) m = fmaxf(m, fmaxf(s[h][0][hl], s[h][1][hl]));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = fmaxf(m, st.mx[hl]);
+        f[hl] = ex2(fmaf(st.mx[hl] - m, st.qfac[hl], (float)(st.vexp - ve)));  // (2^-inf = 0 the first time)
+        st.mx[hl] = m;
+        float l = 0.0f;  // (a tile's sums by themselves: small terms would be lost one by one beside a large one)
+#pragma unroll
+        for (int h = 0; h < NH; h++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                s[h][r][hl] = ex2(fmaf(s[h][r][hl] - m, st.qfac[hl], up));
+                l += s[h][r][hl];
+            }
+        st.l[hl] = fmaf(st.l[hl], f[hl], l);
+    }
+    const float2 ff = make_float2(f[0], f[HL - 1]);
     st.vexp = ve;
-    float l = 0.0f;
-#pragma unroll
-    for (int h = 0; h < NH; h++)
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            s[h][r] = ex2(fmaf(s[h][r] - m, st.qfac, up));
-            l += s[h][r];
-        }
-    st.l = fmaf(st.l, f, l);
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        uint32_t b[NH][2];  // p d of the 16 rows of each set
-        float om = 0.0f;
+        constexpr int PB = FEW ? 1 : 2;  // products of p d
+        uint32_t b[NH][PB][2];           // p d of the 16 rows of each set: rows 2 g, 2 g + 1
+        float om[HL] = {};
 #pragma unroll
         for (int h = 0; h < NH; h++) {
             const float2 d0 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][0][j])), d1 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][1][j]));
-            const float w0 = s[h][0] * d0.x, w1 = s[h][1] * d1.x;
-            om = fmaf(s[h][0], fmaf(8.0f, d0.x, d0.y), fmaf(s[h][1], fmaf(8.0f, d1.x, d1.y), om));
+            const float m0 = fmaf(8.0f, d0.x, d0.y), m1 = fmaf(8.0f, d1.x, d1.y);
+#pragma unroll
+            for (int hl = 0; hl < HL; hl++) om[hl] = fmaf(s[h][0][hl], m0, fmaf(s[h][1][hl], m1, om[hl]));
             uint32_t hi, lo;
-            split2(w0, w1, hi, lo);
-            b[h][0] = turned(__byte_perm(hi, lo, 0x5410));  // row 2 g: (hi, lo)
-            b[h][1] = turned(__byte_perm(hi, lo, 0x7632));  // row 2 g + 1
+            if (FEW) {
+                split2(s[h][0][0] * d0.x, s[h][1][0] * d1.x, hi, lo);
+                b[h][0][0] = turned(__byte_perm(hi, lo, 0x5410));  // row 2 g: (hi, lo)
+                b[h][0][1] = turned(__byte_perm(hi, lo, 0x7632));
+            } else {
+                split2(s[h][0][0] * d0.x, s[h][0][HL - 1] * d0.x, hi, lo);  // row 2 g: both heads
+                b[h][0][0] = turned(hi);
+                b[h][PB - 1][0] = turned(lo);
+                split2(s[h][1][0] * d1.x, s[h][1][HL - 1] * d1.x, hi, lo);
+                b[h][0][1] = turned(hi);
+                b[h][PB - 1][1] = turned(lo);
+            }
         }
-        st.om[j] = fmaf(st.om[j], f, om);
+#pragma unroll
+        for (int hl = 0; hl < HL; hl++) st.om[j][hl] = fmaf(st.om[j][hl], f[hl], om[hl]);
         // this lane's dims: word g of the group, or half a word of a group of 32
         const bool half = NB % 2 && j == NG - 1;
         const uint8_t *vr = vt + 4 * t * RB + 32 * j + (half ? 4 * (gq >> 1) : 4 * gq);
@@ -763,12 +551,15 @@ __device__ __forceinline__ void attend_tile(FewState<NB> &st, const uint8_t *kt,
                 for (int r = 0; r < 4; r++) cw[r] = *reinterpret_cast<const uint32_t *>(vr + (16 * h + r) * RB);
                 codes8(__byte_perm(cw[0], cw[2], sel), x);
                 codes8(__byte_perm(cw[1], cw[3], sel), y);
-                if (h) {
-                    hmma(c[0], x[0], x[1], y[0], y[1], b[h][0], b[h][1]);
-                    hmma(c[1], x[2], x[3], y[2], y[3], b[h][0], b[h][1]);
-                } else {
-                    hmma0(c[0], x[0], x[1], y[0], y[1], b[h][0], b[h][1]);
-                    hmma0(c[1], x[2], x[3], y[2], y[3], b[h][0], b[h][1]);
+#pragma unroll
+                for (int b_ = 0; b_ < PB; b_++) {
+                    if (h || b_) {
+                        hmma(c[0], x[0], x[1], y[0], y[1], b[h][b_][0], b[h][b_][1]);
+                        hmma(c[1], x[2], x[3], y[2], y[3], b[h][b_][0], b[h][b_][1]);
+                    } else {
+                        hmma0(c[0], x[0], x[1], y[0], y[1], b[h][b_][0], b[h][b_][1]);
+                        hmma0(c[1], x[2], x[3], y[2], y[3], b[h][b_][0], b[h][b_][1]);
+                    }
                 }
             }
 #pragma unroll
@@ -780,33 +571,43 @@ __device__ __forceinline__ void attend_tile(FewState<NB> &st, const uint8_t *kt,
     }
 }
 
-template <int NB>
-__device__ __forceinline__ void result(const FewState<NB> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
+// The item's result over its tiles so far, to dst + h * ld (heads h < heads
+// of the group of 8): with fin divided by the sum; else the sums themselves,
+// with the maximum of s and the sum of p behind them.  Lane (g, t) holds its
+// heads' dims 8 g .. 8 g + 7 of each group of 64 (4 g .. 4 g + 3 of one of 32).
+template <int NB, bool FEW>
+__device__ __forceinline__ void result(const State<NB, FEW> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
+    using S = State<NB, FEW>;
     const int gq = lane >> 2, t = lane & 3;
     const float down = __uint_as_float((uint32_t)(127 - 29 + st.vexp) << 23);  // takes the probabilities' 2^(29 - vexp) back
-    float l = st.l;
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (!fin && gq == 0 && t < heads) {
-        dst[t * ld + Q4<NB>::DH] = st.mx * st.qfac;
-        dst[t * ld + Q4<NB>::DH + 1] = l * down;
-    }
-    const float iv = fin ? 1.0f / l : down;
+    for (int hl = 0; hl < S::HL; hl++) {
+        const int h = S::HL * t + hl;
+        float l = st.l[hl];
 #pragma unroll
-    for (int j = 0; j < Q4<NB>::NG; j++) {
-        float m = st.om[j];
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (!fin && gq == 0 && h < heads) {
+            dst[h * ld + Q4<NB>::DH] = st.mx[hl] * st.qfac[hl];
+            dst[h * ld + Q4<NB>::DH + 1] = l * down;
+        }
+        const float iv = fin ? 1.0f / l : down;
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-        const bool half = NB % 2 && j == Q4<NB>::NG - 1;
+        for (int j = 0; j < Q4<NB>::NG; j++) {
+            float m = st.om[j][hl];
 #pragma unroll
-        for (int k = 0; k < (half ? 1 : 2); k++) {
-            const float2 *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
-            const float4 v = make_float4((a[0].x + a[0].y + m) * iv, fmaf(a[1].x + a[1].y, 0.0625f, m) * iv, (b[0].x + b[0].y + m) * iv,
-                                         fmaf(b[1].x + b[1].y, 0.0625f, m) * iv);
-            float *o = dst + t * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
-            if (t >= heads) continue;
-            if (vec) *reinterpret_cast<float4 *>(o) = v;
-            else { o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w; }
+            for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+            const bool half = NB % 2 && j == Q4<NB>::NG - 1;
+#pragma unroll
+            for (int k = 0; k < (half ? 1 : 2); k++) {
+                const float2 *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
+                auto col = [&](const float2 &v) { return FEW ? v.x + v.y : hl ? v.y : v.x; };  // (hi and lo, or the head's)
+                const float4 v = make_float4((col(a[0]) + m) * iv, fmaf(col(a[1]), 0.0625f, m) * iv, (col(b[0]) + m) * iv,
+                                             fmaf(col(b[1]), 0.0625f, m) * iv);
+                float *o = dst + h * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
+                if (h >= heads) continue;
+                if (vec) *reinterpret_cast<float4 *>(o) = v;
+                else { o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w; }
+            }
         }
     }
 }
@@ -865,8 +666,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
     const int cta = blockIdx.x, c0 = cta * per + min(cta, more), cn = per + (cta < more);
     const int wn = cn / Q4_WARPS, wm = cn % Q4_WARPS, u0 = c0 + warp * wn + min(warp, wm), u1 = u0 + wn + (warp < wm);
     uint8_t *const ring = smem + warp * Q4<NB>::WARP_BYTES;
-    float *const kdm = reinterpret_cast<float *>(ring + Q4_STAGES * Q4<NB>::STAGE), *const vdm = kdm + Q4<NB>::META;
-    uint32_t *const fresh = reinterpret_cast<uint32_t *>(vdm + Q4<NB>::META);
+    uint32_t *const fresh = reinterpret_cast<uint32_t *>(ring + Q4_STAGES * Q4<NB>::STAGE);
     float *const slots = reinterpret_cast<float *>(smem + Q4_WARPS * Q4<NB>::WARP_BYTES);  // [warp][GH][SLOT]
     const size_t hstride = (size_t)a.nsplit * (DH + 2);
 
@@ -946,7 +746,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         int tile = p.tile, end = p.end, nt = p.nt, phase = 0, part = 0, stage = 0, fill = 0;
         uint32_t parity = 0, flying = 0;  // phase bits of the stages' barriers; stages whose copies are not waited for
         bool begin = true;
-        std::conditional_t<FEW, FewState<NB>, Q4State<NB>> st;
+        State<NB, FEW> st;
 #pragma unroll 1
         for (int skip = Q4_STAGES - 1; tile < end; skip--) {  // the first turns only start copies
             if (a_tile < a_end) {
@@ -969,9 +769,9 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             if (begin) {
                 phase = g.bulk ? 0 : (int)(ii->off & 15);  // rows lie in the ring at the phase that they have in the cache
                 float x[NB][8];
-                fetch_q<NB>(g, *ii, lane, q_head<NB>(g, *ii, lane, st), x);
+                fetch_q<NB>(g, *ii, lane, q_head<NB, FEW>(g, *ii, lane), x);
                 if (a.append && end == nt) append<NB>(g, *ii, fresh, lane);  // (while q is on its way)
-                load_q<NB>(g, *ii, lane, x, st);
+                load_q<NB, FEW>(g, *ii, lane, x, st);
                 begin = false;
             }
             if (!g.bulk) {
@@ -998,14 +798,14 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                     __syncwarp();
                 }
             }
-            attend_tile<NB>(st, kt, kt + Q4<NB>::SIDE, kdm, vdm, n, lane);
-            __syncwarp();  // the stage and (d, m') are read; they may be written again
+            attend_tile<NB, FEW>(st, kt, kt + Q4<NB>::SIDE, n, lane);
+            __syncwarp();  // the stage is read; it may be written again
             if (++tile == end) {  // the item, or this warp's part of it, ends
                 const int b = ii->b, kh = ii->kh, first = ii->tile;
                 const int h0 = (ii->j - kh * g.HG) * 8, heads = min(8, G - h0), head = kh * G + h0;
                 const bool whole = first == 0 && end == nt;
                 float *slot = part ? reinterpret_cast<float *>(ring) : slots + warp * GH * SLOT;
-                result<NB>(st, lane, whole ? a.out + (size_t)b * a.ldo + (size_t)head * DH : slot, whole ? DH : SLOT, heads, whole, !whole || g.vec);
+                result<NB, FEW>(st, lane, whole ? a.out + (size_t)b * a.ldo + (size_t)head * DH : slot, whole ? DH : SLOT, heads, whole, !whole || g.vec);
                 if (whole) {
                     if (lane < heads && a.nsplit > 1)  // nothing for the combine kernel to do
                         a.ws[((size_t)b * a.H + head + lane) * hstride + DH + 1] = 0.0f;
