@@ -1,23 +1,25 @@
 // attention_q4.cu - decode attention over 4-bit K/V rows (LMC_KV_Q4).
 //
-// With codes c and (d, m) of group j (64 dims) of row t, and m' = m + 8 d:
-//   s_t = sum_j [ d_tj (q_j . c_tj) + m_tj sum(q_j) ] / sqrt(Dh)
-//   o_j = sum_t p_t d_tj (c_tj - 8) + sum_t p_t m'_tj,   p_t = 2^(s_t log2 e - max)
+// With codes c and (d, m) of group j (64 dims) of row t:
+//   s_t = sum_j [ d_tj (q_j . (c_tj - 8)) + (m_tj + 8 d_tj) sum(q_j) ] / sqrt(Dh)
+//   o_j = sum_t p_t d_tj (2 c_tj - 15) / 2 + sum_t p_t (m_tj + 7.5 d_tj),   p_t = 2^(s_t log2 e - max)
 // so the matrix units only ever see whole numbers and fp32 factors; the scales
 // are applied per group outside (keys) or folded into the probabilities
 // (values).  Keys: integer products, q as whole numbers of 23 bits in three
-// signed bytes.  Values: codes centred, because a sum of p d c over positive
-// codes would be large against the result of a long, flat softmax and take its
-// rounding with it.
+// signed bytes.  Codes are centred, because sums over positive codes would be
+// large against the score, and against the result of a long, flat softmax, and
+// take their rounding with them (131072 positions, keys with a few large
+// channels: relative error 1.0e-6, centred in both 0.7e-6, for 4% more time).
 //
-// A value's code as fp16: a nibble ORed into the low bits of 1024.0 is 1024 +
-// c, exactly, and 1032 less is c - 8 (two instructions for two operands); the
-// nibble above it gives 16 (c - 8), and the 16 goes into the final factor.
-// p d becomes an fp16 pair hi + lo (22 bits).  The probabilities are scaled so
-// that p d stays just below 2^15 (the largest exponent of d so far is tracked
-// like the running maximum), so small values keep their relative accuracy.
-// The matrix unit truncates its sums, so a tile's products (and its sums of p and p m') go to
-// fresh accumulators that are added to the running ones in rounded fp32.
+// A value's code as fp16: a nibble ORed into bits 1 to 4 of 1024.0 is 1024 +
+// 2 c, exactly, and 1039 less is 2 c - 15 (two instructions for two operands);
+// the nibble above it gives 16 (2 c - 15), and the 16 goes into the final
+// factor.  p d becomes an fp16 pair hi + lo (22 bits).  The probabilities are
+// scaled so that p d stays just below 2^15 (the largest exponent of d so far is
+// tracked like the running maximum), so small values keep their relative
+// accuracy.  The matrix unit truncates its sums, so a tile's products (and its
+// sums of p and of p with the minima) go to fresh accumulators that are added
+// to the running ones in rounded fp32.
 //
 // Work: tiles of 64 positions (32 from head size 160 on) of one (sequence, kv
 // head, 8 query heads).  All tiles of the batch, in order, are divided evenly
@@ -30,9 +32,9 @@
 // one CTA are merged in shared memory, parts in several CTAs through the
 // workspace by k_q4_combine.
 //
-// Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 41 us, 128 ragged
-// sequences of them 77 us (3.7 and 4.0 TB/s), 64 ragged ones of 4 heads of 64
-// dims 17.9 us, one of 12 heads with 700 positions 7.5 us.  Instructions bound
+// Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 42 us, 128 ragged
+// sequences of them 81 us (3.6 and 3.8 TB/s), 64 ragged ones of 4 heads of 64
+// dims 18.0 us, one of 12 heads with 700 positions 7.5 us.  Instructions bound
 // the first two (matrix, integer and half instructions share the issue), the
 // latency of a warp's chain (its share, the copies, q, a tile, the merge) the
 // others.
@@ -141,7 +143,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const uint8_t *src, int 
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// Eight codes of a word, less 8, as fp16 pairs: nibbles (0, 4), 16 x (1, 5), (2, 6), 16 x (3, 7).
+// Eight codes of a word as fp16 pairs 2 c - 15: nibbles (0, 4), 16 x (1, 5), (2, 6), 16 x (3, 7).
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -152,11 +154,11 @@ __device__ __forceinline__ uint32_t h2sub(uint32_t x, uint32_t y) {
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&c)[4]) {
-    const uint32_t w8 = w >> 8;
-    c[0] = h2sub(and_or(w, 0x000f000fu, 0x64006400u), 0x64086408u);
-    c[1] = h2sub(and_or(w, 0x00f000f0u, 0x64006400u), 0x64806480u);
-    c[2] = h2sub(and_or(w8, 0x000f000fu, 0x64006400u), 0x64086408u);
-    c[3] = h2sub(and_or(w8, 0x00f000f0u, 0x64006400u), 0x64806480u);
+    const uint32_t w1 = w << 1, w8 = w >> 7;  // nibbles one bit up: 1024 + 2 c, 1024 + 32 c
+    c[0] = h2sub(and_or(w1, 0x001e001eu, 0x64006400u), 0x640f640fu);
+    c[1] = h2sub(and_or(w1, 0x01e001e0u, 0x64006400u), 0x64f064f0u);
+    c[2] = h2sub(and_or(w8, 0x001e001eu, 0x64006400u), 0x640f640fu);
+    c[3] = h2sub(and_or(w8, 0x01e001e0u, 0x64006400u), 0x64f064f0u);
 }
 
 // A place in the batch's order of tiles: sequences, their (kv head, head
@@ -271,15 +273,15 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 //          columns 2 t, 2 t + 1 belong to head t and none is idle;
 //   else   eight heads, columns 2 t, 2 t + 1 being heads 2 t, 2 t + 1.
 // Scores: codes as bytes (nibbles of a word are two ANDs and a shift), q as
-// 23-bit whole numbers in three signed bytes: integer products, exact, so codes
-// need no centring here.  FEW: two products, columns (top, middle) and (low, 0);
+// 23-bit whole numbers in three signed bytes: integer products, exact, from which
+// 8 sum(q) is taken before the first rounding.  FEW: two products, columns (top, middle) and (low, 0);
 // else three, one for each byte.
 // Output: p d as fp16 hi, lo, turned to the operand's order with movmatrix.
 // FEW: hi and lo are a head's two columns; else two products.
 // On this chip a warp-level MMA keeps the integer and half pipes from issuing
 // (8 cycles each, measured in one loop with them), so their number counts: FEW
 // has 32 for 32 rows of 128 dims, the other form 56.  4 heads per kv head of
-// 128 dims, the other form against FEW: one sequence of 131072 positions 48.8
+// 128 dims, the other form against FEW (both before keys were centred): one sequence of 131072 positions 48.8
 // -> 40.6 us, 128 ragged ones 95.6 -> 77.4; one head (GPT-2, 700 positions) 7.8
 // -> 7.5.  Eight heads would take FEW twice, at 0.83 of the other's time each.
 template <int NB, bool FEW> struct State {
@@ -287,8 +289,9 @@ template <int NB, bool FEW> struct State {
     static constexpr int LP = FEW ? 2 : 3;  // products of q's bytes
     uint32_t q[LP][NB][2];                  // q as matrix operands
     float qsum[Q4<NB>::NG][HL], qfac[HL];   // sums of the whole numbers, the factor of their products
+    float c8[Q4<NB>::NG][HL][2];            // -8 times the sums of q's upper two bytes (as one number) and of the low one
     float2 o[2 * NB][2];                    // dims x this lane's two columns
-    float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p m', sum p
+    float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p (m + 7.5 d), sum p
     float mx[HL];                           // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
     int vexp;                               // largest exponent field of the values' d so far
 };
@@ -337,12 +340,17 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
     const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
     const float up = __uint_as_float((uint32_t)(127 + 21 - ex) << 23);
     float sum[NG];
+    int low[NG];
 #pragma unroll
-    for (int j = 0; j < NG; j++) sum[j] = 0.0f;
+    for (int j = 0; j < NG; j++) {
+        sum[j] = 0.0f;
+        low[j] = 0;
+    }
 #pragma unroll
     for (int i = 0; i < NB; i++) {
         uint32_t byte[3][2] = {};  // top, middle, low; each 128 more
         float s = 0.0f;
+        int n = 0;  // of the low bytes
 #pragma unroll
         for (int e = 0; e < 8; e++) {  // dims 0, 2, 4, 6 of the word: its low nibbles; 1, 3, 5, 7: its high ones
             const float y = rintf(x[i][e] * up);
@@ -351,9 +359,12 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
 #pragma unroll
             for (int k = 0; k < 3; k++) byte[k][e & 1] |= (b >> (16 - 8 * k) & 0xffu) << (8 * (e >> 1));
         }
+#pragma unroll
+        for (int k = 0; k < 2; k++) n = __dp4a((int)(byte[2][k] ^ 0x80808080u), 0x01010101, n);
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
         sum[i / 2] += s;
+        low[i / 2] += n;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             if (FEW) {
@@ -366,6 +377,11 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
         }
     }
     // lane (g, t) goes on with the heads of columns 2 t (and 2 t + 1)
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        low[j] += __shfl_xor_sync(0xffffffffu, low[j], 1);
+        low[j] += __shfl_xor_sync(0xffffffffu, low[j], 2);
+    }
     const float fac = LOG2E / sqrtf((float)DH) * __uint_as_float((uint32_t)(127 - 21 + ex) << 23);
 #pragma unroll
     for (int hl = 0; hl < S::HL; hl++) {
@@ -373,6 +389,9 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
 #pragma unroll
         for (int j = 0; j < NG; j++) {
             st.qsum[j][hl] = __shfl_sync(0xffffffffu, sum[j], 8 * t + 4 * hl);
+            const int l = __shfl_sync(0xffffffffu, low[j], 8 * t + 4 * hl);
+            st.c8[j][hl][0] = ((float)l - st.qsum[j][hl]) * 0.03125f;  // (8 / 256; 256 divides the difference of the sums)
+            st.c8[j][hl][1] = -8.0f * (float)l;
             st.om[j][hl] = 0.0f;
         }
         st.l[hl] = 0.0f;
@@ -457,12 +476,14 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const float2 d = __half22float2(*reinterpret_cast<const __half2 *>(&f[r][j]));
+                const float m = fmaf(8.0f, d.x, d.y);
 #pragma unroll
                 for (int hl = 0; hl < HL; hl++) {
                     // 2^16 top + 2^8 middle + low: the first two together are below 2^24, exact in fp32
                     const int top = c[0][2 * r + hl], mid = FEW ? c[0][2 * r + 1] : c[1][2 * r + hl], low = c[S::LP - 1][2 * r + hl];
-                    const float x = fmaf((float)(top * 256 + mid), 256.0f, (float)low);
-                    s[h][r][hl] = fmaf(d.y, st.qsum[j][hl], j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
+                    // (below 2^24 too with the 8 of each code taken off)
+                    const float x = fmaf((float)(top * 256 + mid) + st.c8[j][hl][0], 256.0f, (float)low + st.c8[j][hl][1]);
+                    s[h][r][hl] = fmaf(m, st.qsum[j][hl], j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
                 }
             }
         }
@@ -517,7 +538,7 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
 #pragma unroll
         for (int h = 0; h < NH; h++) {
             const float2 d0 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][0][j])), d1 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][1][j]));
-            const float m0 = fmaf(8.0f, d0.x, d0.y), m1 = fmaf(8.0f, d1.x, d1.y);
+            const float m0 = fmaf(7.5f, d0.x, d0.y), m1 = fmaf(7.5f, d1.x, d1.y);
 #pragma unroll
             for (int hl = 0; hl < HL; hl++) om[hl] = fmaf(s[h][0][hl], m0, fmaf(s[h][1][hl], m1, om[hl]));
             uint32_t hi, lo;
@@ -600,7 +621,7 @@ __device__ __forceinline__ void result(const State<NB, FEW> &st, int lane, float
 #pragma unroll
             for (int k = 0; k < (half ? 1 : 2); k++) {
                 const float2 *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
-                auto col = [&](const float2 &v) { return FEW ? v.x + v.y : hl ? v.y : v.x; };  // (hi and lo, or the head's)
+                auto col = [&](const float2 &v) { return 0.5f * (FEW ? v.x + v.y : hl ? v.y : v.x); };  // (hi and lo, or the head's)
                 const float4 v = make_float4((col(a[0]) + m) * iv, fmaf(col(a[1]), 0.0625f, m) * iv, (col(b[0]) + m) * iv,
                                              fmaf(col(b[1]), 0.0625f, m) * iv);
                 float *o = dst + h * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
