@@ -344,13 +344,15 @@ extern "C" int lmc_kv_pages_fork(int *d_pages, int n_seqs, int max_pages, int *d
         return lmc_set_error(LMC_ERR_INVALID, "kv_pages_fork: %d sequences x %d entries, %d pages (at most 16384 "
                              "sequences)", n_seqs, max_pages, n_pages);
     // 32 columns (128 bytes of a row) to a CTA; down to 8 (a 32-byte sector)
-    // while that gives fewer than two CTAs an SM, and as few as fit in shared memory
+    // while that gives fewer than two CTAs an SM, and as few as fit in 128 KiB,
+    // with the parents and changes beside them in 200 (16384 sequences: one column, 192 KiB)
+    constexpr size_t MOST = 200 * 1024;
+    const size_t column = n_seqs * sizeof(int);
     int cs = 5;
     while (cs > 3 && (max_pages >> cs) < 2 * lmc_sm_count()) cs--;
-    while (cs > 0 && ((size_t)n_seqs << cs) * sizeof(int) > 128 * 1024) cs--;
-    const size_t smem = (((size_t)n_seqs << cs) + 2 * (size_t)n_seqs) * sizeof(int);
-    if (smem > 48 * 1024)
-        LMC_CUDA_TRY(cudaFuncSetAttribute(k_pages_fork, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    while (cs > 0 && (column << cs > 128 * 1024 || (column << cs) + 2 * column > MOST)) cs--;
+    const size_t smem = (column << cs) + 2 * column;
+    if (smem > 48 * 1024) LMC_CUDA_TRY(cudaFuncSetAttribute(k_pages_fork, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST));
     LMC_LAUNCH("kv pages fork", k_pages_fork, lmc_cdiv(max_pages, (size_t)1 << cs), 256, smem, lmc_stream(stream), d_pages,
                n_seqs, max_pages, d_refs, n_pages, d_parent, cs);
     return LMC_OK;
