@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) k_pages_fork(int *pages, int n_seqs, int 
         if ((i & mask) < nc) tile[i] = pages[(size_t)(i >> cs) * max_pages + c0 + (i & mask)];
     for (int b = threadIdx.x; b < n_seqs; b += 256) {
         int p = b < 256 ? p0 : parent[b];
-        if (p >= n_seqs) {
+        if (p >= n_seqs || p < -1) {
             atomicExch(&g_kv_pages_err, 1);
             p = b;
         }

@@ -7,6 +7,8 @@ from tests.test_gpu_kv_q4 import dev
 
 pytestmark = pytest.mark.gpu
 
+INVALID = -1
+
 
 def forked(table, parent):
     """The table after a call with parents from -1 on, and its counts."""
@@ -29,3 +31,19 @@ def test_fork_of_many_sequences(cuda, n_seqs, width):
     rt.call("lmc_kv_pages_fork", dt.data_ptr(), n_seqs, width, dr.data_ptr(), n_pages, dp.data_ptr(), None)
     assert np.array_equal(dt.cpu().numpy(), want) and np.array_equal(dr.cpu().numpy(), counts(n_pages))
     assert rt.lib().lmc_device_status() == 0
+
+
+@pytest.mark.parametrize("bad", [-2, -1000000, -2**31])
+def test_fork_of_a_parent_below_minus_one(cuda, bad):
+    """Only -1 gives a row's pages back: a row with any other negative parent
+    stays as it is, in table and counts, and the status tells once.  The other
+    rows are served, one of them from the row that stays."""
+    table = np.array([[0, 1, -1], [2, 3, 4], [5, -1, -1], [2, 6, 7]], np.int32)
+    refs = np.bincount(table[table >= 0], minlength=9).astype(np.int32)
+    dt, dr = dev(cuda, table), dev(cuda, refs)
+    dp = dev(cuda, np.array([1, bad, -1, 3], np.int32))
+    rt.call("lmc_kv_pages_fork", dt.data_ptr(), 4, 3, dr.data_ptr(), 9, dp.data_ptr(), None)
+    assert rt.lib().lmc_device_status() == INVALID and b"kv pages" in rt.lib().lmc_last_error()
+    assert rt.lib().lmc_device_status() == 0
+    want, counts = forked(table, np.array([1, 1, -1, 3]))
+    assert np.array_equal(dt.cpu().numpy(), want) and np.array_equal(dr.cpu().numpy(), counts(9))
