@@ -106,6 +106,11 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
           "l"(reinterpret_cast<unsigned long long &>(c)));
     return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // x, y as fp16 pairs hi + lo
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -289,7 +294,7 @@ template <int NB, bool FEW> struct State {
     static constexpr int LP = FEW ? 2 : 3;  // products of q's bytes
     uint32_t q[LP][NB][2];                  // q as matrix operands
     float qsum[Q4<NB>::NG][HL], qfac[HL];   // sums of the whole numbers, the factor of their products
-    float c8[Q4<NB>::NG][HL][2];            // -8 times the sums of q's upper two bytes (as one number) and of the low one
+    int c8[Q4<NB>::NG][HL][2];              // -8 times the sums of q's upper two bytes (as one number) and of the low one
     float2 o[2 * NB][2];                    // dims x this lane's two columns
     float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p (m + 7.5 d), sum p
     float mx[HL];                           // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
@@ -327,71 +332,68 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
     constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
     const int t = lane & 3;
     const bool odd = lane & 4;
-    float big = 0.0f;
+    float big = 0.0f;  // (NaN when a value is)
 #pragma unroll
     for (int i = 0; i < NB; i++) {
         rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[i][e]));
+        for (int e = 0; e < 8; e++) big = max_nan(big, fabsf(x[i][e]));
     }
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
     // a power of two that brings the head's largest |q| into [2^21, 2^22): three signed bytes hold it
     const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
     const float up = __uint_as_float((uint32_t)(127 + 21 - ex) << 23);
-    float sum[NG];
-    int low[NG];
-#pragma unroll
-    for (int j = 0; j < NG; j++) {
-        sum[j] = 0.0f;
-        low[j] = 0;
-    }
+    int sum[NG][2] = {};  // of the upper two bytes (as one number) and of the low ones: exact
 #pragma unroll
     for (int i = 0; i < NB; i++) {
         uint32_t byte[3][2] = {};  // top, middle, low; each 128 more
-        float s = 0.0f;
-        int n = 0;  // of the low bytes
 #pragma unroll
         for (int e = 0; e < 8; e++) {  // dims 0, 2, 4, 6 of the word: its low nibbles; 1, 3, 5, 7: its high ones
-            const float y = rintf(x[i][e] * up);
-            s += y;  // (a value that is not finite makes the sum, and with it the score, NaN or infinite)
-            const uint32_t b = (uint32_t)__float2int_rn(y) + 0x808080u;
+            const uint32_t b = (uint32_t)__float2int_rn(x[i][e] * up) + 0x808080u;
 #pragma unroll
             for (int k = 0; k < 3; k++) byte[k][e & 1] |= (b >> (16 - 8 * k) & 0xffu) << (8 * (e >> 1));
         }
+        int n[3] = {};
 #pragma unroll
-        for (int k = 0; k < 2; k++) n = __dp4a((int)(byte[2][k] ^ 0x80808080u), 0x01010101, n);
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        sum[i / 2] += s;
-        low[i / 2] += n;
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int b = 0; b < 3; b++) {
+                byte[b][k] ^= 0x80808080u;
+                n[b] = __dp4a((int)byte[b][k], 0x01010101, n[b]);
+            }
+        sum[i / 2][0] += n[0] * 256 + n[1];
+        sum[i / 2][1] += n[2];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             if (FEW) {
-                st.q[0][i][k] = (odd ? byte[1][k] : byte[0][k]) ^ 0x80808080u;
-                st.q[1][i][k] = odd ? 0u : byte[2][k] ^ 0x80808080u;
+                st.q[0][i][k] = odd ? byte[1][k] : byte[0][k];
+                st.q[1][i][k] = odd ? 0u : byte[2][k];
             } else {
 #pragma unroll
-                for (int b = 0; b < S::LP; b++) st.q[b][i][k] = byte[b][k] ^ 0x80808080u;
+                for (int b = 0; b < S::LP; b++) st.q[b][i][k] = byte[b][k];
             }
         }
     }
     // lane (g, t) goes on with the heads of columns 2 t (and 2 t + 1)
 #pragma unroll
-    for (int j = 0; j < NG; j++) {
-        low[j] += __shfl_xor_sync(0xffffffffu, low[j], 1);
-        low[j] += __shfl_xor_sync(0xffffffffu, low[j], 2);
-    }
+    for (int j = 0; j < NG; j++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            sum[j][k] += __shfl_xor_sync(0xffffffffu, sum[j][k], 1);
+            sum[j][k] += __shfl_xor_sync(0xffffffffu, sum[j][k], 2);
+        }
+    const float bad = big - big;  // NaN, and with it every score, when a value is not finite; else 0
     const float fac = LOG2E / sqrtf((float)DH) * __uint_as_float((uint32_t)(127 - 21 + ex) << 23);
 #pragma unroll
     for (int hl = 0; hl < S::HL; hl++) {
         st.qfac[hl] = __shfl_sync(0xffffffffu, fac, 8 * t + 4 * hl);
 #pragma unroll
         for (int j = 0; j < NG; j++) {
-            st.qsum[j][hl] = __shfl_sync(0xffffffffu, sum[j], 8 * t + 4 * hl);
-            const int l = __shfl_sync(0xffffffffu, low[j], 8 * t + 4 * hl);
-            st.c8[j][hl][0] = ((float)l - st.qsum[j][hl]) * 0.03125f;  // (8 / 256; 256 divides the difference of the sums)
-            st.c8[j][hl][1] = -8.0f * (float)l;
+            const int hi = __shfl_sync(0xffffffffu, sum[j][0], 8 * t + 4 * hl), lo = __shfl_sync(0xffffffffu, sum[j][1], 8 * t + 4 * hl);
+            st.qsum[j][hl] = fmaf((float)hi, 256.0f, (float)lo) + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl);  // (one rounding)
+            st.c8[j][hl][0] = -8 * hi;
+            st.c8[j][hl][1] = -8 * lo;
             st.om[j][hl] = 0.0f;
         }
         st.l[hl] = 0.0f;
@@ -479,10 +481,10 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
                 const float m = fmaf(8.0f, d.x, d.y);
 #pragma unroll
                 for (int hl = 0; hl < HL; hl++) {
-                    // 2^16 top + 2^8 middle + low: the first two together are below 2^24, exact in fp32
+                    // 2^16 top + 2^8 middle + low, 8 taken off each code: the first two together, and the
+                    // low one, are below 2^24, exact in fp32
                     const int top = c[0][2 * r + hl], mid = FEW ? c[0][2 * r + 1] : c[1][2 * r + hl], low = c[S::LP - 1][2 * r + hl];
-                    // (below 2^24 too with the 8 of each code taken off)
-                    const float x = fmaf((float)(top * 256 + mid) + st.c8[j][hl][0], 256.0f, (float)low + st.c8[j][hl][1]);
+                    const float x = fmaf((float)(top * 256 + mid + st.c8[j][hl][0]), 256.0f, (float)(low + st.c8[j][hl][1]));
                     s[h][r][hl] = fmaf(m, st.qsum[j][hl], j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
                 }
             }

@@ -1,0 +1,83 @@
+"""Decode attention over 4-bit rows where its number formats could lose bits:
+against 64 bits on the values that the rows stand for.
+
+Every output is sum p v / sum p.  With ds the bound on a score's error, a
+weight p is off by at most 2 ds + 2^-20 relative to it (ds of its own and of
+the maximum, fp32 exponential, p d in 22 bits), and the sums over n positions
+by (n / 4 + 16) 2^-24 (chains of at most n / 4 fp32 additions).  A value is
+taken as (m + 7.5 d) + d (2 c - 15) / 2, two terms of at most the row's largest
+|value| in its group, so per group |do| <= rel * 2 * sum p vmax / sum p with
+rel = 2 ds + 2^-20 + (n / 4 + 16) 2^-24 and vmax the row's largest |value| there."""
+import numpy as np
+import pytest
+
+from lmc_b200 import runtime as rt
+from tests import kv_ref
+from tests.conftest import rel_err
+from tests.test_gpu_kv_q4 import Cache, dev, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+def decode(torch, q, k, v):
+    """q [H][Dh], k and v [Hkv][n][Dh] fp32, the last row the new one ->
+    (out, values of the stored k, of the stored v)."""
+    (H, Dh), (Hkv, n, _) = q.shape, k.shape
+    c = Cache(torch, np.random.default_rng(0), [0], Hkv, Dh, n, 0)
+    for side, (x, vals) in enumerate(((k, c.k), (v, c.v))):
+        r, val = kv_ref.q4_rows(x)
+        c.raw[side][0, :, :n - 1] = r[:, :n - 1]
+        vals[0] = val
+    c.dk, c.dv = dev(torch, c.raw[0]), dev(torch, c.raw[1])
+    out = torch.full((1, H * Dh), 5.0, device="cuda")
+    new = [np.ascontiguousarray(x[:, -1].reshape(1, -1)) for x in (k, v)]
+    c.decode(torch, out, *(dev(torch, a) for a in (q.reshape(1, -1), *new, np.array([n - 1], np.int32))), H // Hkv)
+    assert rt.lib().lmc_device_status() == 0
+    return out.cpu().numpy().reshape(H, Dh), c.k[0], c.v[0]
+
+
+def check(out, q, k, v, ds, norm=True):
+    """Per group of 64 dims against the bound above; ds [H] or a number."""
+    (H, Dh), G = q.shape, q.shape[0] // k.shape[0]
+    n = k.shape[1]
+    for h in range(H):
+        kk, vv = k[h // G], v[h // G]
+        s = kk @ q[h].astype(np.float64) / np.sqrt(Dh)
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        rel = 2 * np.broadcast_to(ds, H)[h] + 2.0 ** -20 + (n / 4 + 16) * 2.0 ** -24
+        for g in range(0, Dh, 64):
+            x, want = vv[:, g:g + 64], p @ vv[:, g:g + 64]
+            worst = np.abs(out[h, g:g + 64] - want).max()
+            assert worst <= rel * 2 * (p @ np.abs(x).max(-1)), (h, g, worst / (p @ np.abs(x).max(-1)), rel)
+            if norm:  # the repository's attention bound
+                assert rel_err(out[h, g:g + 64], want) < 1e-5, (h, g, rel_err(out[h, g:g + 64], want))
+
+
+def keys_with_zero(rng, Hkv, n, Dh, step):
+    """Keys whose groups run from -8 to 7 steps (powers of two), so that m =
+    -8 d exactly, code 8 is exactly 0, and small numbers are stored as 0."""
+    step = np.broadcast_to(step, (Hkv, n, Dh)).astype(np.float32)
+    k = (rng.normal(0, 2.5, (Hkv, n, Dh)) * step).astype(np.float32)
+    k = np.clip(k, -8 * step, 7 * step)
+    k[..., 0::64], k[..., 1::64] = -8 * step[..., 0::64], 7 * step[..., 1::64]
+    return k
+
+
+@pytest.mark.parametrize("G", [1, 4, 5, 8, 9])
+@pytest.mark.parametrize("Dh", [64, 96, 128, 256])
+def test_scores_of_zero_keys_are_zero(cuda, G, Dh):
+    """Keys that are exactly 0 wherever q is not: every score is 0 (ds = 0),
+    the output the mean of the values, however large q and its sum are.  The
+    rows' steps d are 1 and 64."""
+    rng = np.random.default_rng(G + Dh)
+    n = 90
+    k = np.zeros((1, n, Dh), np.float32)
+    step = np.where(np.arange(n) % 2, 64, 1)
+    k[..., 0::64], k[..., 1::64] = -8 * step[:, None], 7 * step[:, None]
+    q = rng.uniform(512, 1024, (G, Dh)).astype(np.float32)
+    q[:, 0::64] = q[:, 1::64] = 0
+    v = rows_of(rng, (1, n, Dh))
+    out, kv, vv = decode(cuda, q, k, v)
+    assert not (kv[:, :, None] * q).any()
+    check(out, q, kv, vv, 0.0)
