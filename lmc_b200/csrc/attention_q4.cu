@@ -5,8 +5,10 @@
 //   o_j = sum_t p_t d_tj (2 c_tj - 15) / 2 + sum_t p_t (m_tj + 7.5 d_tj),   p_t = 2^(s_t log2 e - max)
 // so the matrix units only ever see whole numbers and fp32 factors; the scales
 // are applied per group outside (keys) or folded into the probabilities
-// (values).  Keys: integer products, q as whole numbers of 23 bits in three
-// signed bytes.  Codes are centred, because sums over positive codes would be
+// (values).  Keys: integer products, q as whole numbers in four signed bytes,
+// the largest |q| of a group of 64 dims in [2^29, 2^30): a channel down to 1/64
+// of it keeps all of fp32's bits, a smaller one is off by at most 2^-30 of it.
+// Codes are centred, because sums over positive codes would be
 // large against the score, and against the result of a long, flat softmax, and
 // take their rounding with them (131072 positions, keys with a few large
 // channels: relative error 1.0e-6, centred in both 0.7e-6, for 4% more time).
@@ -278,23 +280,24 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 //          columns 2 t, 2 t + 1 belong to head t and none is idle;
 //   else   eight heads, columns 2 t, 2 t + 1 being heads 2 t, 2 t + 1.
 // Scores: codes as bytes (nibbles of a word are two ANDs and a shift), q as
-// 23-bit whole numbers in three signed bytes: integer products, exact, from which
-// 8 sum(q) is taken before the first rounding.  FEW: two products, columns (top, middle) and (low, 0);
-// else three, one for each byte.
+// 31-bit whole numbers in four signed bytes: integer products, exact, from which
+// 8 sum(q) is taken before the first rounding.  FEW: two products, columns
+// (byte 0, byte 1) and (byte 2, byte 3); else four, one for each byte.
 // Output: p d as fp16 hi, lo, turned to the operand's order with movmatrix.
 // FEW: hi and lo are a head's two columns; else two products.
 // On this chip a warp-level MMA keeps the integer and half pipes from issuing
 // (8 cycles each, measured in one loop with them), so their number counts: FEW
-// has 32 for 32 rows of 128 dims, the other form 56.  4 heads per kv head of
+// has 32 for 32 rows of 128 dims, the other form 64.  4 heads per kv head of
 // 128 dims, the other form against FEW (both before keys were centred): one sequence of 131072 positions 48.8
 // -> 40.6 us, 128 ragged ones 95.6 -> 77.4; one head (GPT-2, 700 positions) 7.8
 // -> 7.5.  Eight heads would take FEW twice, at 0.83 of the other's time each.
 template <int NB, bool FEW> struct State {
     static constexpr int HL = FEW ? 1 : 2;  // heads of a lane
-    static constexpr int LP = FEW ? 2 : 3;  // products of q's bytes
+    static constexpr int LP = FEW ? 2 : 4;  // products of q's bytes
     uint32_t q[LP][NB][2];                  // q as matrix operands
-    float qsum[Q4<NB>::NG][HL], qfac[HL];   // sums of the whole numbers, the factor of their products
-    int c8[Q4<NB>::NG][HL][2];              // -8 times the sums of q's upper two bytes (as one number) and of the low one
+    float w[Q4<NB>::NG][HL];                // factor of the group's whole numbers (a power of two; 1 for the largest)
+    float qsum[Q4<NB>::NG][HL], qfac[HL];   // sums of the whole numbers, times w; the factor of the scores
+    int c8[Q4<NB>::NG][HL][2];              // -8 times the sums of q's upper two bytes (as one number) and of the lower two
     float2 o[2 * NB][2];                    // dims x this lane's two columns
     float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p (m + 7.5 d), sum p
     float mx[HL];                           // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
@@ -332,47 +335,48 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
     constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
     const int t = lane & 3;
     const bool odd = lane & 4;
-    float big = 0.0f;  // (NaN when a value is)
+    // a power of two that brings the group's largest |q| into [2^29, 2^30): four signed bytes hold it
+    float big[NG] = {}, bad = 0.0f;  // (NaN when a value is)
+    int ex[NG], top = -97;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
         rope8(a, p.pos, DH, 32 * i + 8 * t, x[i]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) big = max_nan(big, fabsf(x[i][e]));
+        for (int e = 0; e < 8; e++) big[i / 2] = max_nan(big[i / 2], fabsf(x[i][e]));
     }
-    big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // a power of two that brings the head's largest |q| into [2^21, 2^22): three signed bytes hold it
-    const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 127);
-    const float up = __uint_as_float((uint32_t)(127 + 21 - ex) << 23);
-    int sum[NG][2] = {};  // of the upper two bytes (as one number) and of the low ones: exact
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        big[j] = max_nan(big[j], __shfl_xor_sync(0xffffffffu, big[j], 1));
+        big[j] = max_nan(big[j], __shfl_xor_sync(0xffffffffu, big[j], 2));
+        bad += big[j] - big[j];  // NaN, and with it every score, when a value is not finite; else 0
+        ex[j] = min(max((int)(__float_as_uint(big[j]) >> 23) - 127, -97), 127);
+        top = max(top, ex[j]);
+    }
+    int sum[NG][2] = {};  // of the upper two bytes (as one number) and of the lower two: exact
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-        uint32_t byte[3][2] = {};  // top, middle, low; each 128 more
+        const float up = __uint_as_float((uint32_t)(127 + 29 - ex[i / 2]) << 23);
+        uint32_t byte[4][2] = {};  // the highest first; each 128 more
 #pragma unroll
         for (int e = 0; e < 8; e++) {  // dims 0, 2, 4, 6 of the word: its low nibbles; 1, 3, 5, 7: its high ones
-            const uint32_t b = (uint32_t)__float2int_rn(x[i][e] * up) + 0x808080u;
+            const uint32_t b = (uint32_t)__float2int_rn(x[i][e] * up) + 0x80808080u;
 #pragma unroll
-            for (int k = 0; k < 3; k++) byte[k][e & 1] |= (b >> (16 - 8 * k) & 0xffu) << (8 * (e >> 1));
+            for (int k = 0; k < 4; k++) byte[k][e & 1] |= (b >> (24 - 8 * k) & 0xffu) << (8 * (e >> 1));
         }
-        int n[3] = {};
+        int n[4] = {};
 #pragma unroll
         for (int k = 0; k < 2; k++)
 #pragma unroll
-            for (int b = 0; b < 3; b++) {
+            for (int b = 0; b < 4; b++) {
                 byte[b][k] ^= 0x80808080u;
                 n[b] = __dp4a((int)byte[b][k], 0x01010101, n[b]);
             }
         sum[i / 2][0] += n[0] * 256 + n[1];
-        sum[i / 2][1] += n[2];
+        sum[i / 2][1] += n[2] * 256 + n[3];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            if (FEW) {
-                st.q[0][i][k] = odd ? byte[1][k] : byte[0][k];
-                st.q[1][i][k] = odd ? 0u : byte[2][k];
-            } else {
 #pragma unroll
-                for (int b = 0; b < S::LP; b++) st.q[b][i][k] = byte[b][k];
-            }
+            for (int b = 0; b < S::LP; b++) st.q[b][i][k] = FEW ? (odd ? byte[2 * b + 1][k] : byte[2 * b][k]) : byte[b][k];
         }
     }
     // lane (g, t) goes on with the heads of columns 2 t (and 2 t + 1)
@@ -383,15 +387,17 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
             sum[j][k] += __shfl_xor_sync(0xffffffffu, sum[j][k], 1);
             sum[j][k] += __shfl_xor_sync(0xffffffffu, sum[j][k], 2);
         }
-    const float bad = big - big;  // NaN, and with it every score, when a value is not finite; else 0
-    const float fac = LOG2E / sqrtf((float)DH) * __uint_as_float((uint32_t)(127 - 21 + ex) << 23);
+    const float fac = LOG2E / sqrtf((float)DH) * __uint_as_float((uint32_t)(127 - 29 + top) << 23);
 #pragma unroll
     for (int hl = 0; hl < S::HL; hl++) {
         st.qfac[hl] = __shfl_sync(0xffffffffu, fac, 8 * t + 4 * hl);
 #pragma unroll
         for (int j = 0; j < NG; j++) {
             const int hi = __shfl_sync(0xffffffffu, sum[j][0], 8 * t + 4 * hl), lo = __shfl_sync(0xffffffffu, sum[j][1], 8 * t + 4 * hl);
-            st.qsum[j][hl] = fmaf((float)hi, 256.0f, (float)lo) + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl);  // (one rounding)
+            // (2^-126 for less: below what a score can show)
+            const float w = __uint_as_float((uint32_t)max(127 + __shfl_sync(0xffffffffu, ex[j] - top, 8 * t + 4 * hl), 1) << 23);
+            st.w[j][hl] = w;
+            st.qsum[j][hl] = (fmaf((float)hi, 65536.0f, (float)lo) + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl)) * w;  // (one rounding)
             st.c8[j][hl][0] = -8 * hi;
             st.c8[j][hl][1] = -8 * lo;
             st.om[j][hl] = 0.0f;
@@ -481,10 +487,12 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
                 const float m = fmaf(8.0f, d.x, d.y);
 #pragma unroll
                 for (int hl = 0; hl < HL; hl++) {
-                    // 2^16 top + 2^8 middle + low, 8 taken off each code: the first two together, and the
-                    // low one, are below 2^24, exact in fp32
-                    const int top = c[0][2 * r + hl], mid = FEW ? c[0][2 * r + 1] : c[1][2 * r + hl], low = c[S::LP - 1][2 * r + hl];
-                    const float x = fmaf((float)(top * 256 + mid + st.c8[j][hl][0]), 256.0f, (float)(low + st.c8[j][hl][1]));
+                    // 2^16 upper + lower two bytes' sums, 8 taken off each code: at most 2^23, exact in fp32,
+                    // and 2^24 + 2^16, off by 1 at most
+                    const int hi = FEW ? c[0][2 * r] * 256 + c[0][2 * r + 1] : c[0][2 * r + hl] * 256 + c[1][2 * r + hl];
+                    const int lo = FEW ? c[1][2 * r] * 256 + c[1][2 * r + 1] : c[S::LP - 2][2 * r + hl] * 256 + c[S::LP - 1][2 * r + hl];
+                    float x = fmaf((float)(hi + st.c8[j][hl][0]), 65536.0f, (float)(lo + st.c8[j][hl][1]));
+                    if (NG > 1) x *= st.w[j][hl];
                     s[h][r][hl] = fmaf(m, st.qsum[j][hl], j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
                 }
             }

@@ -81,3 +81,30 @@ def test_scores_of_zero_keys_are_zero(cuda, G, Dh):
     out, kv, vv = decode(cuda, q, k, v)
     assert not (kv[:, :, None] * q).any()
     check(out, q, kv, vv, 0.0)
+
+
+@pytest.mark.parametrize("G", [1, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("where,r", [("groups", 1000), ("groups", 30000), ("within", 30), ("within", 100), ("within", 1000)])
+def test_queries_of_unequal_channels(cuda, G, where, r):
+    """Channels of q that are r times larger, where the keys are r times
+    smaller (one group of 64 dims) or 0 (every 16th dim).
+
+    q is held to a whole number of at least 2^29 for the largest |q| of a
+    group, so a channel is off by at most 2^-30 of that; m + 8 d is 0 here, and
+    what is left of a score are at most 8 fp32 roundings (the whole numbers'
+    sum, times d, the groups added up, the scale, the difference to the
+    maximum), each of at most 2^-24 of sum |q k|."""
+    rng = np.random.default_rng(G + r)
+    Dh, n, Hkv = 128, 200, 2
+    big = np.arange(Dh) >= 64 if where == "groups" else np.arange(Dh) % 16 == 5
+    step = 0.25 * np.where(big, 1 / 2.0 ** np.round(np.log2(r)), 1) if where == "groups" else 0.25
+    k = keys_with_zero(rng, Hkv, n, Dh, step)
+    if where == "within":
+        k[..., big] = 0
+    q = rows_of(rng, (Hkv * G, Dh)) * np.where(big, r, 1).astype(np.float32)
+    v = rows_of(rng, (Hkv, n, Dh))
+    out, kv, vv = decode(cuda, q, k, v)
+    kk, a = np.repeat(np.abs(kv), G, 0), np.abs(q.astype(np.float64))
+    held = sum(2.0 ** -30 * a[:, g:g + 64].max(-1) * kk[:, :, g:g + 64].sum(-1).max(-1) for g in (0, 64))
+    size = np.einsum("hnd,hd->hn", kk, a).max(-1)
+    check(out, q, kv, vv, (held + 8 * 2.0 ** -24 * size) / np.sqrt(Dh))
