@@ -16,10 +16,11 @@
 // A value's code as fp16: a nibble ORed into bits 1 to 4 of 1024.0 is 1024 +
 // 2 c, exactly, and 1039 less is 2 c - 15 (two instructions for two operands);
 // the nibble above it gives 16 (2 c - 15), and the 16 goes into the final
-// factor.  p d becomes an fp16 pair hi + lo (22 bits).  The probabilities are
-// scaled so that p d stays just below 2^15 (the largest exponent of d so far is
-// tracked like the running maximum), so small values keep their relative
-// accuracy.  The matrix unit truncates its sums, so a tile's products (and its
+// factor.  p d becomes an fp16 pair hi + lo (22 bits), scaled by a power of two
+// that keeps it just below 2^15: its largest exponent so far is tracked like the
+// running maximum, for each head and group of 64 dims, so that neither a group of
+// larger values nor a row of large values without weight takes bits from it (a p d
+// below 2^-18 of the largest is off by at most 2^-40 of that).  The matrix unit truncates its sums, so a tile's products (and its
 // sums of p and of p with the minima) go to fresh accumulators that are added
 // to the running ones in rounded fp32.
 //
@@ -59,9 +60,17 @@ constexpr int Q4_STAGES = 2;  // tiles in a warp's ring
 // 4 kv heads, eight query heads each, 18.9, 18.7, 19.1.
 constexpr int Q4_ITEM = 2;
 constexpr float LOG2E = 1.4426950408889634f;
+// Exponent fields of p d that a scale is made for: 2^(141 - field) is a normal
+// number, and p d is at most 65504.
+constexpr int Q4_PE_MIN = 15, Q4_PE_MAX = 142;
 // Limit of a wait for bulk copies (nanoseconds of %globaltimer).
 __device__ long long g_attn_q4_wait_ns = 1000000000ll;
 
+// Head sizes of 224 and 256 with more than four heads: what a lane keeps of its
+// heads' groups lies in shared memory (in registers 192 bytes a thread are
+// spilled at 256 dims; 16 ragged sequences of 8 kv heads, eight query heads
+// each, 52.4 and 43.7 us).
+constexpr bool q4_shared_groups(int NB, bool FEW) { return !FEW && NB > 6; }
 constexpr int q4_tile(int NB) { return NB <= 4 ? 64 : 32; }  // positions per tile (registers and shared memory)
 
 struct Q4Args {
@@ -80,7 +89,8 @@ template <int NB> struct Q4 {
     static constexpr int SIDE = T * RB + 16;              // a tile's K or V rows, from any 4-byte phase
     static constexpr int STAGE = 2 * SIDE;
     static constexpr int FRESH = (2 * RB + 15) / 16 * 16; // the new K and V rows
-    static constexpr int WARP_BYTES = Q4_STAGES * STAGE + FRESH;
+    static constexpr int GROUPS = NG * 8 * 16;            // the queries' groups, where they lie in shared memory
+    static constexpr int warp_bytes(bool FEW) { return Q4_STAGES * STAGE + FRESH + (q4_shared_groups(NB, FEW) ? GROUPS : 0); }
     static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, maximum, sum)
     static_assert(Q4_STAGES * STAGE >= 8 * SLOT * 4, "a partial result fits the ring that it is kept in");
 };
@@ -111,6 +121,11 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 // x, y as fp16 pairs hi + lo
@@ -291,17 +306,24 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 // 128 dims, the other form against FEW (both before keys were centred): one sequence of 131072 positions 48.8
 // -> 40.6 us, 128 ragged ones 95.6 -> 77.4; one head (GPT-2, 700 positions) 7.8
 // -> 7.5.  Eight heads would take FEW twice, at 0.83 of the other's time each.
+struct __align__(16) QGroup {  // of a head's q
+    float w;     // factor of the group's whole numbers (a power of two; 1 for the head's largest)
+    float sum;   // their sum, times w
+    int hi, lo;  // -8 times the sums of their upper two bytes (as one number) and of the lower two
+};
 template <int NB, bool FEW> struct State {
     static constexpr int HL = FEW ? 1 : 2;  // heads of a lane
     static constexpr int LP = FEW ? 2 : 4;  // products of q's bytes
+    static constexpr bool SH = q4_shared_groups(NB, FEW);
     uint32_t q[LP][NB][2];                  // q as matrix operands
-    float w[Q4<NB>::NG][HL];                // factor of the group's whole numbers (a power of two; 1 for the largest)
-    float qsum[Q4<NB>::NG][HL], qfac[HL];   // sums of the whole numbers, times w; the factor of the scores
-    int c8[Q4<NB>::NG][HL][2];              // -8 times the sums of q's upper two bytes (as one number) and of the lower two
+    QGroup own[SH ? 1 : Q4<NB>::NG][HL];    // this lane's heads' groups, or
+    const QGroup *shared;                   // where they lie: [group][8 heads] from this lane's first head on
+    float qfac[HL];                         // the factor of the scores
     float2 o[2 * NB][2];                    // dims x this lane's two columns
     float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p (m + 7.5 d), sum p
-    float mx[HL];                           // maximum of s over qfac; p is 2^(s - max + 29 - vexp)
-    int vexp;                               // largest exponent field of the values' d so far
+    float mx[HL];                           // maximum of s over qfac; p is 2^(s - max)
+    int pe[Q4<NB>::NG][HL];                 // largest exponent field of p d so far; o is times 2^(141 - pe)
+    __device__ __forceinline__ QGroup group(int j, int hl) const { return SH ? shared[8 * j + hl] : own[SH ? 0 : j][hl]; }
 };
 
 __device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -329,7 +351,7 @@ template <int NB, bool FEW> __device__ __forceinline__ int q_head(const Q4Args &
     return FEW ? lane >> 3 : (p.j - p.kh * g.HG) * 8 + (lane >> 2);
 }
 template <int NB, bool FEW>
-__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], State<NB, FEW> &st) {
+__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], State<NB, FEW> &st, QGroup *groups) {
     using S = State<NB, FEW>;
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
@@ -396,18 +418,22 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
             const int hi = __shfl_sync(0xffffffffu, sum[j][0], 8 * t + 4 * hl), lo = __shfl_sync(0xffffffffu, sum[j][1], 8 * t + 4 * hl);
             // (2^-126 for less: below what a score can show)
             const float w = __uint_as_float((uint32_t)max(127 + __shfl_sync(0xffffffffu, ex[j] - top, 8 * t + 4 * hl), 1) << 23);
-            st.w[j][hl] = w;
-            st.qsum[j][hl] = (fmaf((float)hi, 65536.0f, (float)lo) + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl)) * w;  // (one rounding)
-            st.c8[j][hl][0] = -8 * hi;
-            st.c8[j][hl][1] = -8 * lo;
+            const float all = (fmaf((float)hi, 65536.0f, (float)lo) + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl)) * w;  // (one rounding)
+            const QGroup q = {w, all, -8 * hi, -8 * lo};
+            if (!S::SH) st.own[S::SH ? 0 : j][hl] = q;
+            else if (lane < 4) groups[8 * j + 2 * t + hl] = q;
             st.om[j][hl] = 0.0f;
+            st.pe[j][hl] = Q4_PE_MIN;
         }
         st.l[hl] = 0.0f;
         st.mx[hl] = -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = make_float2(0.0f, 0.0f);
-    st.vexp = 0;
+    if (S::SH) {
+        st.shared = groups + 2 * t;
+        __syncwarp();
+    }
 }
 
 // The new K and V rows quantized into `fresh` (two rows) and, by the first
@@ -474,6 +500,9 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
 #pragma unroll
         for (int j = 0; j < NG; j++) {
             int c[S::LP][4] = {};
+            QGroup qg[HL];
+#pragma unroll
+            for (int hl = 0; hl < HL; hl++) qg[hl] = st.group(j, hl);
 #pragma unroll
             for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
                 const uint32_t w0 = k0[4 * i], w1 = k1[4 * i];
@@ -491,15 +520,14 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
                     // and 2^24 + 2^16, off by 1 at most
                     const int hi = FEW ? c[0][2 * r] * 256 + c[0][2 * r + 1] : c[0][2 * r + hl] * 256 + c[1][2 * r + hl];
                     const int lo = FEW ? c[1][2 * r] * 256 + c[1][2 * r + 1] : c[S::LP - 2][2 * r + hl] * 256 + c[S::LP - 1][2 * r + hl];
-                    float x = fmaf((float)(hi + st.c8[j][hl][0]), 65536.0f, (float)(lo + st.c8[j][hl][1]));
-                    if (NG > 1) x *= st.w[j][hl];
-                    s[h][r][hl] = fmaf(m, st.qsum[j][hl], j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
+                    float x = fmaf((float)(hi + qg[hl].hi), 65536.0f, (float)(lo + qg[hl].lo));
+                    if (NG > 1) x *= qg[hl].w;
+                    s[h][r][hl] = fmaf(m, qg[hl].sum, j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
                 }
             }
         }
     }
     uint32_t vf[NH][2][NG];  // (d, m) words of the values' rows
-    uint32_t dmax = 0;
 #pragma unroll
     for (int h = 0; h < NH; h++)
 #pragma unroll
@@ -511,56 +539,82 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
 #pragma unroll
                 for (int j = 0; j < NG; j++) vf[h][r][j] = 0u;
             }
-#pragma unroll
-            for (int j = 0; j < NG; j++) dmax = max(dmax, vf[h][r][j] & 0xffffu);
         }
-    // running maximum and exponent of the values' scales
-    const int ve = max(min((int)(__reduce_max_sync(0xffffffffu, dmax) >> 10), 30), st.vexp);
-    const float up = (float)(29 - ve);
     float f[HL];
 #pragma unroll
-    for (int hl = 0; hl < HL; hl++) {
+    for (int hl = 0; hl < HL; hl++) {  // running maximum
         float m = fmaxf(s[0][0][hl], s[0][1][hl]);
 #pragma unroll
         for (int h = 1; h < NH; h++) m = fmaxf(m, fmaxf(s[h][0][hl], s[h][1][hl]));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         m = fmaxf(m, st.mx[hl]);
-        f[hl] = ex2(fmaf(st.mx[hl] - m, st.qfac[hl], (float)(st.vexp - ve)));  // (2^-inf = 0 the first time)
+        f[hl] = ex2((st.mx[hl] - m) * st.qfac[hl]);  // (2^-inf = 0 the first time)
         st.mx[hl] = m;
         float l = 0.0f;  // (a tile's sums by themselves: small terms would be lost one by one beside a large one)
 #pragma unroll
         for (int h = 0; h < NH; h++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                s[h][r][hl] = ex2(fmaf(s[h][r][hl] - m, st.qfac[hl], up));
+                s[h][r][hl] = ex2((s[h][r][hl] - m) * st.qfac[hl]);
                 l += s[h][r][hl];
             }
         st.l[hl] = fmaf(st.l[hl], f[hl], l);
     }
-    const float2 ff = make_float2(f[0], f[HL - 1]);
-    st.vexp = ve;
+    // largest p d of each group and head: the upper halves of two of them in a word
+    uint32_t top[(NG * HL + 1) / 2] = {};
+#pragma unroll
+    for (int j = 0; j < NG; j++)
+#pragma unroll
+        for (int hl = 0; hl < HL; hl++) {
+            float x = 0.0f;
+#pragma unroll
+            for (int h = 0; h < NH; h++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) x = fmaxf(x, s[h][r][hl] * __low2float(*reinterpret_cast<const __half2 *>(&vf[h][r][j])));
+            const int i = j * HL + hl;
+            top[i / 2] = __byte_perm(top[i / 2], __float_as_uint(x), i % 2 ? 0x7610 : 0x3276);
+        }
+#pragma unroll
+    for (int i = 0; i < (NG * HL + 1) / 2; i++)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top[i] = max_u16x2(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
 #pragma unroll
     for (int j = 0; j < NG; j++) {
         constexpr int PB = FEW ? 1 : 2;  // products of p d
         uint32_t b[NH][PB][2];           // p d of the 16 rows of each set: rows 2 g, 2 g + 1
-        float om[HL] = {};
+        float om[HL] = {}, up[HL], ff[HL];
+#pragma unroll
+        for (int hl = 0; hl < HL; hl++) {
+            const int i = j * HL + hl, was = st.pe[j][hl];
+            // the largest so far goes down with its weight
+            const int now = max((int)(top[i / 2] >> (16 * (i % 2) + 7) & 0xffu), was - 127 + (int)(__float_as_uint(f[hl]) >> 23 & 0xffu));
+            const int e = st.pe[j][hl] = min(max(now, Q4_PE_MIN), Q4_PE_MAX);
+            up[hl] = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
+            ff[hl] = f[hl] * __uint_as_float((uint32_t)(127 + was - e) << 23);
+        }
+        const float2 ff2 = make_float2(ff[0], ff[HL - 1]);
 #pragma unroll
         for (int h = 0; h < NH; h++) {
             const float2 d0 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][0][j])), d1 = __half22float2(*reinterpret_cast<const __half2 *>(&vf[h][1][j]));
             const float m0 = fmaf(7.5f, d0.x, d0.y), m1 = fmaf(7.5f, d1.x, d1.y);
+            float x0[HL], x1[HL];
 #pragma unroll
-            for (int hl = 0; hl < HL; hl++) om[hl] = fmaf(s[h][0][hl], m0, fmaf(s[h][1][hl], m1, om[hl]));
+            for (int hl = 0; hl < HL; hl++) {
+                om[hl] = fmaf(s[h][0][hl], m0, fmaf(s[h][1][hl], m1, om[hl]));
+                x0[hl] = s[h][0][hl] * d0.x * up[hl];
+                x1[hl] = s[h][1][hl] * d1.x * up[hl];
+            }
             uint32_t hi, lo;
             if (FEW) {
-                split2(s[h][0][0] * d0.x, s[h][1][0] * d1.x, hi, lo);
+                split2(x0[0], x1[0], hi, lo);
                 b[h][0][0] = turned(__byte_perm(hi, lo, 0x5410));  // row 2 g: (hi, lo)
                 b[h][0][1] = turned(__byte_perm(hi, lo, 0x7632));
             } else {
-                split2(s[h][0][0] * d0.x, s[h][0][HL - 1] * d0.x, hi, lo);  // row 2 g: both heads
+                split2(x0[0], x0[HL - 1], hi, lo);  // row 2 g: both heads
                 b[h][0][0] = turned(hi);
                 b[h][PB - 1][0] = turned(lo);
-                split2(s[h][1][0] * d1.x, s[h][1][HL - 1] * d1.x, hi, lo);
+                split2(x1[0], x1[HL - 1], hi, lo);
                 b[h][0][1] = turned(hi);
                 b[h][PB - 1][1] = turned(lo);
             }
@@ -595,8 +649,8 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                st.o[i + e][0] = fma2(st.o[i + e][0], ff, make_float2(c[e][0], c[e][1]));
-                st.o[i + e][1] = fma2(st.o[i + e][1], ff, make_float2(c[e][2], c[e][3]));
+                st.o[i + e][0] = fma2(st.o[i + e][0], ff2, make_float2(c[e][0], c[e][1]));
+                st.o[i + e][1] = fma2(st.o[i + e][1], ff2, make_float2(c[e][2], c[e][3]));
             }
         }
     }
@@ -610,7 +664,6 @@ template <int NB, bool FEW>
 __device__ __forceinline__ void result(const State<NB, FEW> &st, int lane, float *dst, int ld, int heads, bool fin, bool vec) {
     using S = State<NB, FEW>;
     const int gq = lane >> 2, t = lane & 3;
-    const float down = __uint_as_float((uint32_t)(127 - 29 + st.vexp) << 23);  // takes the probabilities' 2^(29 - vexp) back
 #pragma unroll
     for (int hl = 0; hl < S::HL; hl++) {
         const int h = S::HL * t + hl;
@@ -619,21 +672,23 @@ __device__ __forceinline__ void result(const State<NB, FEW> &st, int lane, float
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         if (!fin && gq == 0 && h < heads) {
             dst[h * ld + Q4<NB>::DH] = st.mx[hl] * st.qfac[hl];
-            dst[h * ld + Q4<NB>::DH + 1] = l * down;
+            dst[h * ld + Q4<NB>::DH + 1] = l;
         }
-        const float iv = fin ? 1.0f / l : down;
+        const float iv = fin ? 1.0f / l : 1.0f;
 #pragma unroll
         for (int j = 0; j < Q4<NB>::NG; j++) {
             float m = st.om[j][hl];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+            // 2^(pe - 142) and, for the nibbles whose codes are times 16, 2^(pe - 146) (0 below 2^-126)
+            const float low = __uint_as_float((uint32_t)(st.pe[j][hl] - 15) << 23), high = low * 0.0625f;
             const bool half = NB % 2 && j == Q4<NB>::NG - 1;
 #pragma unroll
             for (int k = 0; k < (half ? 1 : 2); k++) {
                 const float2 *a = st.o[4 * j + 2 * k], *b = st.o[4 * j + 2 * k + 1];
-                auto col = [&](const float2 &v) { return 0.5f * (FEW ? v.x + v.y : hl ? v.y : v.x); };  // (hi and lo, or the head's)
-                const float4 v = make_float4((col(a[0]) + m) * iv, fmaf(col(a[1]), 0.0625f, m) * iv, (col(b[0]) + m) * iv,
-                                             fmaf(col(b[1]), 0.0625f, m) * iv);
+                auto col = [&](const float2 &v) { return FEW ? v.x + v.y : hl ? v.y : v.x; };  // (hi and lo, or the head's)
+                const float4 v = make_float4(fmaf(col(a[0]), low, m) * iv, fmaf(col(a[1]), high, m) * iv, fmaf(col(b[0]), low, m) * iv,
+                                             fmaf(col(b[1]), high, m) * iv);
                 float *o = dst + h * ld + 64 * j + (half ? 4 * gq : 8 * gq + 4 * k);
                 if (h >= heads) continue;
                 if (vec) *reinterpret_cast<float4 *>(o) = v;
@@ -696,9 +751,9 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
     auto cta_of = [&](int unit) { return unit < more * (per + 1) ? unit / (per + 1) : more + (unit - more * (per + 1)) / per; };
     const int cta = blockIdx.x, c0 = cta * per + min(cta, more), cn = per + (cta < more);
     const int wn = cn / Q4_WARPS, wm = cn % Q4_WARPS, u0 = c0 + warp * wn + min(warp, wm), u1 = u0 + wn + (warp < wm);
-    uint8_t *const ring = smem + warp * Q4<NB>::WARP_BYTES;
+    uint8_t *const ring = smem + warp * Q4<NB>::warp_bytes(FEW);
     uint32_t *const fresh = reinterpret_cast<uint32_t *>(ring + Q4_STAGES * Q4<NB>::STAGE);
-    float *const slots = reinterpret_cast<float *>(smem + Q4_WARPS * Q4<NB>::WARP_BYTES);  // [warp][GH][SLOT]
+    float *const slots = reinterpret_cast<float *>(smem + Q4_WARPS * Q4<NB>::warp_bytes(FEW));  // [warp][GH][SLOT]
     const size_t hstride = (size_t)a.nsplit * (DH + 2);
 
     if (u0 < u1) {
@@ -802,7 +857,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                 float x[NB][8];
                 fetch_q<NB>(g, *ii, lane, q_head<NB, FEW>(g, *ii, lane), x);
                 if (a.append && end == nt) append<NB>(g, *ii, fresh, lane);  // (while q is on its way)
-                load_q<NB, FEW>(g, *ii, lane, x, st);
+                load_q<NB, FEW>(g, *ii, lane, x, st, reinterpret_cast<QGroup *>(reinterpret_cast<uint8_t *>(fresh) + Q4<NB>::FRESH));
                 begin = false;
             }
             if (!g.bulk) {
@@ -877,7 +932,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             float4 v[PARTS], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int q = 0; q < PARTS; q++) {
-                const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::WARP_BYTES) : slots + (q / 2) * GH * SLOT) + h * SLOT;
+                const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::warp_bytes(FEW)) : slots + (q / 2) * GH * SLOT) + h * SLOT;
                 m[q] = -INFINITY;
                 if (parts >> q & 1) {
                     m[q] = s[DH];
@@ -994,9 +1049,9 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
 
 template <int NB, bool FEW> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
     const int GH = g.a.H / g.a.Hkv < 8 ? g.a.H / g.a.Hkv : 8;
-    const size_t smem = (size_t)Q4_WARPS * Q4<NB>::WARP_BYTES + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
+    const size_t smem = (size_t)Q4_WARPS * Q4<NB>::warp_bytes(FEW) + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
     // the most that any G takes: threads that call with different ones set the same value
-    constexpr int MOST = Q4_WARPS * Q4<NB>::WARP_BYTES + Q4_WARPS * (FEW ? 4 : 8) * Q4<NB>::SLOT * (int)sizeof(float);
+    constexpr int MOST = Q4_WARPS * Q4<NB>::warp_bytes(FEW) + Q4_WARPS * (FEW ? 4 : 8) * Q4<NB>::SLOT * (int)sizeof(float);
     LMC_CUDA_TRY(cudaFuncSetAttribute((k_attn_q4<NB, FEW>), cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
     const int most = lmc_sm_count() * (smem + 2048 <= 114 * 1024 ? 2 : 1), want = max_units / g.rmin;
     LMC_LAUNCH("attention (4-bit rows)", (k_attn_q4<NB, FEW>), want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);

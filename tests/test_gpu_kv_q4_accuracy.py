@@ -108,3 +108,44 @@ def test_queries_of_unequal_channels(cuda, G, where, r):
     held = sum(2.0 ** -30 * a[:, g:g + 64].max(-1) * kk[:, :, g:g + 64].sum(-1).max(-1) for g in (0, 64))
     size = np.einsum("hnd,hd->hn", kk, a).max(-1)
     check(out, q, kv, vv, (held + 8 * 2.0 ** -24 * size) / np.sqrt(Dh))
+
+
+def scores_bound(q, k):
+    """ds of ordinary queries: products of at least 22 bits and 18 fp32
+    roundings of at most 2^-24 of sum |q k|, as in the other attention tests."""
+    G = q.shape[0] // k.shape[0]
+    size = np.einsum("hnd,hd->hn", np.abs(np.repeat(k, G, 0)), np.abs(q.astype(np.float64))).max(-1)
+    return (2.0 ** -22 + 18 * 2.0 ** -24) * size / np.sqrt(q.shape[1])
+
+
+@pytest.mark.parametrize("G", [1, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("Dh,large,small", [(128, 3e3, 3e-3), (128, 3e3, 3e-4), (128, 9e4, 3e-4), (96, 9e4, 3e-4), (256, 9e4, 3e-4)])
+def test_value_groups_of_unequal_size(cuda, G, Dh, large, small):
+    """Groups of a head's values that are far larger than the next: each
+    keeps its own accuracy."""
+    rng = np.random.default_rng(G + Dh)
+    n, Hkv = 150, 2
+    q, k = rows_of(rng, (Hkv * G, Dh)), rows_of(rng, (Hkv, n, Dh))
+    for order in ((large, small), (small, large)):
+        v = rng.uniform(-0.5, 0.5, (Hkv, n, Dh)) * np.where(np.arange(Dh) // 64 % 2, order[1], order[0])
+        out, kv, vv = decode(cuda, q, k, v.astype(np.float32))
+        check(out, q, kv, vv, scores_bound(q, kv))
+
+
+@pytest.mark.parametrize("G", [1, 4, 5, 8])
+@pytest.mark.parametrize("at", [3, 100])
+def test_large_value_of_a_row_without_weight(cuda, G, at):
+    """A row whose values are 1e7 times the others' and whose weight is below
+    e^-45 for one head of each group, 1 for the next: the heads that do not
+    see it keep their accuracy."""
+    rng = np.random.default_rng(G)
+    n, Hkv, Dh = 150, 1, 128
+    q, k = rows_of(rng, (G, Dh)), rows_of(rng, (Hkv, n, Dh)) * np.float32(0.3)
+    # the row's key along q of head 0, downwards (and so that no other head has it as its maximum)
+    k[0, at] = -q[0] * (60 * np.sqrt(Dh) / (q[0] @ q[0]))
+    v = rng.uniform(-0.5, 0.5, (Hkv, n, Dh)) * 3e-4
+    v[0, at] *= 1e8
+    out, kv, vv = decode(cuda, q, k.astype(np.float32), v.astype(np.float32))
+    s = kv[0] @ q[0].astype(np.float64) / np.sqrt(Dh)
+    assert s[at] < s.max() - 45
+    check(out, q, kv, vv, scores_bound(q, kv))
