@@ -1124,8 +1124,8 @@ extern "C" int lmc_attn_q4_status(void) {
     int v = 0;
     LMC_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_attn_q4_err, sizeof(int)));
     if (!v) return LMC_OK;
-    const int zero = 0;
-    LMC_CUDA_TRY(cudaMemcpyToSymbol(g_attn_q4_err, &zero, sizeof(int)));
+    const int left = v & 2 ? v & ~2 : 0;  // one error a call: what is not reported now stays for the next
+    LMC_CUDA_TRY(cudaMemcpyToSymbol(g_attn_q4_err, &left, sizeof(int)));
     if (v & 2) return lmc_set_error(LMC_ERR_TIMEOUT, "4-bit attention: a bounded wait ran out (bulk copy not completed)");
     return lmc_set_error(LMC_ERR_INVALID, "paged attention: a page id outside the pool (page 0 read instead)");
 }
