@@ -61,14 +61,17 @@ int lmc_device_status(void);
  * the GEMV, GEMM and 4-bit attention, the grid barriers of the persistent
  * decode step - in nanoseconds; 0 restores the default of one second.  A wait that runs out
  * records a timeout that lmc_device_status reports; the kernel drains its
- * own copies and returns, and the context stays usable.  No counterpart in
- * LMc (a CPU program has no device waits). */
+ * own copies and returns, and the context stays usable.  Of 4-bit attention
+ * the outputs that needed what did not arrive are NaN, and new rows behind
+ * them may not be in the cache.  No counterpart in LMc (a CPU program has no
+ * device waits). */
 int lmc_set_wait_limit(long long ns);
 /* Self-test of that failure path: runs a device wait that nothing can
  * complete - which = 0: a GEMV ring's mbarrier wait, 1: a persistent-step
- * grid barrier (two CTAs), 2: the 4-bit attention's copy ring - under the
- * current limit.  Returns LMC_ERR_TIMEOUT
- * when the wait ran out as designed (and clears the recorded timeout). */
+ * grid barrier (two CTAs), 2: the 4-bit attention's copy ring, 3: calls of
+ * the 4-bit attention with a tile that never arrives, whose outputs have to
+ * be NaN - under the current limit.  Returns LMC_ERR_TIMEOUT when the wait
+ * ran out as designed (and clears the recorded timeout). */
 int lmc_wait_selftest(int which);
 
 /* Select and initialise CUDA device `device` for the calling thread.

@@ -43,6 +43,7 @@
 // others.
 #include <algorithm>
 #include <type_traits>
+#include <vector>
 
 #include "attention.cuh"
 #include "kv_q4.cuh"
@@ -82,6 +83,7 @@ struct Q4Args {
     int bulk;       // every run of rows starts on a 16-byte boundary, four rows are whole 16-byte pieces
     int run;        // rows that lie together: a page's, at most a tile's
     long long page_bytes; // of one kv head's rows of a page
+    int lose_j, lose_tile; // self-test: warps with this tile of a sequence's item j wait for bytes that never come (-1: none)
 };
 
 template <int NB> struct Q4 {
@@ -197,6 +199,7 @@ struct Item {
 };
 struct Part {  // of an item, left in shared memory by a warp: its first unit, sequence, heads, tiles [first, end) of nt
     int unit, b, head, heads, first, end, nt;
+    int lost;  // a wait ran out: there is no result
 };
 __device__ __forceinline__ int seq_pos(const Q4Args &g, int b) {  // position, or -1 when the row has nothing to do
     const int p = __ldg(g.a.pos + b);
@@ -698,6 +701,27 @@ __device__ __forceinline__ void result(const State<NB, FEW> &st, int lane, float
     }
 }
 
+// After a wait that ran out: the rest of the warp's share, from the item `at` on,
+// has no result.  Its heads' outputs become NaN, here or where parts are merged.
+template <int NB> __device__ __noinline__ void lose_items(const Q4Args &g, Item *at, Part *desc, int part, int lane) {
+    const AttnArgs &a = g.a;
+    constexpr int DH = Q4<NB>::DH;
+    while (at->tile < at->end) {
+        const int h0 = (at->j - at->kh * g.HG) * 8, heads = min(8, g.G - h0), head = at->kh * g.G + h0;
+        if (at->tile == 0 && at->end == at->nt) {
+            float *o = a.out + (size_t)at->b * a.ldo + (size_t)head * DH;
+            for (int i = lane; i < heads * DH; i += 32) o[i] = NAN;
+            if (lane < heads && a.nsplit > 1)
+                a.ws[((size_t)at->b * a.H + head + lane) * ((size_t)a.nsplit * (DH + 2)) + DH + 1] = 0.0f;
+        } else if (lane == 0) {
+            desc[part] = Part{at->unit, at->b, head, heads, at->tile, at->end, at->nt, 1};
+        }
+        part = 1;
+        if (!more_items(g, at)) break;
+        next_item<NB>(g, at);
+    }
+}
+
 template <int NB, bool FEW>
 __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_constant__ Q4Args g) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -800,9 +824,11 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         auto look_up = [&]() {
             if (a.pages && a_tile * T + r0 < a_rows && r0 < T) a_pg = __ldg(ia->row + ((a_tile * T + r0) >> a.page_shift));
         };
-        auto item_ahead = [&]() {
+        auto item_ahead = [&](int i) {  // its first tile goes into stage i
             a_tile = ia->tile;
             a_end = ia->end;
+            if (ia->j == g.lose_j && a_tile <= g.lose_tile && g.lose_tile < a_end && lane == 0)
+                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], 16;" ::"r"(bar + 8 * i) : "memory");
             a_rows = a.append ? ia->pos : ia->pos + 1;
             look_up();
         };
@@ -828,7 +854,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                 bulk_copy(stage + to, cache + off, min(g.run, some - r0) * RB, bar + 8 * i);
             }
         };
-        item_ahead();
+        item_ahead(0);
         int tile = p.tile, end = p.end, nt = p.nt, phase = 0, part = 0, stage = 0, fill = 0;
         uint32_t parity = 0, flying = 0;  // phase bits of the stages' barriers; stages whose copies are not waited for
         bool begin = true;
@@ -841,7 +867,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                 if (++a_tile == a_end) {
                     if (more_items(g, ia)) {
                         next_item<NB>(g, ia);
-                        item_ahead();
+                        item_ahead(fill + 1 == Q4_STAGES ? 0 : fill + 1);
                     } else {
                         a_tile = a_end = 0;
                     }
@@ -866,7 +892,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             } else {
                 bool here = bar_try(bar + 8 * stage, parity >> stage & 1);
                 if (!here) here = bar_wait_long(bar + 8 * stage, parity >> stage & 1);
-                if (!__all_sync(0xffffffffu, here)) break;  // gave up: no result for this item (lmc_device_status)
+                if (!__all_sync(0xffffffffu, here)) break;  // gave up, tile < end (lmc_device_status)
                 parity ^= 1u << stage;
             }
             flying &= ~(1u << stage);
@@ -896,7 +922,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                     if (lane < heads && a.nsplit > 1)  // nothing for the combine kernel to do
                         a.ws[((size_t)b * a.H + head + lane) * hstride + DH + 1] = 0.0f;
                 } else if (lane == 0) {
-                    desc[warp][part] = Part{ii->unit, b, head, heads, first, end, nt};
+                    desc[warp][part] = Part{ii->unit, b, head, heads, first, end, nt, 0};
                 }
                 part = 1;
                 if (!more_items(g, ii)) break;
@@ -910,6 +936,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         // (after a wait that ran out) the copies still in flight, bounded again
         for (int i = 0; g.bulk && i < Q4_STAGES; i++)
             if (flying >> i & 1) bar_wait_long(bar + 8 * i, parity >> i & 1);
+        if (tile < end) lose_items<NB>(g, ii, desc[warp], part, lane);
     }
     __syncthreads();
     // merge this CTA's parts of each item: neighbours in (warp, part) order
@@ -926,6 +953,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
         // the slot is this CTA's place among those that hold the item's tiles
         const int slot = whole ? 0 : cta - cta_of(unit + Q4_ITEM);
         const bool last = !whole && cta_of(unit + Q4_ITEM + d.nt - 1) == cta;
+        const bool lost = __ballot_sync(0xffffffffu, lane < PARTS && (parts >> lane & 1) && desc[lane >> 1][lane & 1].lost);
         for (int i = threadIdx.x; i < d.heads * (DH / 4); i += 32 * Q4_WARPS) {
             const int h = i / (DH / 4), x = 4 * (i % (DH / 4));
             float M = -INFINITY, L = 0.0f, m[PARTS], l[PARTS];
@@ -934,7 +962,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             for (int q = 0; q < PARTS; q++) {
                 const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::warp_bytes(FEW)) : slots + (q / 2) * GH * SLOT) + h * SLOT;
                 m[q] = -INFINITY;
-                if (parts >> q & 1) {
+                if ((parts >> q & 1) && !lost) {
                     m[q] = s[DH];
                     l[q] = s[DH + 1];
                     v[q] = *reinterpret_cast<const float4 *>(s + x);
@@ -943,7 +971,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             }
 #pragma unroll
             for (int q = 0; q < PARTS; q++)
-                if (parts >> q & 1) {
+                if ((parts >> q & 1) && !lost) {
                     const float f = ex2(m[q] - M);
                     L = fmaf(l[q], f, L);
                     acc.x = fmaf(v[q].x, f, acc.x);
@@ -951,6 +979,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                     acc.z = fmaf(v[q].z, f, acc.z);
                     acc.w = fmaf(v[q].w, f, acc.w);
                 }
+            if (lost) L = NAN;  // (and with it the item's output)
             float *w = a.ws + ((size_t)d.b * a.H + d.head + h) * hstride;
             if (whole) {
                 const float iv = 1.0f / L;
@@ -1060,9 +1089,11 @@ template <int NB, bool FEW> int launch(const Q4Args &g, int max_units, cudaStrea
 
 }  // namespace
 
-extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t ws_bytes, cudaStream_t s) {
+static int q4_launch(const AttnArgs *args, int batch, size_t ws_bytes, int lose_j, int lose_tile, cudaStream_t s) {
     Q4Args g;
     g.a = *args;
+    g.lose_j = lose_j;
+    g.lose_tile = lose_tile;
     AttnArgs &a = g.a;
     if (a.S > 1 << 30) return lmc_set_error(LMC_ERR_UNSUPPORTED, "attention: 4-bit rows take contexts of at most 2^30 positions (%d)", a.S);
     // one part per head and workspace slot: the most slots that fit, up to the plan's
@@ -1098,6 +1129,10 @@ extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t w
     return LMC_OK;
 }
 
+extern "C" int lmc_attention_q4_launch(const AttnArgs *args, int batch, size_t ws_bytes, cudaStream_t s) {
+    return q4_launch(args, batch, ws_bytes, -1, -1, s);
+}
+
 extern "C" int lmc_attn_q4_set_wait_limit(long long ns) {
     const long long v = ns > 0 ? ns : 1000000000ll;
     LMC_CUDA_TRY(cudaMemcpyToSymbol(g_attn_q4_wait_ns, &v, sizeof v));
@@ -1117,6 +1152,67 @@ __global__ void k_attn_q4_wait_selftest(int *gave_up) {
 extern "C" int lmc_attn_q4_wait_selftest(int *d_flag, cudaStream_t s) {
     k_attn_q4_wait_selftest<<<1, 32, 0, s>>>(d_flag);
     LMC_LAUNCH_CHECK("wait self-test");
+    return LMC_OK;
+}
+
+// Failure-path self-test: attention over rows of zeros where the copies of one
+// tile of kv head 1 never land, the workspace full of an earlier call's finite
+// numbers.  Head 1 has to be NaN wherever that tile is one of its own, and no
+// other output may be wrong (NaN, where the same warp has it behind the lost one, or 0).
+extern "C" int lmc_attn_q4_lost_selftest(cudaStream_t s) {
+    constexpr int Hkv = 2, Dh = 64, MOST = 400;
+    // sequences, positions, query heads per kv head, lost tile: an item of one warp, of one CTA, of several
+    // CTAs, items one after the other in a warp's share, rows of several workspaces' length
+    static const int cases[][4] = {{2, 40, 1, 0}, {1, 128, 4, 1}, {1, 128, 8, 0}, {1, 4096, 1, 20}, {3, 4000, 8, 61}, {MOST, 200, 1, 2}};
+    float *out = nullptr;
+    uint8_t *cache = nullptr;
+    int rc = LMC_OK;
+    for (const auto &c : cases) {
+        const int B = c[0], S = (c[1] + 3) & ~3, H = Hkv * c[2];
+        const size_t rows = (size_t)B * Hkv * S * kv_q4_row_bytes(Dh), ws = lmc_attention_workspace_bytes(B, H, Dh, S);
+        const size_t q = (size_t)B * H * Dh, kv = (size_t)B * Hkv * Dh;
+        std::vector<float> got(q);
+        std::vector<int> pos(B, c[1] - 1);
+        AttnArgs a = {};
+        cudaError_t e = cudaMalloc((void **)&cache, 2 * rows);
+        if (e == cudaSuccess) e = cudaMalloc((void **)&out, (2 * q + kv) * sizeof(float) + (size_t)B * sizeof(int) + ws);
+        float *const dq = out + q, *const dkv = dq + q;
+        int *const dpos = reinterpret_cast<int *>(dkv + kv);
+        if (e == cudaSuccess) e = cudaMemsetAsync(cache, 0, 2 * rows, s);
+        if (e == cudaSuccess) e = cudaMemsetAsync(out, 0, (2 * q + kv) * sizeof(float), s);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(dpos, pos.data(), (size_t)B * sizeof(int), cudaMemcpyHostToDevice, s);
+        if (e == cudaSuccess) e = cudaMemsetAsync(dpos + B, 0x3f, ws, s);
+        if (e == cudaSuccess) {
+            a.out = out;
+            a.q = dq;
+            a.k_new = a.v_new = dkv;
+            a.k_cache = cache;
+            a.v_cache = cache + rows;
+            a.pos = dpos;
+            a.H = H;
+            a.Hkv = Hkv;
+            a.Dh = Dh;
+            a.S = S;
+            a.ldo = a.ldq = H * Dh;
+            a.ldkv = Hkv * Dh;
+            a.append = 1;
+            a.ws = reinterpret_cast<float *>(dpos + B);
+            rc = q4_launch(&a, B, ws, 1, c[3], s);
+            e = cudaMemcpyAsync(got.data(), out, q * sizeof(float), cudaMemcpyDeviceToHost, s);
+            if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+        }
+        cudaFree(cache);
+        cudaFree(out);
+        cache = nullptr;
+        out = nullptr;
+        if (rc != LMC_OK) return rc;
+        if (e != cudaSuccess) return lmc_set_error(LMC_ERR_CUDA, "wait self-test: %s", cudaGetErrorString(e));
+        for (size_t i = 0; i < q; i++) {
+            const bool mine = (int)(i / Dh % H) / c[2] == 1;
+            if (mine ? got[i] == got[i] : got[i] != 0.0f && got[i] == got[i])
+                return lmc_set_error(LMC_ERR_CUDA, "wait self-test: %d sequences of %d positions: output %zu is %g", B, c[1], i, got[i]);
+        }
+    }
     return LMC_OK;
 }
 

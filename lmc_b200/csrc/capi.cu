@@ -45,12 +45,16 @@ extern "C" int lmc_set_wait_limit(long long ns) {
 }
 
 extern "C" int lmc_wait_selftest(int which) {
-    if (which < 0 || which > 2) return lmc_set_error(LMC_ERR_INVALID, "wait_selftest: %d", which);
+    if (which < 0 || which > 3) return lmc_set_error(LMC_ERR_INVALID, "wait_selftest: %d", which);
     int *d = NULL;
     LMC_CUDA_TRY(cudaMalloc((void **)&d, sizeof(int)));
     LMC_CUDA_TRY(cudaMemset(d, 0, sizeof(int)));
     int rc;
-    if (which != 1) {
+    if (which == 3) {
+        rc = lmc_attn_q4_lost_selftest(0);
+        if (!rc) rc = lmc_device_status();
+        if (rc == LMC_OK) rc = lmc_set_error(LMC_ERR_CUDA, "wait self-test: timeout not recorded");
+    } else if (which != 1) {
         rc = which == 0 ? lmc_tiled_wait_selftest(d, 0) : lmc_attn_q4_wait_selftest(d, 0);
         if (!rc && cudaDeviceSynchronize() != cudaSuccess) rc = lmc_set_error(LMC_ERR_CUDA, "wait self-test sync");
         int gave_up = 0;

@@ -134,6 +134,7 @@ int lmc_kv_append_launch(const float *k, const float *v, int ldk, int ldv, void 
 /* LMC_OK, or LMC_ERR_INVALID once after a kernel of that file met an index
  * outside its range (the flag is cleared). */
 int lmc_attn_q4_wait_selftest(int *d_flag, cudaStream_t s);
+int lmc_attn_q4_lost_selftest(cudaStream_t s);
 int lmc_attn_q4_status(void);
 int lmc_attn_q4_set_wait_limit(long long ns);
 int lmc_kv_rows_status(void);

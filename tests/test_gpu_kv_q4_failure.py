@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from lmc_b200 import runtime as rt
-from tests.test_gpu_kv_q4 import Cache, INVALID, TIMEOUT, dev, rows_of
+from tests.test_gpu_kv_q4 import Cache, INVALID, TIMEOUT, attend, dev, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +24,17 @@ def test_both_errors_are_reported(cuda):
         rt.call("lmc_set_wait_limit", 0)
     assert rt.lib().lmc_device_status() == INVALID and b"page id" in rt.lib().lmc_last_error()
     assert rt.lib().lmc_device_status() == 0
+
+
+def test_lost_tiles_make_their_outputs_nan(cuda):
+    """Calls where one tile of a kv head never arrives: the self-test reports
+    the timeout only if that head is NaN in every sequence that has the tile
+    and nothing else is wrong (parts of a warp, a CTA and several CTAs, with
+    an earlier call's numbers in the workspace); the next call is right."""
+    rt.call("lmc_set_wait_limit", 2_000_000)  # 2 ms
+    try:
+        assert rt.lib().lmc_wait_selftest(3) == TIMEOUT, rt.lib().lmc_last_error()
+        assert rt.lib().lmc_device_status() == 0
+    finally:
+        rt.call("lmc_set_wait_limit", 0)
+    attend(cuda, 61, [100, 20], 2, 4, 64, 128, 16)
