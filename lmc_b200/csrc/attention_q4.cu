@@ -61,9 +61,6 @@ constexpr int Q4_STAGES = 2;  // tiles in a warp's ring
 // 4 kv heads, eight query heads each, 18.9, 18.7, 19.1.
 constexpr int Q4_ITEM = 2;
 constexpr float LOG2E = 1.4426950408889634f;
-// Exponent fields of p d that a scale is made for: 2^(141 - field) is a normal
-// number, and p d is at most 65504.
-constexpr int Q4_PE_MIN = 15, Q4_PE_MAX = 142;
 // Limit of a wait for bulk copies (nanoseconds of %globaltimer).
 __device__ long long g_attn_q4_wait_ns = 1000000000ll;
 
@@ -120,6 +117,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
           "l"(reinterpret_cast<unsigned long long &>(c)));
     return r;
 }
+// Exponent field of p d, as far as a scale is made for it: 2^(141 - field) is a
+// normal number, and p d is at most 65504.
+__device__ __forceinline__ int pd_exponent(float x) { return min(max((int)(__float_as_uint(x) >> 23), 15), 142); }
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -325,7 +325,7 @@ template <int NB, bool FEW> struct State {
     float2 o[2 * NB][2];                    // dims x this lane's two columns
     float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p (m + 7.5 d), sum p
     float mx[HL];                           // maximum of s over qfac; p is 2^(s - max)
-    int pe[Q4<NB>::NG][HL];                 // largest exponent field of p d so far; o is times 2^(141 - pe)
+    float pd[Q4<NB>::NG][HL];               // largest p d so far; o is times 2^(141 - pd_exponent(pd))
     __device__ __forceinline__ QGroup group(int j, int hl) const { return SH ? shared[8 * j + hl] : own[SH ? 0 : j][hl]; }
 };
 
@@ -426,7 +426,7 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
             if (!S::SH) st.own[S::SH ? 0 : j][hl] = q;
             else if (lane < 4) groups[8 * j + 2 * t + hl] = q;
             st.om[j][hl] = 0.0f;
-            st.pe[j][hl] = Q4_PE_MIN;
+            st.pd[j][hl] = 0.0f;
         }
         st.l[hl] = 0.0f;
         st.mx[hl] = -INFINITY;
@@ -589,10 +589,10 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
         float om[HL] = {}, up[HL], ff[HL];
 #pragma unroll
         for (int hl = 0; hl < HL; hl++) {
-            const int i = j * HL + hl, was = st.pe[j][hl];
+            const int i = j * HL + hl, was = pd_exponent(st.pd[j][hl]);
             // the largest so far goes down with its weight
-            const int now = max((int)(top[i / 2] >> (16 * (i % 2) + 7) & 0xffu), was - 127 + (int)(__float_as_uint(f[hl]) >> 23 & 0xffu));
-            const int e = st.pe[j][hl] = min(max(now, Q4_PE_MIN), Q4_PE_MAX);
+            st.pd[j][hl] = fmaxf(__uint_as_float(i % 2 ? top[i / 2] & 0xffff0000u : top[i / 2] << 16), st.pd[j][hl] * f[hl]);
+            const int e = pd_exponent(st.pd[j][hl]);
             up[hl] = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
             ff[hl] = f[hl] * __uint_as_float((uint32_t)(127 + was - e) << 23);
         }
@@ -683,8 +683,8 @@ __device__ __forceinline__ void result(const State<NB, FEW> &st, int lane, float
             float m = st.om[j][hl];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-            // 2^(pe - 142) and, for the nibbles whose codes are times 16, 2^(pe - 146) (0 below 2^-126)
-            const float low = __uint_as_float((uint32_t)(st.pe[j][hl] - 15) << 23), high = low * 0.0625f;
+            // 2^(e - 142), 0 for 2^-127, and a 16th of it for the nibbles whose codes are times 16
+            const float low = __uint_as_float((uint32_t)(pd_exponent(st.pd[j][hl]) - 15) << 23), high = low * 0.0625f;
             const bool half = NB % 2 && j == Q4<NB>::NG - 1;
 #pragma unroll
             for (int k = 0; k < (half ? 1 : 2); k++) {

@@ -36,8 +36,9 @@ def decode(torch, q, k, v):
     return out.cpu().numpy().reshape(H, Dh), c.k[0], c.v[0]
 
 
-def check(out, q, k, v, ds, norm=True):
-    """Per group of 64 dims against the bound above; ds [H] or a number."""
+def check(out, q, k, v, ds, norm=True, least=0.0):
+    """Per group of 64 dims against the bound above; ds [H] or a number, `least`
+    what a weight may be off by at least."""
     (H, Dh), G = q.shape, q.shape[0] // k.shape[0]
     n = k.shape[1]
     for h in range(H):
@@ -49,7 +50,7 @@ def check(out, q, k, v, ds, norm=True):
         for g in range(0, Dh, 64):
             x, want = vv[:, g:g + 64], p @ vv[:, g:g + 64]
             worst = np.abs(out[h, g:g + 64] - want).max()
-            assert worst <= rel * 2 * (p @ np.abs(x).max(-1)), (h, g, worst / (p @ np.abs(x).max(-1)), rel)
+            assert worst <= rel * 2 * (p @ np.abs(x).max(-1)) + least * np.abs(x).max(-1).sum(), (h, g, worst / (p @ np.abs(x).max(-1)), rel)
             if norm:  # the repository's attention bound
                 assert rel_err(out[h, g:g + 64], want) < 1e-5, (h, g, rel_err(out[h, g:g + 64], want))
 
@@ -149,3 +150,36 @@ def test_large_value_of_a_row_without_weight(cuda, G, at):
     s = kv[0] @ q[0].astype(np.float64) / np.sqrt(Dh)
     assert s[at] < s.max() - 45
     check(out, q, kv, vv, scores_bound(q, kv))
+
+
+@pytest.mark.parametrize("G", [1, 5])
+@pytest.mark.parametrize("step", [0.1, 0.67, 3.0])
+@pytest.mark.parametrize("late", [0.0, 3e-4])
+def test_maximum_that_rises_in_every_tile(cuda, G, step, late):
+    """Scores that rise by `step` from one tile of 64 positions to the next
+    over the 140 tiles that a warp has, the values large in the warp's first
+    tile and small or 0 in the others: the scale of p d goes down with the
+    weight, by no more and no less.
+
+    Rows of keys are constant fp16 numbers x (d = 0, one product with sum q),
+    whose scores are off by at most 8 fp32 roundings of sum |q k| = x.  Weights
+    below 2^-126 are 0 in fp32 (steps of 0.67 and 3: e^-93 and e^-417 for the
+    large values), which takes at most 2^-126 |v| of each position."""
+    rng = np.random.default_rng(G)
+    Dh, S, tiles = 32, 1 << 22, 4 * 140  # (a context whose shares are that long: up to 1041 tiles a CTA)
+    n = 64 * tiles
+    x = (np.arange(n) // 64 * step).astype(np.float16).astype(np.float32)
+    v = rng.uniform(-0.5, 0.5, (n, Dh)) * np.where(np.arange(n) // 64 % 140 == 0, 3e3, late)[:, None]
+    q = np.full((G, Dh), np.sqrt(Dh) / Dh, np.float32)
+    (kr, k), (vr, vv) = kv_ref.q4_rows(np.repeat(x[:, None], Dh, 1)), kv_ref.q4_rows(v.astype(np.float32))
+    caches = [cuda.zeros((1, 1, S, kv_ref.row_bytes(Dh)), dtype=cuda.uint8, device="cuda") for _ in range(2)]
+    for c, r in zip(caches, (kr, vr)):
+        c[0, 0, :n - 1] = dev(cuda, r[:-1])
+    out = cuda.full((G, Dh), 5.0, device="cuda")
+    wsb = rt.lib().lmc_attention_workspace_bytes(1, G, Dh, S)
+    ws = cuda.full((wsb,), 0xff, dtype=cuda.uint8, device="cuda")
+    d = [dev(cuda, a) for a in (q, np.repeat(x[-1:], Dh), v[-1].astype(np.float32), np.array([n - 1], np.int32))]
+    rt.call("lmc_attention_decode", out.data_ptr(), *(t.data_ptr() for t in d[:3]), *(c.data_ptr() for c in caches), rt.KV_Q4,
+            d[3].data_ptr(), 1, G, 1, Dh, S, ws.data_ptr(), wsb, None)
+    assert rt.lib().lmc_device_status() == 0
+    check(out.cpu().numpy(), q, k[None], vv[None], 8 * 2.0 ** -24 * x.max(), norm=False, least=2.0 ** -126)
