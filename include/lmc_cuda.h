@@ -202,7 +202,9 @@ unsigned long long lmc_rng_seed(unsigned long long seed);
  * saturate at +-65504) and the code in 0..15 nearest to (x - m) / d, ties to
  * even (decided exactly; all 0 when d is 0).  A group with an infinity or a
  * NaN gets d = NaN: its values read back as NaN.  Such caches start on a
- * 16-byte boundary and hold at most 2^30 positions a sequence.  For `batch` sequences
+ * 16-byte boundary and hold at most 2^30 positions a sequence.  Attention over
+ * them holds a query's channel to fp32, or to 2^-30 of the largest of its group of
+ * 64 where that is more.  For `batch` sequences
  * the caches are batch consecutive [Hkv][S][Dh] slabs and q/k_new/v_new/out
  * are batch rows of H*Dh (q, out) and Hkv*Dh (k_new, v_new) floats.
  * d_pos[b] is the position written this step; positions 0..d_pos[b] are
@@ -353,6 +355,8 @@ typedef struct {
     float rope_theta, norm_eps;
 } lmc_model_config;
 
+/* kv_dtype: LMC_KV_F32, _F16, _Q8 or _Q4; with 4-bit rows the step always runs
+ * kernel by kernel, not as the persistent single-launch step. */
 int lmc_model_load(const char *gguf_path, int max_batch, int kv_dtype, lmc_model **out);
 /* Tensor-parallel shard tp_rank of tp_size (LLaMA; one process per GPU, the
  * caller selects the device first).  No counterpart in LMc, which runs on

@@ -8,10 +8,10 @@
 // (values).  Keys: integer products, q as whole numbers in four signed bytes,
 // the largest |q| of a group of 64 dims in [2^29, 2^30): a channel down to 1/64
 // of it keeps all of fp32's bits, a smaller one is off by at most 2^-30 of it.
-// Codes are centred, because sums over positive codes would be
-// large against the score, and against the result of a long, flat softmax, and
-// take their rounding with them (131072 positions, keys with a few large
-// channels: relative error 1.0e-6, centred in both 0.7e-6, for 4% more time).
+// Codes are centred, because sums over positive codes would be large against
+// the score, and against the result of a long, flat softmax, and take their
+// rounding with them (131072 positions, keys with a few large channels, q then
+// in 23 bits: relative error 1.0e-6, centred in both 0.7e-6, for 4% more time).
 //
 // A value's code as fp16: a nibble ORed into bits 1 to 4 of 1024.0 is 1024 +
 // 2 c, exactly, and 1039 less is 2 c - 15 (two instructions for two operands);
@@ -20,9 +20,10 @@
 // that keeps it just below 2^15: its largest exponent so far is tracked like the
 // running maximum, for each head and group of 64 dims, so that neither a group of
 // larger values nor a row of large values without weight takes bits from it (a p d
-// below 2^-18 of the largest is off by at most 2^-40 of that).  The matrix unit truncates its sums, so a tile's products (and its
-// sums of p and of p with the minima) go to fresh accumulators that are added
-// to the running ones in rounded fp32.
+// below 2^-18 of the largest is off by at most 2^-40 of that).  The matrix unit
+// truncates its sums, so a tile's products (and its sums of p and of p with the
+// minima) go to fresh accumulators that are added to the running ones in rounded
+// fp32.
 //
 // Work: tiles of 64 positions (32 from head size 160 on) of one (sequence, kv
 // head, 8 query heads).  All tiles of the batch, in order, are divided evenly
@@ -35,9 +36,9 @@
 // one CTA are merged in shared memory, parts in several CTAs through the
 // workspace by k_q4_combine.
 //
-// Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 42 us, 128 ragged
-// sequences of them 81 us (3.6 and 3.8 TB/s), 64 ragged ones of 4 heads of 64
-// dims 18.0 us, one of 12 heads with 700 positions 7.5 us.  Instructions bound
+// Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 44 us, 128 ragged
+// sequences of them 84 us (3.4 and 3.6 TB/s), 64 ragged ones of 4 heads of 64
+// dims 18.8 us, one of 12 heads with 700 positions 7.7 us.  Instructions bound
 // the first two (matrix, integer and half instructions share the issue), the
 // latency of a warp's chain (its share, the copies, q, a tile, the merge) the
 // others.
@@ -57,8 +58,8 @@ __device__ int g_attn_q4_err;  // bit 0: a page id outside the pool, bit 1: a wa
 constexpr int Q4_WARPS = 4;
 constexpr int Q4_STAGES = 2;  // tiles in a warp's ring
 // What beginning and ending an item costs, in tiles (q, the new row, the
-// result): 128 ragged sequences of 8 kv heads 85, 79, 80 us with 1, 2, 3; 64 of
-// 4 kv heads, eight query heads each, 18.9, 18.7, 19.1.
+// result): 128 ragged sequences of 8 kv heads 91.3, 84.1, 85.9 us with 1, 2, 3;
+// 64 of 4 kv heads, eight query heads each, 19.4, 18.8, 19.4.
 constexpr int Q4_ITEM = 2;
 constexpr float LOG2E = 1.4426950408889634f;
 // Limit of a wait for bulk copies (nanoseconds of %globaltimer).
@@ -306,9 +307,9 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 // On this chip a warp-level MMA keeps the integer and half pipes from issuing
 // (8 cycles each, measured in one loop with them), so their number counts: FEW
 // has 32 for 32 rows of 128 dims, the other form 64.  4 heads per kv head of
-// 128 dims, the other form against FEW (both before keys were centred): one sequence of 131072 positions 48.8
-// -> 40.6 us, 128 ragged ones 95.6 -> 77.4; one head (GPT-2, 700 positions) 7.8
-// -> 7.5.  Eight heads would take FEW twice, at 0.83 of the other's time each.
+// 128 dims, the other form against FEW: one sequence of 131072 positions 57.0
+// -> 44.0 us, 128 ragged ones 115.6 -> 84.1; one head (GPT-2, 700 positions) 8.1
+// -> 7.7.  Eight heads would take FEW twice, at 0.73 of the other's time each.
 struct __align__(16) QGroup {  // of a head's q
     float w;     // factor of the group's whole numbers (a power of two; 1 for the head's largest)
     float sum;   // their sum, times w
@@ -1005,7 +1006,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
 // workspace; nothing to do when slot 0's sum is zero.  W warps (1 or 4) share
 // a head's parts: four when there are few heads, whose parts are then many
 // (131072 positions of one sequence, 56 parts for each of 32 heads, the whole
-// call: 45.9 us with one, 41.5 with four; 128 sequences of 32 heads 79 and 82).
+// call: 49.3 us with one, 44.0 with four; 128 sequences of 32 heads 84.2 and 88.1).
 template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a, int batch) {
     pdl_wait();
     pdl_launch_dependents();
@@ -1027,7 +1028,7 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
             }
     };
     // Few heads: beside the slots' maxima and sums, before those tell what is in them
-    // (700 positions of 12 heads 8.3 -> 7.8 us); for many heads that reads too much.
+    // (700 positions of 12 heads 8.0 -> 7.7 us); for many heads that reads too much.
     if (W > 1) load(first, a.nsplit);
     // offsets and sums of all slots (at most 64); slots past the last part hold anything
     float m[2], l[2];
@@ -1109,7 +1110,7 @@ static int q4_launch(const AttnArgs *args, int batch, size_t ws_bytes, int lose_
     g.items_only = a.nsplit == 1;
     // an item of NT tiles then lies in at most (NT - 2) / rmin + 2 <= nsplit CTAs;
     // and a CTA has at least an item of one tile (GPT-2, 700 positions, with 1, 3, 6
-    // units a CTA: 8.7, 8.2, 9.6 us; 8 kv heads, 4000 positions: 10.8, 9.8, 10.5)
+    // units a CTA: 8.4, 7.7, 9.3 us; 8 kv heads, 4000 positions: 13.3, 10.8, 11.1)
     g.rmin = g.items_only ? 1 : NT < 2 ? Q4_ITEM + 1 : std::max((NT - 2) / (a.nsplit - 1) + 1, Q4_ITEM + 1);
     g.vec = (((uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.out) & 15) == 0 && a.ldq % 4 == 0 &&
             a.ldkv % 4 == 0 && a.ldo % 4 == 0;

@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t kv_q4_scale(float lo, float hi, float &d, fl
 // The word of codes of x (code i in bits 4 i .. 4 i + 3): the whole number
 // nearest to (x - m) / d, ties to even, clamped to 0..15; 0 when d is 0 or the
 // group is bad.  t is that quotient over 15, clamped to 0..1; 15 t is off by
-// less than 2^-18 (x - m, the reciprocal, two products), so it decides unless
+// less than 2^-17 (x - m, the reciprocal, the product), so it decides unless
 // it lies within 2e-5 of a tie; only then (one value in 25,000) is the word
 // taken again in 64 bits, where x - m is exact (or d is too small for its last
 // bit to matter) and the division cannot round across a tie of two fp16

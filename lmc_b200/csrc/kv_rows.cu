@@ -3,14 +3,14 @@
 //
 // Both stream: append reads 4 Dh bytes per row and side and writes the row's
 // form, read the reverse, so HBM bounds them, and close behind it the
-// instructions per value (4-bit append issues in 75 of 100 cycles); a thread
+// instructions per value (4-bit append issues in 74 of 100 cycles); a thread
 // therefore has the K and the V side of its rows, whose place in the cache it
 // works out once, and starts all loads before it uses the first.  LPR = 4 ..
 // 32 lanes per row, eight dims a lane: append takes neighbouring dims (a word
 // of codes, three shuffles for a group's minimum and maximum; 16 bytes of
 // fp16), read two runs of four (stores without gaps).
 // 32000 rows of 8 x 128, append / read: 4-bit 61 / 50 us (4.9 / 5.9 TB/s),
-// int8 60 / 54 us, fp16 59 / 61 us (6.7 / 6.4 TB/s); 509 rows of 4 x 64 take
+// int8 60 / 54 us, fp16 59 / 61 us (6.7 / 6.4 TB/s), fp32 80 / 79 us (6.6 TB/s); 509 rows of 4 x 64 take
 // 2.9 / 1.8 us in 4 bits, most of it latency.
 #include <type_traits>
 
