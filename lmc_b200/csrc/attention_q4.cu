@@ -1,17 +1,18 @@
 // attention_q4.cu - decode attention over 4-bit K/V rows (LMC_KV_Q4).
 //
 // With codes c and (d, m) of group j (64 dims) of row t:
-//   s_t = sum_j [ d_tj (q_j . (c_tj - 8)) + (m_tj + 8 d_tj) sum(q_j) ] / sqrt(Dh)
+//   s_t = sum_j [ d_tj (q_j . c_tj) + m_tj sum(q_j) ] / sqrt(Dh)
 //   o_j = sum_t p_t d_tj (2 c_tj - 15) / 2 + sum_t p_t (m_tj + 7.5 d_tj),   p_t = 2^(s_t log2 e - max)
 // so the matrix units only ever see whole numbers and fp32 factors; the scales
 // are applied per group outside (keys) or folded into the probabilities
 // (values).  Keys: integer products, q as whole numbers in four signed bytes,
 // the largest |q| of a group of 64 dims in [2^29, 2^30): a channel down to 1/64
 // of it keeps all of fp32's bits, a smaller one is off by at most 2^-30 of it.
-// Codes are centred, because sums over positive codes would be large against
-// the score, and against the result of a long, flat softmax, and take their
-// rounding with them (131072 positions, keys with a few large channels, q then
-// in 23 bits: relative error 1.0e-6, centred in both 0.7e-6, for 4% more time).
+// The products and sum(q) are exact, and the two terms, which can be large
+// against their sum, are added with the rounding of the first one's product kept,
+// so a group's score is rounded relative to itself.  The values' codes are
+// centred, because sums over positive codes would be large against the result of
+// a long, flat softmax and take their rounding with them.
 //
 // A value's code as fp16: a nibble ORed into bits 1 to 4 of 1024.0 is 1024 +
 // 2 c, exactly, and 1039 less is 2 c - 15 (two instructions for two operands);
@@ -299,9 +300,8 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 //          columns 2 t, 2 t + 1 belong to head t and none is idle;
 //   else   eight heads, columns 2 t, 2 t + 1 being heads 2 t, 2 t + 1.
 // Scores: codes as bytes (nibbles of a word are two ANDs and a shift), q as
-// 31-bit whole numbers in four signed bytes: integer products, exact, from which
-// 8 sum(q) is taken before the first rounding.  FEW: two products, columns
-// (byte 0, byte 1) and (byte 2, byte 3); else four, one for each byte.
+// 31-bit whole numbers in four signed bytes: integer products, exact.  FEW: two
+// products, columns (byte 0, byte 1) and (byte 2, byte 3); else four, one for each byte.
 // Output: p d as fp16 hi, lo, turned to the operand's order with movmatrix.
 // FEW: hi and lo are a head's two columns; else two products.
 // On this chip a warp-level MMA keeps the integer and half pipes from issuing
@@ -311,9 +311,8 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 // -> 44.0 us, 128 ragged ones 115.6 -> 84.1; one head (GPT-2, 700 positions) 8.1
 // -> 7.7.  Eight heads would take FEW twice, at 0.73 of the other's time each.
 struct __align__(16) QGroup {  // of a head's q
-    float w;     // factor of the group's whole numbers (a power of two; 1 for the head's largest)
-    float sum;   // their sum, times w
-    int hi, lo;  // -8 times the sums of their upper two bytes (as one number) and of the lower two
+    float w;       // factor of the group's whole numbers (a power of two; 1 for the head's largest)
+    float hi, lo;  // the sums of their upper two bytes, times 2^16, and of the lower two: exact
 };
 template <int NB, bool FEW> struct State {
     static constexpr int HL = FEW ? 1 : 2;  // heads of a lane
@@ -422,8 +421,7 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
             const int hi = __shfl_sync(0xffffffffu, sum[j][0], 8 * t + 4 * hl), lo = __shfl_sync(0xffffffffu, sum[j][1], 8 * t + 4 * hl);
             // (2^-126 for less: below what a score can show)
             const float w = __uint_as_float((uint32_t)max(127 + __shfl_sync(0xffffffffu, ex[j] - top, 8 * t + 4 * hl), 1) << 23);
-            const float all = (fmaf((float)hi, 65536.0f, (float)lo) + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl)) * w;  // (one rounding)
-            const QGroup q = {w, all, -8 * hi, -8 * lo};
+            const QGroup q = {w, 65536.0f * (float)hi + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl), (float)lo};
             if (!S::SH) st.own[S::SH ? 0 : j][hl] = q;
             else if (lane < 4) groups[8 * j + 2 * t + hl] = q;
             st.om[j][hl] = 0.0f;
@@ -517,16 +515,17 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const float2 d = __half22float2(*reinterpret_cast<const __half2 *>(&f[r][j]));
-                const float m = fmaf(8.0f, d.x, d.y);
+                const float d16 = 65536.0f * d.x;
 #pragma unroll
                 for (int hl = 0; hl < HL; hl++) {
-                    // 2^16 upper + lower two bytes' sums, 8 taken off each code: at most 2^23, exact in fp32,
-                    // and 2^24 + 2^16, off by 1 at most
+                    // the sums of the upper and of the lower two bytes: below 2^24, exact in fp32, and below
+                    // 2^25, off by 1 at most
                     const int hi = FEW ? c[0][2 * r] * 256 + c[0][2 * r + 1] : c[0][2 * r + hl] * 256 + c[1][2 * r + hl];
                     const int lo = FEW ? c[1][2 * r] * 256 + c[1][2 * r + 1] : c[S::LP - 2][2 * r + hl] * 256 + c[S::LP - 1][2 * r + hl];
-                    float x = fmaf((float)(hi + qg[hl].hi), 65536.0f, (float)(lo + qg[hl].lo));
-                    if (NG > 1) x *= qg[hl].w;
-                    s[h][r][hl] = fmaf(m, qg[hl].sum, j ? fmaf(d.x, x, s[h][r][hl]) : d.x * x);
+                    // d (q . c) and m sum(q) may cancel: the first one's rounding goes into the low part
+                    const float t = d16 * (float)hi, low = fmaf(d.x, (float)lo, fmaf(d.y, qg[hl].lo, fmaf(d16, (float)hi, -t)));
+                    const float x = fmaf(d.y, qg[hl].hi, t) + low;
+                    s[h][r][hl] = NG == 1 ? x : j ? fmaf(x, qg[hl].w, s[h][r][hl]) : x * qg[hl].w;
                 }
             }
         }

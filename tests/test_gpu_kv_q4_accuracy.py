@@ -183,3 +183,23 @@ def test_maximum_that_rises_in_every_tile(cuda, G, step, late):
             d[3].data_ptr(), 1, G, 1, Dh, S, ws.data_ptr(), wsb, None)
     assert rt.lib().lmc_device_status() == 0
     check(out.cpu().numpy(), q, k[None], vv[None], 8 * 2.0 ** -24 * x.max(), norm=False, least=2.0 ** -126)
+
+
+@pytest.mark.parametrize("G", [1, 4, 5, 8])
+@pytest.mark.parametrize("offset,r", [(100, 1), (100, 100), (100, 1000), (0, 100), (0, 1000)])
+def test_queries_of_unequal_channels_over_keys_of_one_sign(cuda, G, offset, r):
+    """Keys around 100, or from 0 on, that are small in every 16th channel, where q
+    is r times larger: d (q . codes) and m sum(q) are large against the score and
+    cancel.  What is left is of the size of the products q k, as above."""
+    rng = np.random.default_rng(G + r + offset)
+    Dh, n, Hkv = 128, 300, 2
+    big = np.arange(Dh) % 16 == 5
+    k = offset + rng.normal(0, 1, (Hkv, n, Dh)) if offset else np.abs(rng.normal(0, 1, (Hkv, n, Dh)))
+    k[..., big] *= 1.0 / r if offset else 0.0
+    q = rows_of(rng, (Hkv * G, Dh)) * np.where(big, 0.3 * r, 0.3).astype(np.float32)
+    v = rows_of(rng, (Hkv, n, Dh))
+    out, kv, vv = decode(cuda, q, k.astype(np.float32), v)
+    kk, a = np.repeat(np.abs(kv), G, 0), np.abs(q.astype(np.float64))
+    held = sum(2.0 ** -30 * a[:, g:g + 64].max(-1) * kk[:, :, g:g + 64].sum(-1).max(-1) for g in (0, 64))
+    size = np.einsum("hnd,hd->hn", kk, a).max(-1)
+    check(out, q, kv, vv, (held + 8 * 2.0 ** -24 * size) / np.sqrt(Dh))
