@@ -66,11 +66,6 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Limit of a wait for bulk copies (nanoseconds of %globaltimer).
 __device__ long long g_attn_q4_wait_ns = 1000000000ll;
 
-// Head sizes of 224 and 256 with more than four heads: what a lane keeps of its
-// heads' groups lies in shared memory (in registers 192 bytes a thread are
-// spilled at 256 dims; 16 ragged sequences of 8 kv heads, eight query heads
-// each, 52.4 and 43.7 us).
-constexpr bool q4_shared_groups(int NB, bool FEW) { return !FEW && NB > 6; }
 constexpr int q4_tile(int NB) { return NB <= 4 ? 64 : 32; }  // positions per tile (registers and shared memory)
 
 struct Q4Args {
@@ -90,8 +85,7 @@ template <int NB> struct Q4 {
     static constexpr int SIDE = T * RB + 16;              // a tile's K or V rows, from any 4-byte phase
     static constexpr int STAGE = 2 * SIDE;
     static constexpr int FRESH = (2 * RB + 15) / 16 * 16; // the new K and V rows
-    static constexpr int GROUPS = NG * 8 * 16;            // the queries' groups, where they lie in shared memory
-    static constexpr int warp_bytes(bool FEW) { return Q4_STAGES * STAGE + FRESH + (q4_shared_groups(NB, FEW) ? GROUPS : 0); }
+    static constexpr int WARP_BYTES = Q4_STAGES * STAGE + FRESH;
     static constexpr int SLOT = DH + 4;                   // floats of a head's partial result (accumulator, maximum, sum)
     static_assert(Q4_STAGES * STAGE >= 8 * SLOT * 4, "a partial result fits the ring that it is kept in");
 };
@@ -310,23 +304,20 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 // 128 dims, the other form against FEW: one sequence of 131072 positions 57.0
 // -> 44.0 us, 128 ragged ones 115.6 -> 84.1; one head (GPT-2, 700 positions) 8.1
 // -> 7.7.  Eight heads would take FEW twice, at 0.73 of the other's time each.
-struct __align__(16) QGroup {  // of a head's q
+struct QGroup {  // of a head's q
     float w;       // factor of the group's whole numbers (a power of two; 1 for the head's largest)
     float hi, lo;  // the sums of their upper two bytes, times 2^16, and of the lower two: exact
 };
 template <int NB, bool FEW> struct State {
     static constexpr int HL = FEW ? 1 : 2;  // heads of a lane
     static constexpr int LP = FEW ? 2 : 4;  // products of q's bytes
-    static constexpr bool SH = q4_shared_groups(NB, FEW);
     uint32_t q[LP][NB][2];                  // q as matrix operands
-    QGroup own[SH ? 1 : Q4<NB>::NG][HL];    // this lane's heads' groups, or
-    const QGroup *shared;                   // where they lie: [group][8 heads] from this lane's first head on
+    QGroup qg[Q4<NB>::NG][HL];
     float qfac[HL];                         // the factor of the scores
     float2 o[2 * NB][2];                    // dims x this lane's two columns
     float om[Q4<NB>::NG][HL], l[HL];        // this lane's positions: sum p (m + 7.5 d), sum p
     float mx[HL];                           // maximum of s over qfac; p is 2^(s - max)
     float pd[Q4<NB>::NG][HL];               // largest p d so far; o is times 2^(141 - pd_exponent(pd))
-    __device__ __forceinline__ QGroup group(int j, int hl) const { return SH ? shared[8 * j + hl] : own[SH ? 0 : j][hl]; }
 };
 
 __device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -354,7 +345,7 @@ template <int NB, bool FEW> __device__ __forceinline__ int q_head(const Q4Args &
     return FEW ? lane >> 3 : (p.j - p.kh * g.HG) * 8 + (lane >> 2);
 }
 template <int NB, bool FEW>
-__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], State<NB, FEW> &st, QGroup *groups) {
+__device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane, float (&x)[NB][8], State<NB, FEW> &st) {
     using S = State<NB, FEW>;
     const AttnArgs &a = g.a;
     constexpr int DH = Q4<NB>::DH, NG = Q4<NB>::NG;
@@ -421,9 +412,7 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
             const int hi = __shfl_sync(0xffffffffu, sum[j][0], 8 * t + 4 * hl), lo = __shfl_sync(0xffffffffu, sum[j][1], 8 * t + 4 * hl);
             // (2^-126 for less: below what a score can show)
             const float w = __uint_as_float((uint32_t)max(127 + __shfl_sync(0xffffffffu, ex[j] - top, 8 * t + 4 * hl), 1) << 23);
-            const QGroup q = {w, 65536.0f * (float)hi + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl), (float)lo};
-            if (!S::SH) st.own[S::SH ? 0 : j][hl] = q;
-            else if (lane < 4) groups[8 * j + 2 * t + hl] = q;
+            st.qg[j][hl] = {w, 65536.0f * (float)hi + __shfl_sync(0xffffffffu, bad, 8 * t + 4 * hl), (float)lo};
             st.om[j][hl] = 0.0f;
             st.pd[j][hl] = 0.0f;
         }
@@ -432,10 +421,6 @@ __device__ __forceinline__ void load_q(const Q4Args &g, const Item &p, int lane,
     }
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) st.o[i][0] = st.o[i][1] = make_float2(0.0f, 0.0f);
-    if (S::SH) {
-        st.shared = groups + 2 * t;
-        __syncwarp();
-    }
 }
 
 // The new K and V rows quantized into `fresh` (two rows) and, by the first
@@ -502,9 +487,6 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
 #pragma unroll
         for (int j = 0; j < NG; j++) {
             int c[S::LP][4] = {};
-            QGroup qg[HL];
-#pragma unroll
-            for (int hl = 0; hl < HL; hl++) qg[hl] = st.group(j, hl);
 #pragma unroll
             for (int i = 2 * j; i < 2 * j + 2 && i < NB; i++) {
                 const uint32_t w0 = k0[4 * i], w1 = k1[4 * i];
@@ -523,9 +505,9 @@ __device__ __forceinline__ void attend_tile(State<NB, FEW> &st, const uint8_t *k
                     const int hi = FEW ? c[0][2 * r] * 256 + c[0][2 * r + 1] : c[0][2 * r + hl] * 256 + c[1][2 * r + hl];
                     const int lo = FEW ? c[1][2 * r] * 256 + c[1][2 * r + 1] : c[S::LP - 2][2 * r + hl] * 256 + c[S::LP - 1][2 * r + hl];
                     // d (q . c) and m sum(q) may cancel: the first one's rounding goes into the low part
-                    const float t = d16 * (float)hi, low = fmaf(d.x, (float)lo, fmaf(d.y, qg[hl].lo, fmaf(d16, (float)hi, -t)));
-                    const float x = fmaf(d.y, qg[hl].hi, t) + low;
-                    s[h][r][hl] = NG == 1 ? x : j ? fmaf(x, qg[hl].w, s[h][r][hl]) : x * qg[hl].w;
+                    const float t = d16 * (float)hi, low = fmaf(d.x, (float)lo, fmaf(d.y, st.qg[j][hl].lo, fmaf(d16, (float)hi, -t)));
+                    const float x = fmaf(d.y, st.qg[j][hl].hi, t) + low;
+                    s[h][r][hl] = NG == 1 ? x : j ? fmaf(x, st.qg[j][hl].w, s[h][r][hl]) : x * st.qg[j][hl].w;
                 }
             }
         }
@@ -775,9 +757,9 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
     auto cta_of = [&](int unit) { return unit < more * (per + 1) ? unit / (per + 1) : more + (unit - more * (per + 1)) / per; };
     const int cta = blockIdx.x, c0 = cta * per + min(cta, more), cn = per + (cta < more);
     const int wn = cn / Q4_WARPS, wm = cn % Q4_WARPS, u0 = c0 + warp * wn + min(warp, wm), u1 = u0 + wn + (warp < wm);
-    uint8_t *const ring = smem + warp * Q4<NB>::warp_bytes(FEW);
+    uint8_t *const ring = smem + warp * Q4<NB>::WARP_BYTES;
     uint32_t *const fresh = reinterpret_cast<uint32_t *>(ring + Q4_STAGES * Q4<NB>::STAGE);
-    float *const slots = reinterpret_cast<float *>(smem + Q4_WARPS * Q4<NB>::warp_bytes(FEW));  // [warp][GH][SLOT]
+    float *const slots = reinterpret_cast<float *>(smem + Q4_WARPS * Q4<NB>::WARP_BYTES);  // [warp][GH][SLOT]
     const size_t hstride = (size_t)a.nsplit * (DH + 2);
 
     if (u0 < u1) {
@@ -883,7 +865,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
                 float x[NB][8];
                 fetch_q<NB>(g, *ii, lane, q_head<NB, FEW>(g, *ii, lane), x);
                 if (a.append && end == nt) append<NB>(g, *ii, fresh, lane);  // (while q is on its way)
-                load_q<NB, FEW>(g, *ii, lane, x, st, reinterpret_cast<QGroup *>(reinterpret_cast<uint8_t *>(fresh) + Q4<NB>::FRESH));
+                load_q<NB, FEW>(g, *ii, lane, x, st);
                 begin = false;
             }
             if (!g.bulk) {
@@ -960,7 +942,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
             float4 v[PARTS], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int q = 0; q < PARTS; q++) {
-                const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::warp_bytes(FEW)) : slots + (q / 2) * GH * SLOT) + h * SLOT;
+                const float *s = (q % 2 ? reinterpret_cast<const float *>(smem + (q / 2) * Q4<NB>::WARP_BYTES) : slots + (q / 2) * GH * SLOT) + h * SLOT;
                 m[q] = -INFINITY;
                 if ((parts >> q & 1) && !lost) {
                     m[q] = s[DH];
@@ -1078,9 +1060,9 @@ template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a,
 
 template <int NB, bool FEW> int launch(const Q4Args &g, int max_units, cudaStream_t s) {
     const int GH = g.a.H / g.a.Hkv < 8 ? g.a.H / g.a.Hkv : 8;
-    const size_t smem = (size_t)Q4_WARPS * Q4<NB>::warp_bytes(FEW) + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
+    const size_t smem = (size_t)Q4_WARPS * Q4<NB>::WARP_BYTES + (size_t)Q4_WARPS * GH * Q4<NB>::SLOT * sizeof(float);
     // the most that any G takes: threads that call with different ones set the same value
-    constexpr int MOST = Q4_WARPS * Q4<NB>::warp_bytes(FEW) + Q4_WARPS * (FEW ? 4 : 8) * Q4<NB>::SLOT * (int)sizeof(float);
+    constexpr int MOST = Q4_WARPS * Q4<NB>::WARP_BYTES + Q4_WARPS * (FEW ? 4 : 8) * Q4<NB>::SLOT * (int)sizeof(float);
     LMC_CUDA_TRY(cudaFuncSetAttribute((k_attn_q4<NB, FEW>), cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
     const int most = lmc_sm_count() * (smem + 2048 <= 114 * 1024 ? 2 : 1), want = max_units / g.rmin;
     LMC_LAUNCH("attention (4-bit rows)", (k_attn_q4<NB, FEW>), want < 1 ? 1 : want < most ? want : most, 32 * Q4_WARPS, smem, s, g);
