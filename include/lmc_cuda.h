@@ -204,7 +204,8 @@ unsigned long long lmc_rng_seed(unsigned long long seed);
  * NaN gets d = NaN: its values read back as NaN.  Such caches start on a
  * 16-byte boundary and hold at most 2^30 positions a sequence.  Attention over
  * them holds a query's channel to fp32, or to 2^-30 of the largest of its group of
- * 64 where that is more.  For `batch` sequences
+ * 64 where that is more, and a value's weight times d to 22 bits, so an output is
+ * rounded relative to the largest |value| of its group.  For `batch` sequences
  * the caches are batch consecutive [Hkv][S][Dh] slabs and q/k_new/v_new/out
  * are batch rows of H*Dh (q, out) and Hkv*Dh (k_new, v_new) floats.
  * d_pos[b] is the position written this step; positions 0..d_pos[b] are

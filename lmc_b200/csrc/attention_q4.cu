@@ -37,9 +37,9 @@
 // one CTA are merged in shared memory, parts in several CTAs through the
 // workspace by k_q4_combine.
 //
-// Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 44 us, 128 ragged
-// sequences of them 84 us (3.4 and 3.6 TB/s), 64 ragged ones of 4 heads of 64
-// dims 18.8 us, one of 12 heads with 700 positions 7.7 us.  Instructions bound
+// Whole calls: 1 x 131072 positions of 8 kv heads of 128 dims 45 us, 128 ragged
+// sequences of them 85 us (3.4 and 3.6 TB/s), 64 ragged ones of 4 heads of 64
+// dims 19.0 us, one of 12 heads with 700 positions 7.7 us.  Instructions bound
 // the first two (matrix, integer and half instructions share the issue), the
 // latency of a warp's chain (its share, the copies, q, a tile, the merge) the
 // others.
@@ -59,8 +59,8 @@ __device__ int g_attn_q4_err;  // bit 0: a page id outside the pool, bit 1: a wa
 constexpr int Q4_WARPS = 4;
 constexpr int Q4_STAGES = 2;  // tiles in a warp's ring
 // What beginning and ending an item costs, in tiles (q, the new row, the
-// result): 128 ragged sequences of 8 kv heads 91.3, 84.1, 85.9 us with 1, 2, 3;
-// 64 of 4 kv heads, eight query heads each, 19.4, 18.8, 19.4.
+// result): 128 ragged sequences of 8 kv heads 91.8, 85.3, 87.0 us with 1, 2, 3;
+// 64 of 4 kv heads, eight query heads each, 19.5, 19.0, 19.7.
 constexpr int Q4_ITEM = 2;
 constexpr float LOG2E = 1.4426950408889634f;
 // Limit of a wait for bulk copies (nanoseconds of %globaltimer).
@@ -301,9 +301,9 @@ __device__ __forceinline__ void rope8(const AttnArgs &a, int pos, int Dh, int d0
 // On this chip a warp-level MMA keeps the integer and half pipes from issuing
 // (8 cycles each, measured in one loop with them), so their number counts: FEW
 // has 32 for 32 rows of 128 dims, the other form 64.  4 heads per kv head of
-// 128 dims, the other form against FEW: one sequence of 131072 positions 57.0
-// -> 44.0 us, 128 ragged ones 115.6 -> 84.1; one head (GPT-2, 700 positions) 8.1
-// -> 7.7.  Eight heads would take FEW twice, at 0.73 of the other's time each.
+// 128 dims, the other form against FEW: one sequence of 131072 positions 58.0
+// -> 44.7 us, 128 ragged ones 115.1 -> 85.3; one head (GPT-2, 700 positions) 8.2
+// -> 7.7.  Eight heads would take FEW twice, at 0.74 of the other's time each.
 struct QGroup {  // of a head's q
     float w;       // factor of the group's whole numbers (a power of two; 1 for the head's largest)
     float hi, lo;  // the sums of their upper two bytes, times 2^16, and of the lower two: exact
@@ -987,7 +987,7 @@ __global__ void __launch_bounds__(32 * Q4_WARPS, 2) k_attn_q4(const __grid_const
 // workspace; nothing to do when slot 0's sum is zero.  W warps (1 or 4) share
 // a head's parts: four when there are few heads, whose parts are then many
 // (131072 positions of one sequence, 56 parts for each of 32 heads, the whole
-// call: 49.3 us with one, 44.0 with four; 128 sequences of 32 heads 84.2 and 88.1).
+// call: 49.8 us with one, 44.7 with four; 128 sequences of 32 heads 85.3 and 89.2).
 template <int W> __global__ void __launch_bounds__(128) k_q4_combine(AttnArgs a, int batch) {
     pdl_wait();
     pdl_launch_dependents();
@@ -1091,7 +1091,7 @@ static int q4_launch(const AttnArgs *args, int batch, size_t ws_bytes, int lose_
     g.items_only = a.nsplit == 1;
     // an item of NT tiles then lies in at most (NT - 2) / rmin + 2 <= nsplit CTAs;
     // and a CTA has at least an item of one tile (GPT-2, 700 positions, with 1, 3, 6
-    // units a CTA: 8.4, 7.7, 9.3 us; 8 kv heads, 4000 positions: 13.3, 10.8, 11.1)
+    // units a CTA: 8.5, 7.7, 9.3 us; 8 kv heads, 4000 positions: 13.5, 10.8, 11.1)
     g.rmin = g.items_only ? 1 : NT < 2 ? Q4_ITEM + 1 : std::max((NT - 2) / (a.nsplit - 1) + 1, Q4_ITEM + 1);
     g.vec = (((uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.out) & 15) == 0 && a.ldq % 4 == 0 &&
             a.ldkv % 4 == 0 && a.ldo % 4 == 0;
